@@ -3,7 +3,7 @@
 1. ``fused_hoad/libfused_hoad_b200.so`` -- the CUDA kernels and the C ABI of
    ``include/fused_hoad_b200.h``, compiled by nvcc for sm_100a only
    (``-gencode arch=compute_100a,code=sm_100a``), linked against the shared CUDA runtime.
-2. ``fused_hoad/_C*.so`` -- the torch.utils.cpp_extension binding (``csrc/bindings.cpp``),
+2. ``fused_hoad/_C*.so`` -- the torch.utils.cpp_extension binding (``csrc/bindings*.cpp``),
    linked against (1) with an ``$ORIGIN`` rpath so both travel together.
 
 Usage: ``python expanded-gpu-optimization_b200/build.py [--force]``. nvcc cross-compiles, so
@@ -42,7 +42,9 @@ NVCC_FLAGS = [
 CU_SOURCES = [
     "forward_fp32.cu", "forward_tc.cu", "backward_fp32.cu", "backward_tc.cu", "adam.cu",
     "collective.cu", "capi.cu", "noalloc.cu", "biharmonic.cu",
+    "gated_ffn.cu", "residual_norm.cu", "adamw.cu", "capi_blocks.cu",
 ]
+BINDING_SOURCES = ["bindings.cpp", "bindings_blocks.cpp"]
 
 
 def _headers() -> list[Path]:
@@ -88,7 +90,7 @@ def build_native(force: bool = False) -> Path:
 
 def build_binding(force: bool = False) -> Path:
     existing = sorted(PKG.glob("_C*.so"))
-    sources = [CSRC / "bindings.cpp", LIB, *INCLUDE.glob("*.h")]
+    sources = [*(CSRC / name for name in BINDING_SOURCES), LIB, *INCLUDE.glob("*.h")]
     if existing and not force and not _stale(existing[0], sources):
         return existing[0]
     proc = subprocess.run(
@@ -114,7 +116,7 @@ def _setup_binding() -> None:
         ext_modules=[
             CUDAExtension(
                 name="fused_hoad._C",
-                sources=["csrc/bindings.cpp"],
+                sources=[f"csrc/{name}" for name in BINDING_SOURCES],
                 include_dirs=[str(INCLUDE)],
                 library_dirs=[str(PKG)],
                 libraries=["fused_hoad_b200"],

@@ -37,7 +37,7 @@ void check_vector(const torch::Tensor& t, const torch::Tensor& like, int64_t num
                   const char* what) {
   TORCH_CHECK(t.is_cuda() && t.is_contiguous() && t.scalar_type() == torch::kFloat32,
               what, " must be a contiguous float32 CUDA tensor");
-  TORCH_CHECK(t.numel() == numel, what, " must have ", numel, " values");
+  TORCH_CHECK(t.numel() == numel, what, " must have ", std::to_string(numel), " values");
   TORCH_CHECK(t.device() == like.device(), what, " must be on the parameters' device");
 }
 
@@ -372,7 +372,10 @@ int64_t read_device_status(int64_t device) {
   return static_cast<int64_t>(status);
 }
 
+void bind_blocks(pybind11::module& module);  // bindings_blocks.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, module) {
+  bind_blocks(module);
   module.def("fused_forward_laplacian", &fused_forward_laplacian,
              "Fixed MLP forward pass and input Laplacian (CUDA, sm_100a)",
              pybind11::arg("coordinates"), pybind11::arg("parameters"),

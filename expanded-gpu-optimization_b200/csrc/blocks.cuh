@@ -1,0 +1,70 @@
+// Shared pieces of the gated residual trunk's kernels (feed-forward block, norms, AdamW):
+// element types, and the launchers between the kernel files and the C ABI (capi_blocks.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/fused_hoad_b200.h"
+#include "kernels.cuh"
+
+namespace fhb {
+
+using bf16 = __nv_bfloat16;
+
+inline size_t dtype_bytes(int dtype) { return dtype == FHB_DTYPE_F32 ? 4 : 2; }
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(bf16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) {
+  return x;
+}
+template <>
+__device__ __forceinline__ bf16 from_float<bf16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+
+// The block's activation and its derivative at g: tanh, or silu = g sigma(g) with derivative
+// sigma (1 + g (1 - sigma)).
+__device__ __forceinline__ void block_activation(int activation, float g, float& a, float& slope) {
+  if (activation == FHB_ACTIVATION_TANH) {
+    a = tanhf(g);
+    slope = 1.0f - a * a;
+  } else {
+    const float s = 1.0f / (1.0f + expf(-g));
+    a = g * s;
+    slope = s * (1.0f + g * (1.0f - s));
+  }
+}
+#endif
+
+// ---- gated_ffn.cu ----
+size_t ffn_saved_bytes(const fhb_ffn_problem& p);
+size_t ffn_workspace_bytes(const fhb_ffn_problem& p, bool backward, const DeviceInfo& dev);
+cudaError_t launch_ffn_forward(const fhb_ffn_problem& p, void* y, void* saved, void* workspace,
+                               const DeviceInfo& dev, cudaStream_t stream);
+cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, int64_t grad_y_stride,
+                                const void* saved, const fhb_ffn_grads& grads, void* workspace,
+                                const DeviceInfo& dev, cudaStream_t stream);
+
+// ---- residual_norm.cu ----
+cudaError_t launch_residual_norm(const fhb_norm_problem& p, void* total, void* normed,
+                                 float* stats, const DeviceInfo& dev, cudaStream_t stream);
+size_t residual_norm_workspace_bytes(const fhb_norm_problem& p, const DeviceInfo& dev);
+cudaError_t launch_residual_norm_backward(const fhb_norm_problem& p, const void* grad_total,
+                                          int64_t grad_total_stride, const void* grad_normed,
+                                          int64_t grad_normed_stride, const float* stats,
+                                          const fhb_norm_grads& grads, void* workspace,
+                                          const DeviceInfo& dev, cudaStream_t stream);
+
+// ---- adamw.cu ----
+cudaError_t launch_adamw(const fhb_adamw_tensor* tensors, int64_t n_tensors, int state_bits,
+                         int64_t* step, double lr, double beta1, double beta2, double eps,
+                         double weight_decay, cudaStream_t stream);
+
+}  // namespace fhb

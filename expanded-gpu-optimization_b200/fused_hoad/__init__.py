@@ -18,7 +18,9 @@ from fused_hoad._extension import (
 )
 from fused_hoad.backends import BACKENDS, FIXED_CONTRACT_BACKENDS, get_backend
 from fused_hoad.backends.fused import FusedForwardLaplacian, fused_laplacian
+from fused_hoad.blocks import GatedResidualTrunk, gated_feed_forward, residual_norm, rms_norm
 from fused_hoad.distributed import PeerExchange, shard_range
+from fused_hoad.optim import AdamW, adamw_step, decode_states
 from fused_hoad.parameters import (
     POISSON_PARAMETER_COUNT,
     POISSON_PARAMETER_LAYOUT,
@@ -37,30 +39,37 @@ from fused_hoad.problem import (
 from fused_hoad.training import PoissonTrainer, cuda_graph_step
 
 __all__ = [
+    "AdamW",
     "BACKENDS",
     "DEFAULT_POISSON_MLP",
     "FIXED_CONTRACT_BACKENDS",
     "FusedForwardLaplacian",
+    "GatedResidualTrunk",
     "MLPConfig",
     "POISSON_PARAMETER_COUNT",
     "POISSON_PARAMETER_LAYOUT",
     "PeerExchange",
     "PoissonTrainer",
+    "adamw_step",
     "bind_model_to_flat",
     "build_mlp",
     "cuda_graph_step",
+    "decode_states",
     "extension_available",
     "fused_forward_biharmonic",
     "fused_forward_laplacian",
     "fused_forward_laplacian_backward",
     "fused_forward_laplacian_host",
     "fused_laplacian",
+    "gated_feed_forward",
     "get_backend",
     "load_extension",
     "manufactured_solution",
     "manufactured_source",
     "pack_poisson_parameters",
     "read_device_status",
+    "residual_norm",
+    "rms_norm",
     "shard_range",
     "uniform_points",
     "unpack_poisson_parameters",

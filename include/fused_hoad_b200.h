@@ -294,6 +294,120 @@ int fhb_train_step(const float* coords, int64_t n, int64_t n_total, const float*
                    float* grad_out, float* loss_out, int version, int activation,
                    void* workspace, size_t workspace_bytes, fhb_stream_t stream);
 
+/*
+ * ---- Gated residual trunks: feed-forward block, norms, optimizer ----
+ * The operators of deep gated residual networks, next to the fixed MLP above: no counterpart
+ * in the reference. Tensors are row-major with unit stride in the last dimension; strides are
+ * in elements between rows. Types: FHB_DTYPE_F32 and FHB_DTYPE_BF16; products, sums, norms and
+ * states are held in 32 bits whatever the type, and rounded once on output unless stated.
+ */
+#define FHB_DTYPE_F32 0
+#define FHB_DTYPE_BF16 1
+
+/*
+ * A gated feed-forward block on `tokens` rows of `width` values:
+ *     g = x w_gate^T + b_gate,  u = x w_up^T + b_up,  h = act(g) * u,  y = h w_down^T + b_down
+ * with x [tokens][width], w_gate, w_up [hidden][width], w_down [out_width][hidden], biases
+ * [hidden], [hidden], [out_width] (each may be NULL), act tanh or silu (FHB_ACTIVATION_*).
+ * All tensors have type `dtype`. h is rounded to `dtype` between the two products (as are the
+ * gradients of g and u in the backward): they are operands of a product of that type.
+ */
+typedef struct fhb_ffn_problem {
+  int64_t tokens, width, hidden, out_width;
+  int dtype, activation;
+  const void *x, *w_gate, *w_up, *w_down;
+  int64_t x_stride, w_gate_stride, w_up_stride, w_down_stride;
+  const void *b_gate, *b_up, *b_down;
+} fhb_ffn_problem;
+/* Where the backward writes; each may be NULL (not computed). All contiguous, type `dtype`. */
+typedef struct fhb_ffn_grads {
+  void *x, *w_gate, *w_up, *w_down, *b_gate, *b_up, *b_down;
+} fhb_ffn_grads;
+/* Bytes of the buffer in which the forward keeps what the backward needs (opaque). */
+size_t fhb_ffn_saved_bytes(const fhb_ffn_problem* problem);
+/* Workspace of the forward (backward == 0) or the backward call on the current device. */
+size_t fhb_ffn_workspace_bytes(const fhb_ffn_problem* problem, int backward);
+/*
+ * y [tokens][out_width], contiguous. `saved` (fhb_ffn_saved_bytes bytes, 16-byte aligned) is
+ * filled for fhb_ffn_backward, or NULL where no gradient is wanted. Workspace 16-byte aligned.
+ * tokens == 0 is a no-op.
+ */
+int fhb_ffn_forward(const fhb_ffn_problem* problem, void* y, void* saved, void* workspace,
+                    size_t workspace_bytes, fhb_stream_t stream);
+/*
+ * Gradients for grad_y [tokens][out_width] (row stride grad_y_stride), from the forward's
+ * `saved`. Sums run in a fixed order: results are bitwise reproducible for given sizes and
+ * device. tokens == 0 writes zeros to the weights' and biases' gradients.
+ */
+int fhb_ffn_backward(const fhb_ffn_problem* problem, const void* grad_y, int64_t grad_y_stride,
+                     const void* saved, const fhb_ffn_grads* grads, void* workspace,
+                     size_t workspace_bytes, fhb_stream_t stream);
+
+/*
+ * The RMS norms before and after a block with its gate and residual scale, in one pass:
+ *     z = rms(branch) * post_weight   (z = branch where post_weight is NULL)
+ *     total = scale * residual + gate * z,   normed = rms(total) * pre_weight
+ * with rms(v) = v / sqrt(mean(v^2) + eps) over the row's `width` values: the residual stream
+ * after one block and the next block's input. residual and total have type residual_dtype,
+ * everything else `dtype`. branch may be NULL: total = scale * residual (then gate and
+ * post_weight are NULL too). gate (NULL: 1) has one contiguous row of `width` values for every
+ * gate_rows consecutive rows (`rows` of them share row 0 of a per-channel gate; 1: a full one).
+ * scale is *residual_scale_ptr (device, float) where that is given, else residual_scale.
+ */
+typedef struct fhb_norm_problem {
+  int64_t rows, width;
+  int residual_dtype, dtype;
+  const void *residual, *branch, *pre_weight, *post_weight, *gate;
+  int64_t residual_stride, branch_stride, gate_rows;
+  const float* residual_scale_ptr;
+  float residual_scale, eps;
+} fhb_norm_problem;
+/* Where the backward writes; each may be NULL. Row tensors contiguous; gate [groups][width],
+ * groups = ceil(rows / gate_rows); residual_scale one float. */
+typedef struct fhb_norm_grads {
+  void *residual, *branch, *pre_weight, *post_weight, *gate;
+  float* residual_scale;
+} fhb_norm_grads;
+/* total (may be NULL) and normed [rows][width] contiguous; stats (NULL, or 2 * rows floats)
+ * receives what the backward needs: 1 / rms of branch and total per row. rows == 0: no-op. */
+int fhb_residual_norm(const fhb_norm_problem* problem, void* total, void* normed, float* stats,
+                      fhb_stream_t stream);
+size_t fhb_residual_norm_workspace_bytes(const fhb_norm_problem* problem);
+/* grad_total and grad_normed (row strides given; each may be NULL: zeros) to the gradients, in
+ * a fixed order of sums (bitwise reproducible). rows == 0 zeroes the weights' gradients. */
+int fhb_residual_norm_backward(const fhb_norm_problem* problem, const void* grad_total,
+                               int64_t grad_total_stride, const void* grad_normed,
+                               int64_t grad_normed_stride, const float* stats,
+                               const fhb_norm_grads* grads, void* workspace,
+                               size_t workspace_bytes, fhb_stream_t stream);
+
+/*
+ * One AdamW step (decoupled weight decay) over many tensors, torch.optim.AdamW semantics:
+ *     p *= 1 - lr weight_decay;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *     p -= lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * `tensors` is a HOST array (read during the call). param and grad have type dtype, each
+ * tensor its own. state_bits 32: exp_avg and exp_avg_sq are float. state_bits 8: they hold
+ * e4m3 codes (one byte) of m and of sqrt(v), with one float scale for every block of
+ * FHB_ADAMW_BLOCK consecutive values (the last block may be short):
+ *     scale = max(max|value| * (1/448), 2^-126),  code = e4m3(value / scale), nearest even;
+ * a sqrt(v) that is not zero takes at least the smallest code, 2^-9. The update uses m and v
+ * before they are coded. A block with a NaN or infinite value decodes to NaN throughout.
+ * `step` is a device int64 counter of the steps taken so far, read (t = step + 1) and then
+ * advanced on the stream, so the call can be replayed from a CUDA graph.
+ */
+#define FHB_ADAMW_BLOCK 256
+typedef struct fhb_adamw_tensor {
+  void* param;
+  const void* grad;
+  void *exp_avg, *exp_avg_sq;
+  float *exp_avg_scale, *exp_avg_sq_scale; /* state_bits 8 only */
+  int64_t count;
+  int dtype;
+} fhb_adamw_tensor;
+int fhb_adamw_step(const fhb_adamw_tensor* tensors, int64_t n_tensors, int state_bits,
+                   int64_t* step, double lr, double beta1, double beta2, double eps,
+                   double weight_decay, fhb_stream_t stream);
+
 /* Reads and clears the status word of `device` (synchronises that device). */
 int fhb_read_device_status(int device, unsigned int* status_out);
 
