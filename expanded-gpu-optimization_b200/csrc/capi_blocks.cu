@@ -6,8 +6,9 @@
 
 namespace {
 
-constexpr int64_t kMaxRows = int64_t{1} << 31;    // rows of an activation
+constexpr int64_t kMaxRows = int64_t{1} << 30;    // rows of an activation
 constexpr int64_t kMaxColumns = int64_t{1} << 22;  // values of a row
+constexpr uintptr_t kRoomAlignment = 128;         // of workspaces and saved buffers
 constexpr int64_t kMaxCount = int64_t{1} << 40;   // values of a tensor
 
 bool valid_dtype(int dtype) { return dtype == FHB_DTYPE_F32 || dtype == FHB_DTYPE_BF16; }
@@ -30,7 +31,7 @@ int check_vector(const void* p, int dtype, bool required) {
 int check_workspace(const void* workspace, size_t bytes, size_t need) {
   if (need == 0) return FHB_OK;
   if (workspace == nullptr || bytes < need) return FHB_ERR_WORKSPACE;
-  return aligned(workspace, 16) ? FHB_OK : FHB_ERR_MISALIGNED;
+  return aligned(workspace, kRoomAlignment) ? FHB_OK : FHB_ERR_MISALIGNED;
 }
 
 // The first code that is not FHB_OK.
@@ -47,7 +48,9 @@ int check_ffn_sizes(const fhb_ffn_problem* p) {
       p->tokens < 0 || p->width < 1 || p->hidden < 1 || p->out_width < 1)
     return FHB_ERR_INVALID_ARGUMENT;
   if (p->tokens > kMaxRows || p->width > kMaxColumns || p->hidden > kMaxColumns ||
-      p->out_width > kMaxColumns || p->tokens * p->hidden > kMaxCount)
+      p->out_width > kMaxColumns || p->tokens * p->hidden > kMaxCount ||
+      p->tokens * p->width > kMaxCount || p->tokens * p->out_width > kMaxCount ||
+      p->hidden * p->width > kMaxCount || p->hidden * p->out_width > kMaxCount)
     return FHB_ERR_TOO_LARGE;
   return FHB_OK;
 }
@@ -102,7 +105,7 @@ int fhb_ffn_forward(const fhb_ffn_problem* problem, void* y, void* saved, void* 
   if (problem->tokens == 0) return FHB_OK;
   code = check_vector(y, problem->dtype, true);
   if (code != FHB_OK) return code;
-  if (!aligned(saved, 16)) return FHB_ERR_MISALIGNED;
+  if (!aligned(saved, kRoomAlignment)) return FHB_ERR_MISALIGNED;
   const fhb::DeviceInfo* dev = nullptr;
   code = fhb::current_device_info(&dev);
   if (code != FHB_OK) return code;
@@ -127,7 +130,7 @@ int fhb_ffn_backward(const fhb_ffn_problem* problem, const void* grad_y, int64_t
       check_vector(grads->b_down, dtype, false));
   if (code != FHB_OK) return code;
   if (problem->tokens > 0 && saved == nullptr) return FHB_ERR_INVALID_ARGUMENT;
-  if (!aligned(saved, 16)) return FHB_ERR_MISALIGNED;
+  if (!aligned(saved, kRoomAlignment)) return FHB_ERR_MISALIGNED;
   const fhb::DeviceInfo* dev = nullptr;
   code = fhb::current_device_info(&dev);
   if (code != FHB_OK) return code;

@@ -2,208 +2,314 @@
 // y = h Wd^T + bd, and its gradients
 //     dh = dy Wd,  du = dh act(g),  dg = dh u act'(g),
 //     dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h,  db = column sums.
-#include "blocks.cuh"
+//
+// Two products forward (both projections, the activation and the gate in the first), four
+// backward (dg and du in the first; dx as one sum over both weights; dWg and dWu in one launch),
+// on the tensor cores (gemm_tc.cu).
+#include <algorithm>
+
+#include "gemm_tc.cuh"
 
 namespace fhb {
 namespace {
 
-// C[m][n] = sum over terms t, k of A_t(m, k) B_t(n, k) + bias[n], operands with any strides,
-// FP32 sums. One 64 x 64 tile per CTA, 16 of K at a time, 4 x 4 results per thread.
-constexpr int kTile = 64, kStep = 16;
+int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
-template <typename T>
-struct Operand {
-  const T* p;
-  int64_t mn, k;  // strides along the result's dimension and along K
-};
-template <typename T>
-struct Product {
-  Operand<T> a[2], b[2];
-  int terms;
-  int64_t m, n, k;
-  const T* bias;
+// Pieces of one buffer, 128-byte aligned; without a buffer it only counts.
+struct Room {
+  char* base;
+  size_t used = 0;
+  void* take(size_t bytes) {
+    void* p = base != nullptr ? base + used : nullptr;
+    used += static_cast<size_t>(round_up(static_cast<int64_t>(bytes), 128));
+    return p;
+  }
 };
 
-template <typename T, typename TC>
-__global__ void __launch_bounds__(256)
-    gemm_kernel(Product<T> p, TC* __restrict__ c, int64_t c_stride) {
-  __shared__ float as[kStep][kTile + 4], bs[kStep][kTile + 4];
-  const int64_t tiles_n = (p.n + kTile - 1) / kTile;
-  const int64_t m0 = (blockIdx.x / tiles_n) * kTile, n0 = (blockIdx.x % tiles_n) * kTile;
-  const int tm = (threadIdx.x / 16) * 4, tn = (threadIdx.x % 16) * 4;
-  float acc[4][4] = {};
-  for (int t = 0; t < p.terms; ++t) {
-    const Operand<T> a = p.a[t], b = p.b[t];
-    for (int64_t k0 = 0; k0 < p.k; k0 += kStep) {
-      for (int i = threadIdx.x; i < kTile * kStep; i += 256) {
-        // consecutive threads follow the operand's unit stride
-        const int am = a.k == 1 ? i / kStep : i % kTile, ak = a.k == 1 ? i % kStep : i / kTile;
-        const int bn = b.k == 1 ? i / kStep : i % kTile, bk = b.k == 1 ? i % kStep : i / kTile;
-        as[ak][am] = m0 + am < p.m && k0 + ak < p.k
-                         ? to_float(a.p[(m0 + am) * a.mn + (k0 + ak) * a.k]) : 0.0f;
-        bs[bk][bn] = n0 + bn < p.n && k0 + bk < p.k
-                         ? to_float(b.p[(n0 + bn) * b.mn + (k0 + bk) * b.k]) : 0.0f;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int kk = 0; kk < kStep; ++kk)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(as[kk][tm + i], bs[kk][tn + j], acc[i][j]);
-      __syncthreads();
-    }
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t row = m0 + tm + i, col = n0 + tn + j;
-      if (row >= p.m || col >= p.n) continue;
-      const float v = acc[i][j] + (p.bias != nullptr ? to_float(p.bias[col]) : 0.0f);
-      c[row * c_stride + col] = from_float<TC>(v);
-    }
-}
-
-template <typename T, typename TC>
-cudaError_t gemm(const Product<T>& p, TC* c, int64_t c_stride, cudaStream_t stream) {
-  const int64_t tiles = ((p.m + kTile - 1) / kTile) * ((p.n + kTile - 1) / kTile);
-  if (tiles == 0) return cudaSuccess;
-  if (tiles > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  gemm_kernel<<<static_cast<unsigned>(tiles), 256, 0, stream>>>(p, c, c_stride);
-  return cudaGetLastError();
-}
-
-template <typename T>
-__global__ void gate_kernel(const float* __restrict__ g, const float* __restrict__ u,
-                            T* __restrict__ h, int64_t count, int activation) {
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < count; i += gridDim.x * 256ll) {
-    float a, slope;
-    block_activation(activation, g[i], a, slope);
-    h[i] = from_float<T>(a * u[i]);
-  }
-}
-
-template <typename T>
-__global__ void gate_backward_kernel(const float* __restrict__ dh, const float* __restrict__ g,
-                                     const float* __restrict__ u, T* __restrict__ dg,
-                                     T* __restrict__ du, int64_t count, int activation) {
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < count; i += gridDim.x * 256ll) {
-    float a, slope;
-    block_activation(activation, g[i], a, slope);
-    du[i] = from_float<T>(dh[i] * a);
-    dg[i] = from_float<T>(dh[i] * u[i] * slope);
-  }
-}
-
-// out[c] = sum over rows of in[r][c], in row order.
-template <typename T>
-__global__ void column_sum_kernel(const T* __restrict__ in, int64_t stride, int64_t rows,
-                                  int64_t columns, T* __restrict__ out) {
-  const int64_t c = blockIdx.x * 64ll + threadIdx.x;
-  if (c >= columns) return;
-  float s = 0.0f;
-  for (int64_t r = 0; r < rows; ++r) s += to_float(in[r * stride + c]);
-  out[c] = from_float<T>(s);
-}
-
-template <typename T>
-void column_sum(const T* in, int64_t stride, int64_t rows, int64_t columns, void* out,
-                cudaStream_t stream) {
-  if (out != nullptr)
-    column_sum_kernel<<<static_cast<unsigned>((columns + 63) / 64), 64, 0, stream>>>(
-        in, stride, rows, columns, static_cast<T*>(out));
-}
-
-int64_t round16(int64_t bytes) { return (bytes + 15) & ~int64_t{15}; }
-
-// Saved for the backward: g and u in FP32, h in the block's type.
+// What the forward keeps: h in operand form and the activation's factors.
 struct Saved {
-  float *g, *u;
-  void* h;
+  TcMatrix h;
+  TcFactors factors;
 };
-Saved saved_at(const fhb_ffn_problem& p, void* base) {
-  char* c = static_cast<char*>(base);
-  const int64_t wide = round16(p.tokens * p.hidden * 4);
-  return {reinterpret_cast<float*>(c), reinterpret_cast<float*>(c + wide), c + 2 * wide};
+Saved saved_in(const fhb_ffn_problem& p, Room& room) {
+  Saved s;
+  s.h = tc_result(room.take(tc_result_bytes(p.tokens, p.hidden, p.dtype)), p.tokens, p.hidden, p.dtype);
+  s.factors = tc_factors(room.take(tc_factor_bytes(p.tokens, p.hidden, p.dtype)), p.tokens, p.hidden, p.dtype);
+  return s;
+}
+
+// ---- column sums (the biases' gradients) ----
+// Rows of one part: 512, more where there would be over 2,048 parts.
+int64_t part_rows_of(int64_t rows) { return std::max<int64_t>(512, (rows + 2047) / 2048); }
+struct ColumnSource {
+  const void* p;  // T, or a TcMatrix's planes
+  int64_t stride, plane, columns;
+  bool operand;
+  void* out;
+};
+struct ColumnSources {
+  ColumnSource source[3];
+  int64_t rows, part_rows, widest;
+  float* parts;  // [source][part][widest]
+  int64_t part_count;
+};
+
+// One part: 64 columns, its rows over 8 warps, then the warps' sums in order.
+template <typename T>
+__global__ void __launch_bounds__(256) column_parts_kernel(ColumnSources s) {
+  const ColumnSource& src = s.source[blockIdx.z];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t c0 = blockIdx.x * 64ll;
+  if (c0 >= src.columns) return;
+  const int64_t first = blockIdx.y * s.part_rows;
+  const int64_t last = min(first + s.part_rows, s.rows);
+  float sum[2] = {};
+  for (int64_t r = first + warp; r < last; r += 8)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int64_t c = c0 + lane + 32 * j, at = r * src.stride + c;
+      if (c >= src.columns) continue;
+      if (src.operand) {
+        const bf16* p = static_cast<const bf16*>(src.p) + at;
+        float v = to_float(p[0]);
+        if (sizeof(T) == 4) v += to_float(p[src.plane]) + to_float(p[2 * src.plane]);
+        sum[j] += v;
+      } else {
+        sum[j] += to_float(static_cast<const T*>(src.p)[at]);
+      }
+    }
+  __shared__ float by_warp[8][64];
+  by_warp[warp][lane] = sum[0];
+  by_warp[warp][lane + 32] = sum[1];
+  __syncthreads();
+  if (threadIdx.x < 64 && c0 + threadIdx.x < src.columns) {
+    float total = 0.0f;
+    for (int w = 0; w < 8; ++w) total += by_warp[w][threadIdx.x];
+    s.parts[(blockIdx.z * s.part_count + blockIdx.y) * s.widest + c0 + threadIdx.x] = total;
+  }
 }
 
 template <typename T>
-cudaError_t forward(const fhb_ffn_problem& p, void* y, void* saved, void* workspace,
-                    cudaStream_t stream) {
-  const Saved s = saved_at(p, saved != nullptr ? saved : workspace);
-  const int64_t t = p.tokens, d = p.width, h = p.hidden, o = p.out_width;
-  const Operand<T> x{static_cast<const T*>(p.x), p.x_stride, 1};
-  const Operand<T> wg{static_cast<const T*>(p.w_gate), p.w_gate_stride, 1};
-  const Operand<T> wu{static_cast<const T*>(p.w_up), p.w_up_stride, 1};
-  const Operand<T> wd{static_cast<const T*>(p.w_down), p.w_down_stride, 1};
-  const Operand<T> hidden{static_cast<const T*>(s.h), h, 1};
-  cudaError_t e = gemm(Product<T>{{x}, {wg}, 1, t, h, d, static_cast<const T*>(p.b_gate)}, s.g, h, stream);
-  if (e == cudaSuccess)
-    e = gemm(Product<T>{{x}, {wu}, 1, t, h, d, static_cast<const T*>(p.b_up)}, s.u, h, stream);
-  if (e != cudaSuccess) return e;
-  gate_kernel<<<1184, 256, 0, stream>>>(s.g, s.u, static_cast<T*>(s.h), t * h, p.activation);
-  return gemm(Product<T>{{hidden}, {wd}, 1, t, o, h, static_cast<const T*>(p.b_down)},
-              static_cast<T*>(y), o, stream);
+__global__ void __launch_bounds__(64) column_totals_kernel(ColumnSources s) {
+  const ColumnSource& src = s.source[blockIdx.y];
+  const int64_t c = blockIdx.x * 64ll + threadIdx.x;
+  if (c >= src.columns) return;
+  float total = 0.0f;
+  for (int64_t part = 0; part < s.part_count; ++part)
+    total += s.parts[(blockIdx.y * s.part_count + part) * s.widest + c];
+  static_cast<T*>(src.out)[c] = from_float<T>(total);
 }
 
 template <typename T>
-cudaError_t backward(const fhb_ffn_problem& p, const T* dy, int64_t dy_stride, const void* saved,
-                     const fhb_ffn_grads& out, void* workspace, cudaStream_t stream) {
-  const Saved s = saved_at(p, const_cast<void*>(saved));
-  const int64_t t = p.tokens, d = p.width, h = p.hidden, o = p.out_width;
-  const int64_t wide = round16(t * h * 4), narrow = round16(t * h * sizeof(T));
-  char* ws = static_cast<char*>(workspace);
-  float* dh = reinterpret_cast<float*>(ws);
-  T* dg = reinterpret_cast<T*>(ws + wide);
-  T* du = reinterpret_cast<T*>(ws + wide + narrow);
-  const T* x = static_cast<const T*>(p.x);
-  const T *wg = static_cast<const T*>(p.w_gate), *wu = static_cast<const T*>(p.w_up);
-  cudaError_t e = gemm(Product<T>{{{dy, dy_stride, 1}},
-                                  {{static_cast<const T*>(p.w_down), 1, p.w_down_stride}}, 1, t, h, o},
-                       dh, h, stream);
-  if (e != cudaSuccess) return e;
-  if (t > 0)
-    gate_backward_kernel<<<1184, 256, 0, stream>>>(dh, s.g, s.u, dg, du, t * h, p.activation);
-  if (out.x != nullptr)
-    e = gemm(Product<T>{{{dg, h, 1}, {du, h, 1}}, {{wg, 1, p.w_gate_stride}, {wu, 1, p.w_up_stride}},
-                        2, t, d, h},
-             static_cast<T*>(out.x), d, stream);
-  if (e == cudaSuccess && out.w_gate != nullptr)
-    e = gemm(Product<T>{{{dg, 1, h}}, {{x, 1, p.x_stride}}, 1, h, d, t}, static_cast<T*>(out.w_gate), d, stream);
-  if (e == cudaSuccess && out.w_up != nullptr)
-    e = gemm(Product<T>{{{du, 1, h}}, {{x, 1, p.x_stride}}, 1, h, d, t}, static_cast<T*>(out.w_up), d, stream);
-  if (e == cudaSuccess && out.w_down != nullptr)
-    e = gemm(Product<T>{{{dy, 1, dy_stride}}, {{static_cast<const T*>(s.h), 1, h}}, 1, o, h, t},
-             static_cast<T*>(out.w_down), h, stream);
-  if (e != cudaSuccess) return e;
-  column_sum(dg, h, t, h, out.b_gate, stream);
-  column_sum(du, h, t, h, out.b_up, stream);
-  column_sum(dy, dy_stride, t, o, out.b_down, stream);
+cudaError_t column_sums(ColumnSources& s, int count, cudaStream_t stream) {
+  if (count == 0) return cudaSuccess;
+  const unsigned columns = static_cast<unsigned>((s.widest + 63) / 64);
+  column_parts_kernel<T><<<dim3(columns, static_cast<unsigned>(s.part_count), count), 256, 0, stream>>>(s);
+  column_totals_kernel<T><<<dim3(columns, count), 64, 0, stream>>>(s);
   return cudaGetLastError();
+}
+
+// ---- the products ----
+struct Operands {
+  TcMatrix x, w_gate, w_up, w_down, dy;
+};
+
+// Operand forms of the inputs, copied into `room` where they have to be (and where it is real).
+cudaError_t operands_in(const fhb_ffn_problem& p, const void* dy, int64_t dy_stride, Room& room,
+                        Operands& o, cudaStream_t stream) {
+  struct {
+    const void* p;
+    int64_t rows, cols, stride;
+    TcMatrix* out;
+  } const inputs[] = {{p.x, p.tokens, p.width, p.x_stride, &o.x},
+                      {p.w_gate, p.hidden, p.width, p.w_gate_stride, &o.w_gate},
+                      {p.w_up, p.hidden, p.width, p.w_up_stride, &o.w_up},
+                      {p.w_down, p.out_width, p.hidden, p.w_down_stride, &o.w_down},
+                      {dy, p.tokens, p.out_width, dy_stride, &o.dy}};
+  for (const auto& in : inputs) {
+    if (in.p == nullptr) continue;
+    void* place = room.take(tc_operand_bytes(in.p, in.rows, in.cols, in.stride, p.dtype));
+    if (room.base == nullptr) {
+      *in.out = tc_result(nullptr, in.rows, in.cols, p.dtype);
+      continue;
+    }
+    const cudaError_t e = tc_operand(in.p, in.rows, in.cols, in.stride, p.dtype, place, in.out, stream);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+TcProduct gate_product(const fhb_ffn_problem& p, const Operands& o, const Saved& s, bool keep) {
+  TcProduct q;
+  q.m = p.tokens, q.n = p.hidden, q.k = p.width;
+  q.a[0] = o.x, q.b[0] = o.w_gate, q.b[1] = o.w_up;
+  q.epilogue = TcEpilogue::kGate;
+  q.dtype = p.dtype;
+  q.bias[0] = p.b_gate, q.bias[1] = p.b_up;
+  q.gated[0] = s.h;
+  if (keep) q.factors = s.factors;
+  q.activation = p.activation;
+  return q;
+}
+
+TcProduct store_product(const fhb_ffn_problem& p, int64_t m, int64_t n, int64_t k, void* out) {
+  TcProduct q;
+  q.m = m, q.n = n, q.k = k;
+  q.dtype = p.dtype;
+  q.out[0] = out;
+  q.out_stride = n;
+  return q;
+}
+
+TcProduct down_product(const fhb_ffn_problem& p, const Operands& o, const Saved& s, void* y) {
+  TcProduct q = store_product(p, p.tokens, p.out_width, p.hidden, y);
+  q.a[0] = s.h, q.b[0] = o.w_down;
+  q.bias[0] = p.b_down;
+  return q;
+}
+
+struct Backward {
+  TcMatrix dg, du;
+  TcProduct hidden, x, weights, down;
+  bool want_x, want_weights, want_down;
+};
+Backward backward_of(const fhb_ffn_problem& p, const Operands& o, const Saved& s,
+                     const fhb_ffn_grads& out, Room& room) {
+  Backward b;
+  const size_t bytes = tc_result_bytes(p.tokens, p.hidden, p.dtype);
+  b.dg = tc_result(room.take(bytes), p.tokens, p.hidden, p.dtype);
+  b.du = tc_result(room.take(bytes), p.tokens, p.hidden, p.dtype);
+  b.hidden = store_product(p, p.tokens, p.hidden, p.out_width, nullptr);
+  b.hidden.a[0] = o.dy, b.hidden.b[0] = o.w_down;
+  b.hidden.b_k_major = false;
+  b.hidden.epilogue = TcEpilogue::kGateGrad;
+  b.hidden.gated[0] = b.dg, b.hidden.gated[1] = b.du;
+  b.hidden.factors = s.factors;
+  b.want_x = out.x != nullptr;
+  b.x = store_product(p, p.tokens, p.width, p.hidden, out.x);
+  b.x.a[0] = b.dg, b.x.a[1] = b.du, b.x.b[0] = o.w_gate, b.x.b[1] = o.w_up;
+  b.x.b_k_major = false;
+  b.x.sum_terms = 2;
+  b.want_weights = out.w_gate != nullptr || out.w_up != nullptr;
+  const bool both = out.w_gate != nullptr && out.w_up != nullptr;
+  b.weights = store_product(p, p.hidden, p.width, p.tokens, both || out.w_up == nullptr ? out.w_gate : out.w_up);
+  b.weights.a[0] = both || out.w_up == nullptr ? b.dg : b.du;
+  if (both) b.weights.a[1] = b.du, b.weights.out[1] = out.w_up;
+  b.weights.groups = both ? 2 : 1;
+  b.weights.b[0] = o.x;
+  b.weights.a_k_major = b.weights.b_k_major = false;
+  b.want_down = out.w_down != nullptr;
+  b.down = store_product(p, p.out_width, p.hidden, p.tokens, out.w_down);
+  b.down.a[0] = o.dy, b.down.b[0] = s.h;
+  b.down.a_k_major = b.down.b_k_major = false;
+  return b;
+}
+
+// Stands for "every gradient wanted" where sizes are asked for before the outputs exist.
+fhb_ffn_grads all_grads(const fhb_ffn_problem& p) {
+  static char any;
+  return {&any, &any, &any, &any, &any, &any, &any};
+}
+
+int64_t column_part_count(const fhb_ffn_problem& p) {
+  const int64_t rows = part_rows_of(p.tokens);
+  return (p.tokens + rows - 1) / rows;
 }
 
 }  // namespace
 
 size_t ffn_saved_bytes(const fhb_ffn_problem& p) {
-  return 2 * round16(p.tokens * p.hidden * 4) + round16(p.tokens * p.hidden * dtype_bytes(p.dtype));
+  Room room{nullptr};
+  saved_in(p, room);
+  return room.used;
 }
 
-size_t ffn_workspace_bytes(const fhb_ffn_problem& p, bool backward, const DeviceInfo&) {
-  if (!backward) return ffn_saved_bytes(p);
-  return round16(p.tokens * p.hidden * 4) + 2 * round16(p.tokens * p.hidden * dtype_bytes(p.dtype));
+size_t ffn_workspace_bytes(const fhb_ffn_problem& p, bool backward, const DeviceInfo& dev) {
+  Room room{nullptr};
+  Operands o;
+  if (p.tokens == 0) return 0;
+  if (!backward) {
+    operands_in(p, nullptr, 0, room, o, nullptr);
+    const Saved s = saved_in(p, room);
+    const size_t parts = gemm_tc_workspace_bytes(down_product(p, o, s, nullptr), dev);
+    room.take(parts);
+    return room.used;
+  }
+  // the upstream gradient may need a copy: the size asked for does not depend on it
+  operands_in(p, nullptr, 0, room, o, nullptr);
+  room.take(tc_result_bytes(p.tokens, p.out_width, p.dtype));
+  Room aside{nullptr};
+  const Saved s = saved_in(p, aside);
+  const Backward b = backward_of(p, o, s, all_grads(p), room);
+  TcProduct one = b.weights;  // a single weight's gradient may be split further
+  one.groups = 1;
+  size_t parts = 0;
+  for (const TcProduct* q : {&b.x, &b.weights, static_cast<const TcProduct*>(&one), &b.down})
+    parts = std::max(parts, gemm_tc_workspace_bytes(*q, dev));
+  room.take(parts);
+  room.take(static_cast<size_t>(3 * column_part_count(p) * std::max(p.hidden, p.out_width) * 4));
+  return room.used;
 }
 
 cudaError_t launch_ffn_forward(const fhb_ffn_problem& p, void* y, void* saved, void* workspace,
-                               const DeviceInfo&, cudaStream_t stream) {
-  return p.dtype == FHB_DTYPE_F32 ? forward<float>(p, y, saved, workspace, stream)
-                                  : forward<bf16>(p, y, saved, workspace, stream);
+                               const DeviceInfo& dev, cudaStream_t stream) {
+  Room room{static_cast<char*>(workspace)}, kept{static_cast<char*>(saved)};
+  Operands o;
+  cudaError_t e = operands_in(p, nullptr, 0, room, o, stream);
+  if (e != cudaSuccess) return e;
+  const Saved s = saved_in(p, saved != nullptr ? kept : room);
+  e = launch_gemm_tc(gate_product(p, o, s, saved != nullptr), nullptr, dev, stream);
+  if (e != cudaSuccess) return e;
+  const TcProduct down = down_product(p, o, s, y);
+  return launch_gemm_tc(down, room.take(gemm_tc_workspace_bytes(down, dev)), dev, stream);
 }
 
 cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, int64_t grad_y_stride,
-                                const void* saved, const fhb_ffn_grads& grads, void* workspace,
-                                const DeviceInfo&, cudaStream_t stream) {
-  return p.dtype == FHB_DTYPE_F32
-             ? backward(p, static_cast<const float*>(grad_y), grad_y_stride, saved, grads, workspace, stream)
-             : backward(p, static_cast<const bf16*>(grad_y), grad_y_stride, saved, grads, workspace, stream);
+                                const void* saved, const fhb_ffn_grads& out, void* workspace,
+                                const DeviceInfo& dev, cudaStream_t stream) {
+  const size_t size = dtype_bytes(p.dtype);
+  if (p.tokens == 0) {
+    const struct {
+      void* p;
+      int64_t count;
+    } zero[] = {{out.w_gate, p.hidden * p.width}, {out.w_up, p.hidden * p.width},
+                {out.w_down, p.out_width * p.hidden}, {out.b_gate, p.hidden}, {out.b_up, p.hidden},
+                {out.b_down, p.out_width}};
+    for (const auto& z : zero) {
+      if (z.p == nullptr) continue;
+      const cudaError_t e = cudaMemsetAsync(z.p, 0, z.count * size, stream);
+      if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+  }
+  Room room{static_cast<char*>(workspace)}, kept{static_cast<char*>(const_cast<void*>(saved))};
+  Operands o;
+  cudaError_t e = operands_in(p, grad_y, grad_y_stride, room, o, stream);
+  if (e != cudaSuccess) return e;
+  const Saved s = saved_in(p, kept);
+  const Backward b = backward_of(p, o, s, out, room);
+  size_t parts = 0;
+  for (const auto& [want, q] : {std::pair{b.want_x, &b.x}, std::pair{b.want_weights, &b.weights},
+                                std::pair{b.want_down, &b.down}})
+    if (want) parts = std::max(parts, gemm_tc_workspace_bytes(*q, dev));
+  void* sums = room.take(parts);  // one product after the other
+  e = launch_gemm_tc(b.hidden, nullptr, dev, stream);
+  if (e == cudaSuccess && b.want_x) e = launch_gemm_tc(b.x, sums, dev, stream);
+  if (e == cudaSuccess && b.want_weights) e = launch_gemm_tc(b.weights, sums, dev, stream);
+  if (e == cudaSuccess && b.want_down) e = launch_gemm_tc(b.down, sums, dev, stream);
+  if (e != cudaSuccess) return e;
+  ColumnSources columns{};
+  int count = 0;
+  if (out.b_gate != nullptr) columns.source[count++] = {b.dg.p, b.dg.stride, b.dg.plane, p.hidden, true, out.b_gate};
+  if (out.b_up != nullptr) columns.source[count++] = {b.du.p, b.du.stride, b.du.plane, p.hidden, true, out.b_up};
+  if (out.b_down != nullptr) columns.source[count++] = {grad_y, grad_y_stride, 0, p.out_width, false, out.b_down};
+  columns.rows = p.tokens;
+  columns.part_rows = part_rows_of(p.tokens);
+  columns.widest = std::max(p.hidden, p.out_width);
+  columns.part_count = column_part_count(p);
+  columns.parts = static_cast<float*>(room.take(0));
+  return p.dtype == FHB_DTYPE_F32 ? column_sums<float>(columns, count, stream)
+                                  : column_sums<bf16>(columns, count, stream);
 }
 
 }  // namespace fhb

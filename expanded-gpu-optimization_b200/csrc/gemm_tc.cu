@@ -1,0 +1,969 @@
+// Matrix products of the gated feed-forward block on the tensor cores (tcgen05, TMEM, TMA).
+//
+// One persistent CTA per SM (or a pair of CTAs on two SMs that share a 256-row tile): warp 8
+// copies operand tiles of 64 of K into a ring in shared memory (TMA, 128-byte swizzle), warp 9
+// issues the MMAs into one of two TMEM accumulators, and warps 0-7 turn the other accumulator
+// into results. Operands may lie along K or across it in memory: the tile copies and the MMA
+// descriptors follow, nothing is transposed in a pass of its own.
+#include "gemm_tc.cuh"
+
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+namespace fhb {
+namespace {
+
+constexpr int kKBlock = 64;                      // K of one ring slot: 128 bytes of bf16
+constexpr int kRows = 128;                       // result rows of one CTA
+constexpr int kMaxColumns = 256;                 // result columns of a tile
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = 32 * (kEpilogueWarps + 2);
+constexpr int kMaxSlots = 10;
+constexpr int kRingBytes = 208 * 1024;
+constexpr int kMaxTerms = 12;
+constexpr int kATileBytes = kRows * kKBlock * 2;  // 16 KB
+
+struct Maps {
+  CUtensorMap a[2], b[2];
+};
+
+struct Args {
+  int64_t m, n;               // result rows and columns (gate: n hidden features, 2 n columns)
+  int tiles_m, tiles_n, groups, parts;
+  int k_blocks, part_blocks;  // of K, and of each part of K
+  int columns;                // columns of a tile (both halves of a gate tile)
+  int slots, terms;
+  uint8_t a_map[kMaxTerms], b_map[kMaxTerms], a_plane[kMaxTerms], b_plane[kMaxTerms];
+  int a_k_major, b_k_major;
+  int a_rows;                 // rows of one A copy (fewer than 128 where m is small)
+  uint32_t idesc;
+  // results
+  void* out[2];
+  int64_t out_stride;
+  int out_wide;               // 32-byte stores are aligned
+  const void* bias[2];
+  bf16* gated[2];
+  int64_t gated_stride, gated_plane;
+  TcFactors factors;
+  int activation;
+  float* partial;
+  int64_t partial_stride;
+  unsigned int* status;
+};
+
+// ---- PTX pieces that the other kernels' header does not have ----
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t smem, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+template <int Cg>
+__device__ __forceinline__ void copy_tile(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                          uint32_t bar) {
+  if (Cg == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        ".cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+
+// Shared-memory matrix descriptor of a tile in 128-byte swizzle. K-major: rows of 128 bytes
+// (64 of K), groups of 8 rows 1024 bytes apart (`lbo` unused). MN-major: blocks of 64 rows or
+// columns, each 64 of K by 128 bytes; `lbo` between blocks, 1024 bytes between 8 of K.
+__device__ __forceinline__ uint64_t tile_descriptor(uint32_t smem, uint32_t lbo) {
+  return static_cast<uint64_t>((smem >> 4) & 0x3FFFu) |
+         (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16) |
+         (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// The four MMAs (K = 16 each) of one ring slot, issued by one elected lane of a converged warp.
+template <int Cg>
+__device__ __forceinline__ void mma_slot(uint32_t d, uint64_t a, uint64_t b, uint32_t a_step,
+                                         uint32_t b_step, uint32_t idesc, uint32_t accumulate) {
+#define FHB_MMA_SLOT(GROUP)                                                             \
+  asm volatile(                                                                         \
+      "{\n\t.reg .pred e, p, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3, sa, sb;\n\t"       \
+      "setp.ne.b32 p, %6, 0;\n\tsetp.eq.b32 t, %6, %6;\n\t"                             \
+      "cvt.u64.u32 sa, %3;\n\tcvt.u64.u32 sb, %4;\n\t"                                  \
+      "add.u64 a1, %1, sa;\n\tadd.u64 a2, a1, sa;\n\tadd.u64 a3, a2, sa;\n\t"           \
+      "add.u64 b1, %2, sb;\n\tadd.u64 b2, b1, sb;\n\tadd.u64 b3, b2, sb;\n\t"           \
+      "elect.sync _|e, 0xffffffff;\n\t"                                                 \
+      "@e tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], %1, %2, %5, p;\n\t"          \
+      "@e tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], a1, b1, %5, t;\n\t"          \
+      "@e tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], a2, b2, %5, t;\n\t"          \
+      "@e tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], a3, b3, %5, t;\n\t}" ::"r"(d), \
+      "l"(a), "l"(b), "r"(a_step), "r"(b_step), "r"(idesc), "r"(accumulate)             \
+      : "memory")
+  if (Cg == 2)
+    FHB_MMA_SLOT("2");
+  else
+    FHB_MMA_SLOT("1");
+#undef FHB_MMA_SLOT
+}
+
+// Arrives on `bar` (in both CTAs of a pair) when the MMAs issued so far are done.
+template <int Cg>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if (Cg == 2)
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster"
+        ".multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+  else
+    tc::commit_warp(bar);
+}
+
+template <int Cg>
+__device__ __forceinline__ void allocate_tmem(uint32_t* dst) {
+  if (Cg == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tc::tmem_alloc(dst, 512);
+    tc::tmem_relinquish();
+  }
+}
+template <int Cg>
+__device__ __forceinline__ void free_tmem(uint32_t tmem) {
+  if (Cg == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  else
+    tc::tmem_dealloc(tmem, 512);
+}
+
+// 32 consecutive TMEM columns of the warp's 32 rows: one row per lane.
+__device__ __forceinline__ void load_columns(uint32_t tmem, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(tmem)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// 32 bytes in one access, 32-byte aligned: a whole memory sector per thread.
+__device__ __forceinline__ void store32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void load32(const void* p, uint32_t* v) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]),
+                 "=r"(v[6]), "=r"(v[7])
+               : "l"(p)
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// x as a sum of three bf16 (FP32's 24 significant bits in pieces of 8): each piece is the
+// remainder cut after 8 significant bits, so every difference is exact, the sum is x, and no
+// piece overflows. An infinity or a NaN is all in the first.
+__device__ __forceinline__ void split_f32(float x, float& a, float& b, float& c) {
+  a = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
+  if (!(fabsf(x) < INFINITY)) {
+    a = x;
+    b = c = 0.0f;
+    return;
+  }
+  b = __uint_as_float(__float_as_uint(x - a) & 0xFFFF0000u);
+  c = (x - a) - b;
+}
+
+// 32 values of a row in operand form (bf16, or three planes), 32-byte aligned.
+template <typename T>
+__device__ __forceinline__ void store_operand(bf16* p, int64_t plane, const float (&v)[32]) {
+  uint32_t w[16];
+  if (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+    store32(p, w);
+    store32(p + 16, w + 8);
+  } else {
+    uint32_t w1[16], w2[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float a[2], b[2], c[2];
+      split_f32(v[2 * i], a[0], b[0], c[0]);
+      split_f32(v[2 * i + 1], a[1], b[1], c[1]);
+      w[i] = pack_bf16(a[0], a[1]);
+      w1[i] = pack_bf16(b[0], b[1]);
+      w2[i] = pack_bf16(c[0], c[1]);
+    }
+    store32(p, w);
+    store32(p + 16, w + 8);
+    store32(p + plane, w1);
+    store32(p + plane + 16, w1 + 8);
+    store32(p + 2 * plane, w2);
+    store32(p + 2 * plane + 16, w2 + 8);
+  }
+}
+
+// 32 results of a row from column n0 on, those below n.
+template <typename T>
+__device__ __forceinline__ void store_results(T* row, int64_t n0, int64_t n, bool wide,
+                                              const float (&v)[32]) {
+  T* p = row + n0;
+  if (wide && n0 + 32 <= n) {
+    uint32_t w[32];
+    if (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+      store32(p, w);
+      store32(p + 16, w + 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) store32(p + 8 * i, w + 8 * i);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (n0 + i < n) p[i] = from_float<T>(v[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void add_bias(const void* bias, int64_t n0, int64_t n, float (&v)[32]) {
+  if (bias == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (n0 + i < n) v[i] += to_float(static_cast<const T*>(bias)[n0 + i]);
+}
+
+// The power of 2 that brings a group's largest magnitude into [2^14, 2^15), the top of f16's
+// range (values down to 2^-28 of the largest keep f16's 11 bits), from its FP32 exponent e,
+// kept where the power and its inverse are normal FP32 numbers.
+__device__ __forceinline__ float group_scale(float largest, uint32_t& e) {
+  e = min(max(__float_as_uint(largest) >> 23, 15u), 254u);
+  return __uint_as_float((268u - e) << 23);
+}
+__device__ __forceinline__ float group_unscale(uint32_t e) {
+  return __uint_as_float((e - 14u) << 23);
+}
+
+// 32 factors of one kind into their place (see TcFactors).
+template <typename T>
+__device__ __forceinline__ void store_factors(const TcFactors& f, int64_t place, const float (&v)[32]) {
+  uint32_t w[32];
+  if (sizeof(T) == 2) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(v[i]));
+    uint32_t e;
+    const float scale = group_scale(top, e);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const __half2 h = __floats2half2_rn(v[2 * i] * scale, v[2 * i + 1] * scale);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    __half* p = static_cast<__half*>(f.values) + place * kFactorGroup;
+    store32(p, w);
+    store32(p + 16, w + 8);
+    f.exponents[place] = static_cast<unsigned char>(e);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
+    float* p = static_cast<float*>(f.values) + place * kFactorGroup;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store32(p + 8 * i, w + 8 * i);
+  }
+}
+// v[i] *= factor i.
+template <typename T>
+__device__ __forceinline__ void times_factors(const TcFactors& f, int64_t place, float (&v)[32]) {
+  uint32_t w[32];
+  if (sizeof(T) == 2) {
+    const __half* p = static_cast<const __half*>(f.values) + place * kFactorGroup;
+    load32(p, w);
+    load32(p + 16, w + 8);
+    const float unscale = group_unscale(f.exponents[place]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] *= x.x * unscale;
+      v[2 * i + 1] *= x.y * unscale;
+    }
+  } else {
+    const float* p = static_cast<const float*>(f.values) + place * kFactorGroup;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load32(p + 8 * i, w + 8 * i);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] *= __uint_as_float(w[i]);
+  }
+}
+
+// One item of work: a tile of one group's result and one part of K.
+struct Item {
+  int group, part, first_block, blocks;
+  int64_t m0, n0;  // first row of the tile (of the pair), first column (gate: feature)
+};
+template <int Cg, bool Gate>
+__device__ __forceinline__ Item item_at(const Args& p, int64_t index) {
+  const int tiles = p.tiles_m * p.tiles_n;
+  Item it;
+  const int rest = static_cast<int>(index / tiles);
+  int tile = static_cast<int>(index % tiles);
+  it.part = rest % p.parts;
+  it.group = rest / p.parts;
+  // bands of 8 tile rows, column by column: the tiles in flight share their operands in L2
+  const int band = tile / (8 * p.tiles_n);
+  const int rows = min(8, p.tiles_m - 8 * band);
+  tile -= band * 8 * p.tiles_n;
+  it.m0 = static_cast<int64_t>(8 * band + tile % rows) * (kRows * Cg);
+  it.n0 = static_cast<int64_t>(tile / rows) * (Gate ? p.columns / 2 : p.columns);
+  it.first_block = it.part * p.part_blocks;
+  it.blocks = min(p.part_blocks, p.k_blocks - it.first_block);
+  return it;
+}
+
+// FP32 blocks: the tensor core cuts each sum to FP32 instead of rounding it, an error that
+// grows with the number of additions and has a sign. K is summed in chunks of kChunkBlocks
+// ring slots per term, and the chunks in registers, rounded.
+constexpr int kChunkBlocks = 2;
+template <typename T>
+__device__ __forceinline__ int chunk_count(int blocks) {
+  return sizeof(T) == 4 ? (blocks + kChunkBlocks - 1) / kChunkBlocks : 1;
+}
+
+template <int Cg, TcEpilogue E, typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
+  constexpr bool kGateTile = E == TcEpilogue::kGate;
+  constexpr bool kChunked = sizeof(T) == 4;
+  extern __shared__ unsigned char raw[];
+  __shared__ uint64_t full[kMaxSlots], empty[kMaxSlots], sum_full[2], sum_empty[2];
+  __shared__ uint32_t tmem_at;
+  const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = Cg == 2 ? cluster_rank() : 0;
+  const int b_rows = p.columns / Cg;  // rows of this CTA's B tile
+  const uint32_t slot_bytes = kATileBytes + static_cast<uint32_t>(b_rows) * kKBlock * 2;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.slots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sum_full[i], 1);
+      mbar_init(&sum_empty[i], kEpilogueWarps * Cg);
+    }
+    fence_barrier_init();
+  }
+  if (warp == kEpilogueWarps) allocate_tmem<Cg>(&tmem_at);
+  tc::fence_before_sync();
+  __syncthreads();
+  if (Cg == 2) cluster_sync();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_at;
+
+  const int64_t items = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.parts * p.groups;
+  const int64_t first = blockIdx.x / Cg, stride = gridDim.x / Cg;
+
+  if (warp == kEpilogueWarps) {
+    // ---- copies ----
+    if (lane == 0) {
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      int64_t issued = 0;
+      const uint32_t a_bytes = p.a_k_major ? static_cast<uint32_t>(p.a_rows) * kKBlock * 2 : kATileBytes;
+      const uint32_t bytes = Cg * (a_bytes + static_cast<uint32_t>(b_rows) * kKBlock * 2);
+      for (int64_t index = first; ok && index < items; index += stride) {
+        const Item it = item_at<Cg, kGateTile>(p, index);
+        const int chunks = chunk_count<T>(it.blocks);
+        const int64_t a0 = it.m0 + rank * kRows;
+        for (int c = 0; ok && c < chunks; ++c) {
+          const int low = it.first_block + (kChunked ? c * kChunkBlocks : 0);
+          const int high = kChunked ? min(low + kChunkBlocks, it.first_block + it.blocks)
+                                    : it.first_block + it.blocks;
+          for (int t = 0; ok && t < p.terms; ++t) {
+            const CUtensorMap* am = &maps.a[p.a_map[t] + (p.groups == 2 ? it.group : 0)];
+            const CUtensorMap* bm = &maps.b[p.b_map[t]];
+            for (int kb = low; kb < high; ++kb) {
+              if (!mbar_wait_bounded(&empty[slot], phase ^ 1, p.status, FHB_STATUS_MMA_TIMEOUT)) {
+                ok = false;
+                break;
+              }
+              if (rank == 0) mbar_arrive_expect_tx(&full[slot], bytes);
+              const uint32_t bar = Cg == 2 ? in_cta(smem_u32(&full[slot]), 0) : smem_u32(&full[slot]);
+              const uint32_t at = ring + slot * slot_bytes, bt = at + kATileBytes;
+              const int k0 = kb * kKBlock;
+              if (p.a_k_major) {
+                copy_tile<Cg>(at, am, k0, static_cast<int>(a0), p.a_plane[t], bar);
+              } else {
+                copy_tile<Cg>(at, am, static_cast<int>(a0), k0, p.a_plane[t], bar);
+                copy_tile<Cg>(at + 8192, am, static_cast<int>(a0) + 64, k0, p.a_plane[t], bar);
+              }
+              if (kGateTile) {
+                // one half of the columns from each weight (always K-major)
+                if (Cg == 2) {
+                  copy_tile<Cg>(bt, &maps.b[rank], k0, static_cast<int>(it.n0), p.b_plane[t], bar);
+                } else {
+                  copy_tile<Cg>(bt, &maps.b[0], k0, static_cast<int>(it.n0), p.b_plane[t], bar);
+                  copy_tile<Cg>(bt + b_rows * kKBlock, &maps.b[1], k0, static_cast<int>(it.n0), p.b_plane[t], bar);
+                }
+              } else {
+                const int b0 = static_cast<int>(it.n0) + static_cast<int>(rank) * b_rows;
+                if (p.b_k_major)
+                  copy_tile<Cg>(bt, bm, k0, b0, p.b_plane[t], bar);
+                else
+                  for (int i = 0; i < b_rows; i += 64)
+                    copy_tile<Cg>(bt + i * kKBlock * 2, bm, b0 + i, k0, p.b_plane[t], bar);
+              }
+              ++issued;
+              if (++slot == p.slots) {
+                slot = 0;
+                phase ^= 1;
+              }
+            }
+          }
+        }
+      }
+      // the last copies have landed before this CTA's memory is given up (as far as they can be
+      // seen from here: the pair's barriers are in CTA 0, which waits for them in its MMAs)
+      if (!ok && rank == 0)
+        for (int s = 0; s < p.slots && issued > 0; ++s, --issued) {
+          slot = slot == 0 ? p.slots - 1 : slot - 1;
+          if (slot == p.slots - 1) phase ^= 1;
+          mbar_wait_bounded(&full[slot], phase, p.status, FHB_STATUS_MMA_TIMEOUT);
+        }
+    }
+    __syncwarp();
+  } else if (warp == kEpilogueWarps + 1) {
+    // ---- MMAs (a pair's are issued by its first CTA) ----
+    if (rank == 0) {
+      int slot = 0;
+      uint32_t phase = 0;
+      int64_t sums = 0;
+      bool ok = true;
+      const uint32_t a_step = p.a_k_major ? 2 : 128, b_step = p.b_k_major ? 2 : 128;  // 16 of K
+      for (int64_t index = first; ok && index < items; index += stride) {
+        const Item it = item_at<Cg, kGateTile>(p, index);
+        const int chunks = chunk_count<T>(it.blocks);
+        for (int c = 0; ok && c < chunks; ++c, ++sums) {
+          const int low = kChunked ? c * kChunkBlocks : 0;
+          const int blocks = kChunked ? min(kChunkBlocks, it.blocks - low) : it.blocks;
+          const int buffer = static_cast<int>(sums & 1);
+          ok = mbar_wait_bounded(&sum_empty[buffer], static_cast<uint32_t>((sums >> 1) & 1) ^ 1,
+                                 p.status, FHB_STATUS_MMA_TIMEOUT);
+          if (!ok) break;
+          tc::fence_after_sync();
+          const int steps = blocks * p.terms;
+          for (int i = 0; i < steps; ++i) {
+            ok = mbar_wait_bounded(&full[slot], phase, p.status, FHB_STATUS_MMA_TIMEOUT);
+            if (!ok) break;
+            tc::fence_after_sync();
+            const uint32_t at = ring + slot * slot_bytes;
+            mma_slot<Cg>(tmem + buffer * kMaxColumns, tile_descriptor(at, 8192),
+                         tile_descriptor(at + kATileBytes, 8192), a_step, b_step, p.idesc, i != 0);
+            commit<Cg>(&empty[slot]);
+            if (++slot == p.slots) {
+              slot = 0;
+              phase ^= 1;
+            }
+          }
+          if (ok) commit<Cg>(&sum_full[buffer]);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- results: each warp has 32 rows; the two halves of the warps share the columns ----
+    const int quadrant = warp % 4, half = warp / 4, pairs = p.columns / 64;
+    const uint32_t release = Cg == 2 ? in_cta(smem_u32(&sum_empty[0]), 0) : smem_u32(&sum_empty[0]);
+    int64_t sums = 0;
+    bool ok = true;
+    for (int64_t index = first; ok && index < items; index += stride) {
+      const Item it = item_at<Cg, kGateTile>(p, index);
+      const int chunks = chunk_count<T>(it.blocks);
+      const int64_t row = it.m0 + rank * kRows + quadrant * 32 + lane;
+      // two groups of 32 columns at a time: a gate tile's g and u, else neighbours
+      const auto finish = [&](int pair, float (&v0)[32], float (&v1)[32]) {
+        if (row >= p.m) return;
+        if constexpr (E == TcEpilogue::kGate) {
+          const int64_t n0 = it.n0 + 32 * pair;
+          if (n0 >= p.n) return;
+          add_bias<T>(p.bias[0], n0, p.n, v0);
+          add_bias<T>(p.bias[1], n0, p.n, v1);
+          float h[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float a, slope;
+            block_activation(p.activation, v0[i], a, slope);
+            h[i] = a * v1[i];
+            v0[i] = a;
+            v1[i] *= slope;
+          }
+          store_operand<T>(p.gated[0] + row * p.gated_stride + n0, p.gated_plane, h);
+          if (p.factors.values != nullptr) {
+            const int64_t place = (row * p.factors.groups + n0 / kFactorGroup) * 2;
+            store_factors<T>(p.factors, place, v0);
+            store_factors<T>(p.factors, place + 1, v1);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float(&v)[32] = j == 0 ? v0 : v1;
+            const int64_t n0 = it.n0 + 64 * pair + 32 * j;
+            if (n0 >= p.n) break;
+            if constexpr (E == TcEpilogue::kGateGrad) {
+              const int64_t place = (row * p.factors.groups + n0 / kFactorGroup) * 2;
+              float d[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) d[i] = v[i];
+              times_factors<T>(p.factors, place, d);  // du = dh act(g)
+              times_factors<T>(p.factors, place + 1, v);
+              const int64_t at = row * p.gated_stride + n0;
+              store_operand<T>(p.gated[0] + at, p.gated_plane, v);
+              store_operand<T>(p.gated[1] + at, p.gated_plane, d);
+            } else if constexpr (E == TcEpilogue::kPartial) {
+              float* out = p.partial + ((static_cast<int64_t>(it.group) * p.parts + it.part) * p.m + row) * p.partial_stride;
+              store_results<float>(out, n0, p.partial_stride, true, v);
+            } else {
+              add_bias<T>(p.bias[0], n0, p.n, v);
+              store_results<T>(static_cast<T*>(p.out[it.group]) + row * p.out_stride, n0, p.n, p.out_wide != 0, v);
+            }
+          }
+        }
+      };
+      float acc0[32], acc1[32];
+      for (int c = 0; c < chunks; ++c, ++sums) {
+        const int buffer = static_cast<int>(sums & 1);
+        ok = mbar_wait_bounded(&sum_full[buffer], static_cast<uint32_t>((sums >> 1) & 1), p.status,
+                               FHB_STATUS_MMA_TIMEOUT);
+        // a wait that gave up: the warps agree, since what follows is for whole warps
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc::fence_after_sync();
+        const uint32_t from = tmem + buffer * kMaxColumns + (static_cast<uint32_t>(quadrant * 32) << 16);
+        for (int pair = half; pair < pairs; pair += 2) {
+          __syncwarp();
+          const uint32_t c0 = from + (kGateTile ? 32 * pair : 64 * pair);
+          const uint32_t c1 = kGateTile ? from + p.columns / 2 + 32 * pair : c0 + 32;
+          if (kChunked && c > 0) {
+            float v[32];
+            load_columns(c0, v);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc0[i] += v[i];
+            load_columns(c1, v);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc1[i] += v[i];
+          } else {
+            load_columns(c0, acc0);
+            load_columns(c1, acc1);
+            tc::wait_ld();
+          }
+          if (pair + 2 >= pairs) {  // the accumulator has been read
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+              if (Cg == 2) arrive_remote(release + buffer * 8);
+              else mbar_arrive(&sum_empty[buffer]);
+            }
+          }
+          if (!kChunked || c + 1 == chunks) finish(pair, acc0, acc1);
+        }
+        if (half >= pairs) {  // a tile of 64 columns leaves the second half of the warps idle
+          __syncwarp();
+          if (lane == 0) {
+            if (Cg == 2) arrive_remote(release + buffer * 8);
+            else mbar_arrive(&sum_empty[buffer]);
+          }
+        }
+      }
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (Cg == 2) cluster_sync();
+  if (warp == kEpilogueWarps) free_tmem<Cg>(tmem);
+}
+
+// out[m][n] = the sum of the parts in order + bias[n].
+template <typename T>
+__global__ void __launch_bounds__(256)
+    add_parts_kernel(const float* __restrict__ partial, int64_t part_values, int64_t stride, int parts,
+                     int64_t m, int64_t n, const T* __restrict__ bias, T* __restrict__ out,
+                     int64_t out_stride) {
+  const int64_t quads = stride / 4;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < m * quads; i += gridDim.x * 256ll) {
+    const int64_t row = i / quads, c = (i % quads) * 4;
+    const float4* src = reinterpret_cast<const float4*>(partial + row * stride + c);
+    float4 s = src[0];
+    for (int k = 1; k < parts; ++k) {
+      const float4 v = src[k * (part_values / 4)];
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+    }
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < n)
+        out[row * out_stride + c + j] = from_float<T>(v[j] + (bias != nullptr ? to_float(bias[c + j]) : 0.0f));
+  }
+}
+
+// Rows of `cols` values into rows of `stride` bf16 (a multiple of 8, the rest zero): a copy, or
+// the three planes of FP32 values.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    pack_kernel(const T* __restrict__ in, int64_t rows, int64_t cols, int64_t in_stride,
+                bf16* __restrict__ out, int64_t stride, int64_t plane) {
+  const int64_t pieces = stride / 8;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * pieces; i += gridDim.x * 256ll) {
+    const int64_t row = i / pieces, c = (i % pieces) * 8;
+    const T* src = in + row * in_stride + c;
+    float v[8];
+    if (sizeof(T) == 4 && c + 8 <= cols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+      const float4 x = reinterpret_cast<const float4*>(src)[0], y = reinterpret_cast<const float4*>(src)[1];
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_float(src[j]) : 0.0f;
+    }
+    bf16* dst = out + row * stride + c;
+    uint32_t w[3][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (sizeof(T) == 2) {
+        w[0][j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+      } else {
+        float x[3], y[3];
+        split_f32(v[2 * j], x[0], x[1], x[2]);
+        split_f32(v[2 * j + 1], y[0], y[1], y[2]);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) w[q][j] = pack_bf16(x[q], y[q]);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < (sizeof(T) == 2 ? 1 : 3); ++q)
+      *reinterpret_cast<uint4*>(dst + q * plane) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+  }
+}
+
+int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+int64_t blocks_of(int64_t x, int64_t size) { return (x + size - 1) / size; }
+
+// ---- the plan of a product: tile, pairing, parts of K ----
+struct Plan {
+  int cg, columns, parts, part_blocks, k_blocks, tiles_m, tiles_n, terms, slots, grid;
+  int64_t partial_stride;
+};
+
+// Chooses by an estimate of the launch's cycles. A ring slot costs its MMAs (4 x columns / 2
+// cycles a CTA, the same work in a pair with half the B tile each) or the copies of its bytes
+// (about 64 a cycle), whichever is longer; an item costs about 2,000 cycles more (its first
+// copies, its last results), and a second launch that adds the parts about 3,000 and its bytes.
+Plan plan_of(const TcProduct& p, const DeviceInfo& dev) {
+  const bool wide = p.dtype == FHB_DTYPE_F32, gate = p.epilogue == TcEpilogue::kGate;
+  const int terms = p.sum_terms * (wide ? 6 : 1);
+  const int k_blocks = static_cast<int>(blocks_of(p.k, kKBlock));
+  const int64_t n_columns = gate ? 2 * p.n : p.n;
+  Plan best{};
+  double least = 0.0;
+  for (int cg = 1; cg <= 2; ++cg)
+    for (int columns = 64; columns <= (wide ? 128 : kMaxColumns); columns *= 2) {
+      if (cg == 2 && columns < 128) continue;  // an operand across K comes in blocks of 64
+      if (cg == 2 && p.m <= kRows) continue;
+      const int64_t tiles_m = blocks_of(p.m, kRows * cg);
+      const int64_t tiles_n = blocks_of(n_columns, columns);
+      const int64_t tiles = tiles_m * tiles_n * p.groups;
+      const int64_t units = dev.sms / cg;
+      const int most = p.epilogue == TcEpilogue::kStore ? std::min(k_blocks, 64) : 1;
+      for (int parts = 1; parts <= most; ++parts) {
+        if (parts > 1 && tiles * (parts - 1) >= 4 * units) break;
+        const int part_blocks = static_cast<int>(blocks_of(k_blocks, parts));
+        if (blocks_of(k_blocks, part_blocks) != parts) continue;
+        const double mma = 2.0 * columns, copy = (kATileBytes + 128.0 * columns / cg) / 64.0;
+        const double item = 2000.0 + static_cast<double>(part_blocks) * terms * std::max(mma, copy);
+        double cycles = static_cast<double>(blocks_of(tiles * parts, units)) * item;
+        if (parts > 1)
+          cycles += 3000.0 + 8.0 * static_cast<double>(p.m) * n_columns * p.groups * parts / (64.0 * dev.sms);
+        if (least == 0.0 || cycles < least) {
+          least = cycles;
+          best.cg = cg;
+          best.columns = columns;
+          best.parts = parts;
+          best.part_blocks = part_blocks;
+          best.tiles_m = static_cast<int>(tiles_m);
+          best.tiles_n = static_cast<int>(tiles_n);
+          best.grid = static_cast<int>(std::min<int64_t>(tiles * parts, units)) * cg;
+        }
+      }
+    }
+  best.k_blocks = k_blocks;
+  best.terms = terms;
+  best.slots = std::min(kMaxSlots, kRingBytes / (kATileBytes + best.columns / best.cg * kKBlock * 2));
+  best.partial_stride = round_up(p.n, 32);
+  return best;
+}
+
+// ---- TMA tile maps ----
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled g_encode = nullptr;
+
+// Tiles of 64 columns (128 bytes, swizzled) by `box_rows` rows of one plane.
+bool tile_map(const TcMatrix& x, int box_rows, CUtensorMap* out) {
+  const cuuint64_t size[3] = {static_cast<cuuint64_t>(x.cols), static_cast<cuuint64_t>(x.rows),
+                              static_cast<cuuint64_t>(x.planes)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(x.stride) * 2,
+                                 static_cast<cuuint64_t>(x.planes > 1 ? x.plane : x.stride) * 2};
+  const cuuint32_t box[3] = {kKBlock, static_cast<cuuint32_t>(box_rows), 1}, step[3] = {1, 1, 1};
+  const auto encode = [&] {
+    return g_encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<bf16*>(x.p), size, strides,
+                    box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (encode()) return true;
+  // the driver call needs a context on this thread, which the runtime makes current only with
+  // the thread's first call that needs one (autograd's threads may not have made any)
+  int device = 0;
+  return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && encode();
+}
+
+size_t smem_bytes(const Plan& plan) {
+  return static_cast<size_t>(plan.slots) * (kATileBytes + plan.columns / plan.cg * kKBlock * 2) + 1024;
+}
+
+template <int Cg, TcEpilogue E, typename T>
+cudaError_t launch(const Maps& maps, const Args& args, const Plan& plan, cudaStream_t stream) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = Cg;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(plan.grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem_bytes(plan);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = Cg == 2 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, gemm_tc_kernel<Cg, E, T>, maps, args);
+}
+
+template <TcEpilogue E>
+cudaError_t launch_kind(bool wide, const Maps& maps, const Args& args, const Plan& plan, cudaStream_t stream) {
+  if (wide)
+    return plan.cg == 2 ? launch<2, E, float>(maps, args, plan, stream)
+                        : launch<1, E, float>(maps, args, plan, stream);
+  return plan.cg == 2 ? launch<2, E, bf16>(maps, args, plan, stream)
+                      : launch<1, E, bf16>(maps, args, plan, stream);
+}
+
+template <int Cg, TcEpilogue E>
+cudaError_t prepare_kind() {
+  const cudaError_t e = cudaFuncSetAttribute(gemm_tc_kernel<Cg, E, float>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes + 1024);
+  return e != cudaSuccess ? e
+                          : cudaFuncSetAttribute(gemm_tc_kernel<Cg, E, bf16>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes + 1024);
+}
+
+template <typename T>
+cudaError_t add_parts(const TcProduct& p, const Plan& plan, const float* partial, const DeviceInfo& dev,
+                      cudaStream_t stream) {
+  const int64_t values = p.m * plan.partial_stride;
+  const int64_t blocks = std::min<int64_t>(blocks_of(values / 4, 256), 8ll * dev.sms);
+  for (int g = 0; g < p.groups; ++g) {
+    add_parts_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
+        partial + g * plan.parts * values, values, plan.partial_stride, plan.parts, p.m, p.n,
+        static_cast<const T*>(p.bias[0]), static_cast<T*>(p.out[g]), p.out_stride);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace
+
+cudaError_t prepare_gemm_tc() {
+  void* entry = nullptr;
+  cudaDriverEntryPointQueryResult found;
+  cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000,
+                                                   cudaEnableDefault, &found);
+  if (e != cudaSuccess) return e;
+  if (found != cudaDriverEntryPointSuccess || entry == nullptr) return cudaErrorSymbolNotFound;
+  g_encode = reinterpret_cast<EncodeTiled>(entry);
+  for (auto prepare : {prepare_kind<1, TcEpilogue::kStore>, prepare_kind<2, TcEpilogue::kStore>,
+                       prepare_kind<1, TcEpilogue::kPartial>, prepare_kind<2, TcEpilogue::kPartial>,
+                       prepare_kind<1, TcEpilogue::kGate>, prepare_kind<2, TcEpilogue::kGate>,
+                       prepare_kind<1, TcEpilogue::kGateGrad>, prepare_kind<2, TcEpilogue::kGateGrad>})
+    if ((e = prepare()) != cudaSuccess) return e;
+  return cudaSuccess;
+}
+
+size_t gemm_tc_workspace_bytes(const TcProduct& p, const DeviceInfo& dev) {
+  const Plan plan = plan_of(p, dev);
+  return plan.parts == 1 ? 0 : static_cast<size_t>(plan.parts) * p.groups * p.m * plan.partial_stride * 4;
+}
+
+cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, const DeviceInfo& dev,
+                           cudaStream_t stream) {
+  const Plan plan = plan_of(p, dev);
+  const bool wide = p.dtype == FHB_DTYPE_F32, gate = p.epilogue == TcEpilogue::kGate;
+  Args args{};
+  args.m = p.m;
+  args.n = p.n;
+  args.tiles_m = plan.tiles_m;
+  args.tiles_n = plan.tiles_n;
+  args.groups = p.groups;
+  args.parts = plan.parts;
+  args.k_blocks = plan.k_blocks;
+  args.part_blocks = plan.part_blocks;
+  args.columns = plan.columns;
+  args.slots = plan.slots;
+  // FP32: the products of planes whose sizes multiply to 2^-16 of the whole or more, smallest
+  // first (the dropped ones are below 2^-24)
+  constexpr uint8_t planes[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
+  for (int q = 0; q < (wide ? 6 : 1); ++q)
+    for (int s = 0; s < p.sum_terms; ++s) {
+      const int t = args.terms++;
+      args.a_map[t] = args.b_map[t] = static_cast<uint8_t>(s);
+      args.a_plane[t] = wide ? planes[q][0] : 0;
+      args.b_plane[t] = wide ? planes[q][1] : 0;
+    }
+  args.a_k_major = p.a_k_major;
+  args.b_k_major = p.b_k_major;
+  args.a_rows = static_cast<int>(std::min<int64_t>(kRows, round_up(p.m, 8)));
+  args.idesc = (1u << 4) | (1u << 7) | (1u << 10) | (p.a_k_major ? 0u : tc::kIdescAMnMajor) |
+               (p.b_k_major ? 0u : tc::kIdescBMnMajor) |
+               (static_cast<uint32_t>(plan.columns) >> 3 << 17) |
+               (static_cast<uint32_t>(kRows * plan.cg) >> 4 << 24);  // bf16 in, FP32 sums
+  for (int i = 0; i < 2; ++i) {
+    args.out[i] = p.out[i];
+    args.bias[i] = p.bias[i];
+    args.gated[i] = const_cast<bf16*>(p.gated[i].p);
+  }
+  args.out_stride = p.out_stride;
+  const int64_t out_bytes = p.out_stride * static_cast<int64_t>(dtype_bytes(p.dtype));
+  args.out_wide = out_bytes % 32 == 0 && reinterpret_cast<uintptr_t>(p.out[0]) % 32 == 0 &&
+                  reinterpret_cast<uintptr_t>(p.out[1]) % 32 == 0;
+  args.gated_stride = p.gated[0].stride;
+  args.gated_plane = p.gated[0].plane;
+  args.factors = p.factors;
+  args.activation = p.activation;
+  args.partial = static_cast<float*>(workspace);
+  args.partial_stride = plan.partial_stride;
+  args.status = dev.status;
+
+  Maps maps{};
+  const int b_rows = plan.columns / plan.cg;
+  const int a_box = p.a_k_major ? args.a_rows : kKBlock;
+  const int b_box = !p.b_k_major ? kKBlock : gate ? plan.columns / 2 : b_rows;
+  for (int i = 0; i < 2; ++i) {
+    if (!tile_map(p.a[p.a[i].p != nullptr ? i : 0], a_box, &maps.a[i]) ||
+        !tile_map(p.b[p.b[i].p != nullptr ? i : 0], b_box, &maps.b[i]))
+      return cudaErrorInvalidValue;
+  }
+  switch (p.epilogue) {
+    case TcEpilogue::kGate: return launch_kind<TcEpilogue::kGate>(wide, maps, args, plan, stream);
+    case TcEpilogue::kGateGrad: return launch_kind<TcEpilogue::kGateGrad>(wide, maps, args, plan, stream);
+    default: break;
+  }
+  if (plan.parts == 1) return launch_kind<TcEpilogue::kStore>(wide, maps, args, plan, stream);
+  const cudaError_t e = launch_kind<TcEpilogue::kPartial>(wide, maps, args, plan, stream);
+  if (e != cudaSuccess) return e;
+  return wide ? add_parts<float>(p, plan, args.partial, dev, stream)
+              : add_parts<bf16>(p, plan, args.partial, dev, stream);
+}
+
+namespace {
+bool copies_by_tile(const void* p, int64_t stride, int dtype) {
+  return dtype == FHB_DTYPE_BF16 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0;
+}
+}  // namespace
+
+size_t tc_result_bytes(int64_t rows, int64_t cols, int dtype) {
+  return static_cast<size_t>(rows) * round_up(cols, 32) * 2 * (dtype == FHB_DTYPE_F32 ? 3 : 1);
+}
+
+TcMatrix tc_result(void* room, int64_t rows, int64_t cols, int dtype) {
+  const int64_t stride = round_up(cols, 32);
+  return {static_cast<const bf16*>(room), rows, cols, stride, rows * stride, dtype == FHB_DTYPE_F32 ? 3 : 1};
+}
+
+size_t tc_operand_bytes(const void* p, int64_t rows, int64_t cols, int64_t stride, int dtype) {
+  return copies_by_tile(p, stride, dtype) ? 0 : tc_result_bytes(rows, cols, dtype);
+}
+
+cudaError_t tc_operand(const void* p, int64_t rows, int64_t cols, int64_t stride, int dtype,
+                       void* room, TcMatrix* out, cudaStream_t stream) {
+  if (copies_by_tile(p, stride, dtype)) {
+    *out = {static_cast<const bf16*>(p), rows, cols, stride, 0, 1};
+    return cudaSuccess;
+  }
+  *out = tc_result(room, rows, cols, dtype);
+  const int64_t pieces = rows * (out->stride / 8);
+  if (pieces == 0) return cudaSuccess;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(blocks_of(pieces, 256), 2368));
+  if (dtype == FHB_DTYPE_F32)
+    pack_kernel<float><<<grid, 256, 0, stream>>>(static_cast<const float*>(p), rows, cols, stride,
+                                                 static_cast<bf16*>(room), out->stride, out->plane);
+  else
+    pack_kernel<bf16><<<grid, 256, 0, stream>>>(static_cast<const bf16*>(p), rows, cols, stride,
+                                                static_cast<bf16*>(room), out->stride, out->plane);
+  return cudaGetLastError();
+}
+
+size_t tc_factor_bytes(int64_t tokens, int64_t hidden, int dtype) {
+  const int64_t places = tokens * blocks_of(hidden, kFactorGroup) * 2;
+  return static_cast<size_t>(dtype == FHB_DTYPE_F32 ? places * kFactorGroup * 4
+                                                    : places * kFactorGroup * 2 + round_up(places, 32));
+}
+
+TcFactors tc_factors(void* room, int64_t tokens, int64_t hidden, int dtype) {
+  const int64_t groups = blocks_of(hidden, kFactorGroup), places = tokens * groups * 2;
+  unsigned char* base = static_cast<unsigned char*>(room);
+  return {room, dtype == FHB_DTYPE_F32 ? nullptr : base + places * kFactorGroup * 2, groups};
+}
+
+}  // namespace fhb

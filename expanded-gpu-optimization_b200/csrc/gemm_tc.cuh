@@ -1,0 +1,78 @@
+// Matrix products on the tensor cores for the gated feed-forward block: operands, the plan of a
+// product and its launcher (gemm_tc.cu).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "blocks.cuh"
+
+namespace fhb {
+
+// A bf16 matrix in memory, rows x columns, rows `stride` elements apart (a multiple of 8, base
+// 16-byte aligned: what a TMA tile copy needs). An FP32 matrix is three such planes whose sum
+// it is (split_f32 in gemm_tc.cu), `plane` elements apart.
+struct TcMatrix {
+  const bf16* p = nullptr;
+  int64_t rows = 0, cols = 0, stride = 0, plane = 0;
+  int planes = 1;
+};
+
+// What a product does with its sums.
+enum class TcEpilogue {
+  kStore,     // out[m][n] = sum + bias[n], in the output type
+  kPartial,   // FP32 sums of one part of K into the workspace (added up by a second kernel)
+  kGate,      // two products g, u side by side: h = act(g) u, and what the backward needs
+  kGateGrad,  // the gradients of g and u from that of h
+};
+
+// What the forward keeps of the activation for the backward, for 32 consecutive hidden features
+// of one token: f1 = act(g) and f2 = u act'(g), so that du = dh f1 and dg = dh f2.
+// bf16 block: f16 values times one power of 2 for each of the two groups of 32 (an exponent
+// byte each), so the range is FP32's and the rounding 2^-12 of the group's largest value --
+// 16 times below the bf16 rounding of dg and du that follows. FP32 block: FP32 values.
+constexpr int kFactorGroup = 32;
+struct TcFactors {
+  void* values = nullptr;          // [token][group][2][32], __half or float
+  unsigned char* exponents = nullptr;  // [token][group][2]
+  int64_t groups = 0;
+};
+
+// One product, or two of the same shape that share a launch: C[m][n] = sum over terms and k of
+// A(m, k) B(n, k). An operand is K-major (memory rows are m or n) or not (memory rows are k).
+struct TcProduct {
+  int64_t m = 0, n = 0, k = 0;
+  TcMatrix a[2], b[2];
+  bool a_k_major = true, b_k_major = true;
+  int groups = 1;     // 2: A = a[0] or a[1] (B = b[0] in both), results to out[0] and out[1]
+  int sum_terms = 1;  // 2: the sum of a[0] b[0] and a[1] b[1]
+  TcEpilogue epilogue = TcEpilogue::kStore;
+  int dtype = FHB_DTYPE_BF16;  // of the block: the type of out and bias; FP32: three planes
+  void* out[2] = {nullptr, nullptr};
+  int64_t out_stride = 0;
+  const void* bias[2] = {nullptr, nullptr};
+  // kGate: h; kGateGrad: dg and du (TcMatrix rows x cols are theirs)
+  TcMatrix gated[2];
+  TcFactors factors;
+  int activation = 0;
+};
+
+// Workspace of a product: the FP32 partial sums of its parts of K (0 where it has one).
+size_t gemm_tc_workspace_bytes(const TcProduct& p, const DeviceInfo& dev);
+cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, const DeviceInfo& dev,
+                           cudaStream_t stream);
+
+// `rows` x `cols` elements of type `dtype` with row stride `stride` as tensor-core operand:
+// the matrix itself where it can be copied by TMA, else its copy in `room` (bytes:
+// tc_operand_bytes; 0 where no copy is needed).
+size_t tc_operand_bytes(const void* p, int64_t rows, int64_t cols, int64_t stride, int dtype);
+cudaError_t tc_operand(const void* p, int64_t rows, int64_t cols, int64_t stride, int dtype,
+                       void* room, TcMatrix* out, cudaStream_t stream);
+// A matrix of the block's type in operand form at `room`, to be written by a product.
+size_t tc_result_bytes(int64_t rows, int64_t cols, int dtype);
+TcMatrix tc_result(void* room, int64_t rows, int64_t cols, int dtype);
+size_t tc_factor_bytes(int64_t tokens, int64_t hidden, int dtype);
+TcFactors tc_factors(void* room, int64_t tokens, int64_t hidden, int dtype);
+
+}  // namespace fhb

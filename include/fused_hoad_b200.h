@@ -328,8 +328,9 @@ size_t fhb_ffn_saved_bytes(const fhb_ffn_problem* problem);
 /* Workspace of the forward (backward == 0) or the backward call on the current device. */
 size_t fhb_ffn_workspace_bytes(const fhb_ffn_problem* problem, int backward);
 /*
- * y [tokens][out_width], contiguous. `saved` (fhb_ffn_saved_bytes bytes, 16-byte aligned) is
- * filled for fhb_ffn_backward, or NULL where no gradient is wanted. Workspace 16-byte aligned.
+ * y [tokens][out_width], contiguous. `saved` (fhb_ffn_saved_bytes bytes, 128-byte aligned)
+ * is filled for fhb_ffn_backward, or NULL where no gradient is wanted. Workspaces of these
+ * operators are 128-byte aligned.
  * tokens == 0 is a no-op.
  */
 int fhb_ffn_forward(const fhb_ffn_problem* problem, void* y, void* saved, void* workspace,
