@@ -8,6 +8,7 @@ namespace {
 
 constexpr int64_t kMaxRows = int64_t{1} << 30;    // rows of an activation
 constexpr int64_t kMaxColumns = int64_t{1} << 22;  // values of a row
+constexpr int64_t kMaxNormWidth = 32768;         // values of a row that a CTA can hold
 constexpr uintptr_t kRoomAlignment = 128;         // of workspaces and saved buffers
 constexpr int64_t kMaxCount = int64_t{1} << 40;   // values of a tensor
 
@@ -73,8 +74,7 @@ int check_norm(const fhb_norm_problem* p) {
       (p->branch == nullptr && p->rows > 0 && (p->gate != nullptr || p->post_weight != nullptr)) ||
       (p->gate != nullptr && p->gate_rows < 1))
     return FHB_ERR_INVALID_ARGUMENT;
-  if (p->rows > kMaxRows || p->width > kMaxColumns || p->rows * p->width > kMaxCount)
-    return FHB_ERR_TOO_LARGE;
+  if (p->rows > kMaxRows || p->width > kMaxNormWidth) return FHB_ERR_TOO_LARGE;
   return first_of(
       check_matrix(p->residual, p->rows, p->width, p->residual_stride, p->residual_dtype),
       p->branch == nullptr ? FHB_OK
@@ -159,7 +159,7 @@ int fhb_residual_norm(const fhb_norm_problem* problem, void* total, void* normed
 size_t fhb_residual_norm_workspace_bytes(const fhb_norm_problem* problem) {
   const fhb::DeviceInfo* dev = nullptr;
   if (problem == nullptr || problem->rows < 0 || problem->width < 1 || problem->rows > kMaxRows ||
-      problem->width > kMaxColumns || fhb::current_device_info(&dev) != FHB_OK)
+      problem->width > kMaxNormWidth || fhb::current_device_info(&dev) != FHB_OK)
     return 0;
   return fhb::residual_norm_workspace_bytes(*problem, *dev);
 }

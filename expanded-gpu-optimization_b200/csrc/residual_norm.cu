@@ -8,223 +8,527 @@
 // mean(q th), so the backward needs one round of three row sums:
 //     S1 = sum q th,   A = sum (dT + it q) c z,   B = sum th c z,
 //     sum dt c z = A - it (S1 / width) B.
+//
+// Bound by memory: every input is read once and every output written once, a row at a time in
+// registers. A row is spread over 8, 16 or 32 lanes of a warp (32 to 8 rows a CTA), or over one
+// CTA, eight values a thread; a thread keeps its columns' weights, and in the backward the sums
+// of its columns, from row to row. The column sums end in a second kernel, in a fixed order.
+#include <algorithm>
+
 #include "blocks.cuh"
 
 namespace fhb {
 namespace {
 
-constexpr int kThreads = 256;
-
-// Sums of K values over the CTA, in a fixed order, to every thread.
-template <int K>
-__device__ __forceinline__ void block_sum(float (&v)[K]) {
-  __shared__ float part[K][kThreads / 32];
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-#pragma unroll
-    for (int m = 16; m >= 1; m >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], m);
-    if (threadIdx.x % 32 == 0) part[k][threadIdx.x / 32] = v[k];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    v[k] = 0.0f;
-    for (int w = 0; w < kThreads / 32; ++w) v[k] += part[k][w];
-  }
-}
+constexpr int kVector = 8;  // values of a row that a thread holds together
 
 struct NormArgs {
   const void *residual, *branch, *pre_weight, *post_weight, *gate;
-  int64_t rows, width, residual_stride, branch_stride, gate_rows;
+  int64_t rows, residual_stride, branch_stride, gate_rows;
+  int width;
   const float* scale_ptr;
   float scale, eps;
 };
 
-// One CTA per row (grid-stride).
-template <typename TR, typename T>
-__global__ void __launch_bounds__(kThreads)
+// How a row lies over threads. Lanes: 8, 16, 32 (parts of a warp, 256-thread CTAs) or 0 (the
+// whole CTA, at most Most threads). V vectors a thread. Wide: a vector is 8 neighbours and moved
+// in 16-byte accesses; else its values lie a row of threads apart, so that a warp's accesses
+// are neighbours at any width, offset and stride.
+template <int Lanes_, int Most_, int V_, bool Wide_>
+struct Layout {
+  static constexpr int Lanes = Lanes_, Most = Most_, V = V_;
+  static constexpr int Resident = Most <= 256 ? 2 : 1;  // CTAs an SM holds in the backward
+  static constexpr bool Wide = Wide_;
+  static __device__ __forceinline__ int lanes() { return Lanes ? Lanes : static_cast<int>(blockDim.x); }
+  static __device__ __forceinline__ int lane() {
+    return Lanes ? static_cast<int>(threadIdx.x) % Lanes : static_cast<int>(threadIdx.x);
+  }
+  static __device__ __forceinline__ int slots() { return Lanes ? static_cast<int>(blockDim.x) / Lanes : 1; }
+  static __device__ __forceinline__ int slot() { return Lanes ? static_cast<int>(threadIdx.x) / Lanes : 0; }
+  static __device__ __forceinline__ int column(int v, int i) {
+    return Wide ? (v * lanes() + lane()) * kVector + i : (v * kVector + i) * lanes() + lane();
+  }
+};
+
+template <typename L, typename T>
+__device__ __forceinline__ void load_row(const T* row, int width, float (&x)[L::V][kVector]) {
+#pragma unroll
+  for (int v = 0; v < L::V; ++v) {
+    if (L::Wide) {
+      const int c = L::column(v, 0);
+      if (c < width) {
+        if (sizeof(T) == 2) {
+          const uint4 w = *reinterpret_cast<const uint4*>(row + c);
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[v][2 * i] = __uint_as_float(u[i] << 16);
+            x[v][2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+          }
+        } else {
+          const float4 a = reinterpret_cast<const float4*>(row + c)[0];
+          const float4 b = reinterpret_cast<const float4*>(row + c)[1];
+          x[v][0] = a.x, x[v][1] = a.y, x[v][2] = a.z, x[v][3] = a.w;
+          x[v][4] = b.x, x[v][5] = b.y, x[v][6] = b.z, x[v][7] = b.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kVector; ++i) x[v][i] = 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVector; ++i) {
+        const int c = L::column(v, i);
+        x[v][i] = c < width ? to_float(row[c]) : 0.0f;
+      }
+    }
+  }
+}
+
+template <typename L, typename T>
+__device__ __forceinline__ void store_row(T* row, int width, const float (&x)[L::V][kVector]) {
+#pragma unroll
+  for (int v = 0; v < L::V; ++v) {
+    if (L::Wide) {
+      const int c = L::column(v, 0);
+      if (c >= width) continue;
+      if (sizeof(T) == 2) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(x[v][2 * i + 1]), "f"(x[v][2 * i]));
+        *reinterpret_cast<uint4*>(row + c) = make_uint4(u[0], u[1], u[2], u[3]);
+      } else {
+        reinterpret_cast<float4*>(row + c)[0] = make_float4(x[v][0], x[v][1], x[v][2], x[v][3]);
+        reinterpret_cast<float4*>(row + c)[1] = make_float4(x[v][4], x[v][5], x[v][6], x[v][7]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVector; ++i) {
+        const int c = L::column(v, i);
+        if (c < width) row[c] = from_float<T>(x[v][i]);
+      }
+    }
+  }
+}
+
+template <typename L>
+__device__ __forceinline__ void fill(float (&x)[L::V][kVector], float value) {
+#pragma unroll
+  for (int v = 0; v < L::V; ++v)
+#pragma unroll
+    for (int i = 0; i < kVector; ++i) x[v][i] = value;
+}
+
+// Sums of K values over the threads of a row, in a fixed order, to all of them. `round` flips
+// between calls: two buffers need one barrier a call.
+template <typename L, int K>
+__device__ __forceinline__ void row_sum(float (&s)[K], int& round) {
+  constexpr int kFirst = L::Lanes ? L::Lanes / 2 : 16;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int m = kFirst; m >= 1; m >>= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], m);
+  if (L::Lanes) return;
+  __shared__ float part[2][K][32];
+  const int warps = static_cast<int>(blockDim.x) / 32;
+  if (threadIdx.x % 32 == 0)
+#pragma unroll
+    for (int k = 0; k < K; ++k) part[round][k][threadIdx.x / 32] = s[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int lane = static_cast<int>(threadIdx.x) % 32;
+    s[k] = lane < warps ? part[round][k][lane] : 0.0f;
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], m);
+  }
+  round ^= 1;
+}
+
+// A row's value where the row exists: rows of a warp's other slots take part in its shuffles.
+#define FHB_EACH(L) \
+  _Pragma("unroll") for (int v = 0; v < L::V; ++v) _Pragma("unroll") for (int i = 0; i < kVector; ++i)
+
+template <typename L, typename TR, typename T>
+__global__ void __launch_bounds__(L::Most)
     norm_kernel(NormArgs a, TR* __restrict__ total, T* __restrict__ normed,
                 float* __restrict__ stats) {
   const float scale = a.scale_ptr != nullptr ? *a.scale_ptr : a.scale;
-  const T *pre = static_cast<const T*>(a.pre_weight), *post = static_cast<const T*>(a.post_weight);
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const TR* r = static_cast<const TR*>(a.residual) + row * a.residual_stride;
-    const T* b = a.branch != nullptr ? static_cast<const T*>(a.branch) + row * a.branch_stride : nullptr;
-    const T* gate = a.gate != nullptr
-                        ? static_cast<const T*>(a.gate) + row / a.gate_rows * a.width : nullptr;
+  const float inverse = 1.0f / static_cast<float>(a.width);
+  const bool post = a.post_weight != nullptr, gated = a.gate != nullptr;
+  const bool one_gate = gated && a.gate_rows >= a.rows;
+  float wpre[L::V][kVector], wpost[L::V][kVector], gate[L::V][kVector];
+  load_row<L>(static_cast<const T*>(a.pre_weight), a.width, wpre);
+  if (post) load_row<L>(static_cast<const T*>(a.post_weight), a.width, wpost);
+  if (one_gate) load_row<L>(static_cast<const T*>(a.gate), a.width, gate);
+  int round = 0;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * L::slots();
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * L::slots(); first < a.rows; first += step) {
+    const int64_t row = first + L::slot();
+    const bool real = row < a.rows;
+    float t[L::V][kVector], b[L::V][kVector];
+    fill<L>(t, 0.0f);
+    fill<L>(b, 0.0f);
+    if (real) {
+      load_row<L>(static_cast<const TR*>(a.residual) + row * a.residual_stride, a.width, t);
+      if (a.branch != nullptr)
+        load_row<L>(static_cast<const T*>(a.branch) + row * a.branch_stride, a.width, b);
+      if (gated && !one_gate)
+        load_row<L>(static_cast<const T*>(a.gate) + row / a.gate_rows * a.width, a.width, gate);
+    }
     float ib = 1.0f;
-    if (post != nullptr) {
+    if (post) {
       float s[1] = {};
-      for (int64_t c = threadIdx.x; c < a.width; c += kThreads) {
-        const float v = to_float(b[c]);
-        s[0] += v * v;
-      }
-      block_sum(s);
-      ib = 1.0f / sqrtf(s[0] / a.width + a.eps);
+      FHB_EACH(L) s[0] += b[v][i] * b[v][i];
+      row_sum<L>(s, round);
+      ib = 1.0f / sqrtf(s[0] * inverse + a.eps);
     }
-    const auto value = [&](int64_t c) {
-      float t = scale * to_float(r[c]);
-      if (b != nullptr) {
-        float z = to_float(b[c]);
-        if (post != nullptr) z = z * ib * to_float(post[c]);
-        t += gate != nullptr ? to_float(gate[c]) * z : z;
-      }
-      return t;
-    };
     float s[1] = {};
-    for (int64_t c = threadIdx.x; c < a.width; c += kThreads) {
-      const float t = value(c);
-      s[0] += t * t;
+    FHB_EACH(L) {
+      float z = b[v][i];
+      if (post) z = z * ib * wpost[v][i];
+      if (gated) z *= gate[v][i];
+      t[v][i] = scale * t[v][i] + z;
+      s[0] += t[v][i] * t[v][i];
     }
-    block_sum(s);
-    const float it = 1.0f / sqrtf(s[0] / a.width + a.eps);
-    for (int64_t c = threadIdx.x; c < a.width; c += kThreads) {
-      const float t = value(c);
-      if (total != nullptr) total[row * a.width + c] = from_float<TR>(t);
-      normed[row * a.width + c] = from_float<T>(t * it * to_float(pre[c]));
-    }
-    if (stats != nullptr && threadIdx.x == 0) {
+    row_sum<L>(s, round);
+    const float it = 1.0f / sqrtf(s[0] * inverse + a.eps);
+    if (!real) continue;
+    if (total != nullptr) store_row<L>(total + row * a.width, a.width, t);
+    FHB_EACH(L) t[v][i] = t[v][i] * it * wpre[v][i];
+    store_row<L>(normed + row * a.width, a.width, t);
+    if (stats != nullptr && L::lane() == 0) {
       stats[2 * row] = ib;
       stats[2 * row + 1] = it;
     }
   }
 }
 
+// ---- backward ----
+// Rows are cut into units: `parts` equal parts of every gate group (of all rows without a gate
+// or with one per channel). A slot takes whole units, so a group's sum over its rows is made
+// from at most `parts` pieces.
+struct Units {
+  int64_t groups, group_rows, parts, part_rows, slots, grid;
+};
 struct NormGrads {
   const void *total, *normed;
   int64_t total_stride, normed_stride;
-  void *residual, *branch;
-  float *dt;  // [rows][width], the gradient of t
+  void *residual, *branch, *gate;  // gate: groups of one part, written here
+  float* columns;      // [grid][3][width]: sums for dwpre, dwpost, dgate (one per channel)
+  float* gate_parts;   // [group][part][width] where groups have several parts
+  float* scale_parts;  // [grid]
+  bool want_pre, want_post, want_gate, want_scale;
 };
 
-// Row part: dr, db and dt.
-template <typename TR, typename T>
-__global__ void __launch_bounds__(kThreads)
-    norm_backward_kernel(NormArgs a, NormGrads g, const float* __restrict__ stats) {
+template <typename L, typename TR, typename T>
+__global__ void __launch_bounds__(L::Most, L::Resident)
+    norm_backward_kernel(NormArgs a, NormGrads g, Units units, const float* __restrict__ stats) {
   const float scale = a.scale_ptr != nullptr ? *a.scale_ptr : a.scale;
-  const T *pre = static_cast<const T*>(a.pre_weight), *post = static_cast<const T*>(a.post_weight);
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const TR* r = static_cast<const TR*>(a.residual) + row * a.residual_stride;
-    const T* b = a.branch != nullptr ? static_cast<const T*>(a.branch) + row * a.branch_stride : nullptr;
-    const T* gate = a.gate != nullptr
-                        ? static_cast<const T*>(a.gate) + row / a.gate_rows * a.width : nullptr;
-    const TR* dtotal = g.total != nullptr ? static_cast<const TR*>(g.total) + row * g.total_stride : nullptr;
-    const T* dn = g.normed != nullptr ? static_cast<const T*>(g.normed) + row * g.normed_stride : nullptr;
-    const float ib = stats[2 * row], it = stats[2 * row + 1];
-    const auto pieces = [&](int64_t c, float& cz, float& th, float& q, float& dT) {
-      cz = 0.0f;
-      if (b != nullptr) {
-        cz = to_float(b[c]);
-        if (post != nullptr) cz = cz * ib * to_float(post[c]);
-        if (gate != nullptr) cz *= to_float(gate[c]);
+  const float inverse = 1.0f / static_cast<float>(a.width);
+  const bool post = a.post_weight != nullptr, gated = a.gate != nullptr, branch = a.branch != nullptr;
+  const bool by_group = gated && units.groups > 1;
+  float wpre[L::V][kVector], wpost[L::V][kVector], gate[L::V][kVector];
+  load_row<L>(static_cast<const T*>(a.pre_weight), a.width, wpre);
+  if (post) load_row<L>(static_cast<const T*>(a.post_weight), a.width, wpost);
+  if (gated) load_row<L>(static_cast<const T*>(a.gate), a.width, gate);
+  float spre[L::V][kVector], spost[L::V][kVector], sgate[L::V][kVector], sscale = 0.0f;
+  fill<L>(spre, 0.0f);
+  fill<L>(spost, 0.0f);
+  fill<L>(sgate, 0.0f);
+  int round = 0;
+  const int64_t count = units.groups * units.parts;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * L::slots();
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * L::slots(); first < count; first += step) {
+    const int64_t unit = first + L::slot();
+    const int64_t group = unit / units.parts, part = unit % units.parts;
+    const int64_t group_end = min((group + 1) * units.group_rows, a.rows);
+    const int64_t begin = group * units.group_rows + part * units.part_rows;
+    const int64_t end = unit < count ? min(begin + units.part_rows, group_end) : begin;
+    if (by_group && unit < count)
+      load_row<L>(static_cast<const T*>(a.gate) + group * a.width, a.width, gate);
+    // the slots of a warp go through as many rows together, some of them without a row
+    for (int64_t k = 0; k < units.part_rows; ++k) {
+      const int64_t row = begin + k;
+      const bool real = row < end;
+      if (L::Lanes == 0 && !real) break;
+      float r[L::V][kVector], b[L::V][kVector], dT[L::V][kVector], dn[L::V][kVector];
+      fill<L>(r, 0.0f);
+      fill<L>(b, 0.0f);
+      fill<L>(dT, 0.0f);
+      fill<L>(dn, 0.0f);
+      float ib = 1.0f, it = 1.0f;
+      if (real) {
+        load_row<L>(static_cast<const TR*>(a.residual) + row * a.residual_stride, a.width, r);
+        if (branch) load_row<L>(static_cast<const T*>(a.branch) + row * a.branch_stride, a.width, b);
+        if (g.total != nullptr)
+          load_row<L>(static_cast<const TR*>(g.total) + row * g.total_stride, a.width, dT);
+        if (g.normed != nullptr)
+          load_row<L>(static_cast<const T*>(g.normed) + row * g.normed_stride, a.width, dn);
+        ib = stats[2 * row];
+        it = stats[2 * row + 1];
       }
-      th = (scale * to_float(r[c]) + cz) * it;
-      q = dn != nullptr ? to_float(dn[c]) * to_float(pre[c]) : 0.0f;
-      dT = dtotal != nullptr ? to_float(dtotal[c]) : 0.0f;
-    };
-    float s[3] = {};
-    float cz, th, q, dT;
-    for (int64_t c = threadIdx.x; c < a.width; c += kThreads) {
-      pieces(c, cz, th, q, dT);
-      s[0] += q * th;
-      s[1] += (dT + it * q) * cz;
-      s[2] += th * cz;
+      float s[3] = {};
+      FHB_EACH(L) {
+        float cz = b[v][i];
+        if (post) cz = cz * ib * wpost[v][i];
+        if (gated) cz *= gate[v][i];
+        const float th = (scale * r[v][i] + cz) * it, q = dn[v][i] * wpre[v][i];
+        s[0] += q * th;
+        s[1] += (dT[v][i] + it * q) * cz;
+        s[2] += th * cz;
+      }
+      row_sum<L>(s, round);
+      if (!real) continue;
+      const float m1 = s[0] * inverse, m2 = (s[1] - it * m1 * s[2]) * inverse;
+      FHB_EACH(L) {
+        const float bh = b[v][i] * ib, z = post ? bh * wpost[v][i] : b[v][i];
+        const float cz = gated ? gate[v][i] * z : z;
+        const float th = (scale * r[v][i] + cz) * it, q = dn[v][i] * wpre[v][i];
+        const float dt = dT[v][i] + it * (q - th * m1);
+        const float dz = gated ? dt * gate[v][i] : dt;
+        spre[v][i] += dn[v][i] * th;
+        spost[v][i] += dz * bh;
+        sgate[v][i] += dt * z;
+        sscale += dt * r[v][i];
+        r[v][i] = scale * dt;
+        b[v][i] = post ? ib * (dz * wpost[v][i] - bh * m2) : dz;
+      }
+      if (g.residual != nullptr) store_row<L>(static_cast<TR*>(g.residual) + row * a.width, a.width, r);
+      if (g.branch != nullptr) store_row<L>(static_cast<T*>(g.branch) + row * a.width, a.width, b);
     }
-    block_sum(s);
-    const float m1 = s[0] / a.width, m2 = (s[1] - it * m1 * s[2]) / a.width;
-    for (int64_t c = threadIdx.x; c < a.width; c += kThreads) {
-      pieces(c, cz, th, q, dT);
-      const float dt = dT + it * (q - th * m1);
-      g.dt[row * a.width + c] = dt;
-      if (g.residual != nullptr) static_cast<TR*>(g.residual)[row * a.width + c] = from_float<TR>(scale * dt);
-      if (g.branch != nullptr) {
-        float p = gate != nullptr ? dt * to_float(gate[c]) : dt;
-        if (post != nullptr) p = ib * (p * to_float(post[c]) - to_float(b[c]) * ib * m2);
-        static_cast<T*>(g.branch)[row * a.width + c] = from_float<T>(p);
+    if (by_group) {
+      if (unit < count && g.want_gate) {
+        if (units.parts == 1)
+          store_row<L>(static_cast<T*>(g.gate) + group * a.width, a.width, sgate);
+        else
+          FHB_EACH(L) {
+            const int c = L::column(v, i);
+            if (c < a.width) g.gate_parts[unit * a.width + c] = sgate[v][i];
+          }
       }
+      fill<L>(sgate, 0.0f);
+    }
+  }
+  // the CTA's column sums: its slots' one after the other
+  extern __shared__ float columns[];
+  float* out = g.columns + static_cast<int64_t>(blockIdx.x) * 3 * a.width;
+  const auto leave = [&](const float (&x)[L::V][kVector], int which) {
+    if (L::Lanes == 0) {
+      FHB_EACH(L) {
+        const int c = L::column(v, i);
+        if (c < a.width) out[which * a.width + c] = x[v][i];
+      }
+      return;
+    }
+    __syncthreads();
+    FHB_EACH(L) {
+      const int c = L::column(v, i);
+      if (c < a.width) columns[L::slot() * a.width + c] = x[v][i];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
+      float sum = 0.0f;
+      for (int k = 0; k < L::slots(); ++k) sum += columns[k * a.width + c];
+      out[which * a.width + c] = sum;
+    }
+  };
+  if (g.want_pre) leave(spre, 0);
+  if (g.want_post) leave(spost, 1);
+  if (g.want_gate && !by_group) leave(sgate, 2);
+  if (g.want_scale) {
+    float s[1] = {sscale};
+    row_sum<L>(s, round);
+    __shared__ float by_slot[32];
+    __syncthreads();
+    if (L::lane() == 0) by_slot[L::slot()] = s[0];
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      float sum = 0.0f;
+      for (int k = 0; k < L::slots(); ++k) sum += by_slot[k];
+      g.scale_parts[blockIdx.x] = sum;
     }
   }
 }
 
-// Column part: one thread per column sums dwpre, dwpost and dgate over the rows in row order,
-// and each CTA leaves its part of da.
-template <typename TR, typename T>
-__global__ void __launch_bounds__(kThreads)
-    norm_columns_kernel(NormArgs a, NormGrads g, const float* __restrict__ stats, T* dpre,
-                        T* dpost, T* dgate, float* __restrict__ da_parts) {
-  const int64_t c = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x;
-  const float scale = a.scale_ptr != nullptr ? *a.scale_ptr : a.scale;
-  float spre = 0.0f, spost = 0.0f, sgate = 0.0f, sda[1] = {};
-  if (c < a.width) {
-    const T* post = static_cast<const T*>(a.post_weight);
-    const float wpost = post != nullptr ? to_float(post[c]) : 1.0f;
-    for (int64_t row = 0; row < a.rows; ++row) {
-      const float r = to_float(static_cast<const TR*>(a.residual)[row * a.residual_stride + c]);
-      const float ib = stats[2 * row], it = stats[2 * row + 1];
-      const float dt = g.dt[row * a.width + c];
-      const int64_t group = row / a.gate_rows;
-      const float gate = a.gate != nullptr ? to_float(static_cast<const T*>(a.gate)[group * a.width + c]) : 1.0f;
-      float bh = 0.0f;
-      if (a.branch != nullptr) bh = to_float(static_cast<const T*>(a.branch)[row * a.branch_stride + c]) * ib;
-      if (g.normed != nullptr)
-        spre += to_float(static_cast<const T*>(g.normed)[row * g.normed_stride + c]) *
-                ((scale * r + gate * bh * wpost) * it);
-      spost += dt * gate * bh;
-      sgate += dt * bh * wpost;
-      sda[0] += dt * r;
-      if (dgate != nullptr && (row + 1 == a.rows || (row + 1) / a.gate_rows != group)) {
-        dgate[group * a.width + c] = from_float<T>(sgate);
-        sgate = 0.0f;
-      }
+// Second kernel of the column sums: out[c] = the rows in[k * stride + c] in a fixed order. One
+// task per blockIdx.y: dwpre, dwpost, dgate of all rows; the scale; then the gate groups.
+struct Totals {
+  const float* columns;
+  const float* gate_parts;
+  const float* scale_parts;
+  int64_t grid, parts, width;
+  void *pre, *post, *gate;
+  float* scale;
+  bool by_group;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) norm_totals_kernel(Totals t) {
+  const int64_t task = blockIdx.y;
+  const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+  if (task == 3) {
+    if (blockIdx.x != 0 || t.scale == nullptr) return;
+    __shared__ double by_thread[256];
+    double s = 0.0;
+    for (int64_t k = threadIdx.x; k < t.grid; k += 256) s += t.scale_parts[k];
+    by_thread[threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      s = 0.0;
+      for (int k = 0; k < 256; ++k) s += by_thread[k];
+      *t.scale = static_cast<float>(s);
     }
-    if (dpre != nullptr) dpre[c] = from_float<T>(spre);
-    if (dpost != nullptr) dpost[c] = from_float<T>(spost);
-    if (dgate != nullptr && a.rows == 0) dgate[c] = from_float<T>(0.0f);
+    return;
   }
-  block_sum(sda);
-  if (threadIdx.x == 0) da_parts[blockIdx.x] = sda[0];
+  const float* in;
+  int64_t rows, stride;
+  T* out;
+  if (task < 3) {
+    in = t.columns + task * t.width;
+    rows = t.grid;
+    stride = 3 * t.width;
+    out = static_cast<T*>(task == 0 ? t.pre : task == 1 ? t.post : t.by_group ? nullptr : t.gate);
+  } else {
+    in = t.gate_parts + (task - 4) * t.parts * t.width;
+    rows = t.parts;
+    stride = t.width;
+    out = static_cast<T*>(t.gate) + (task - 4) * t.width;
+  }
+  if (out == nullptr) return;
+  __shared__ float by_group[8][32];
+  const int64_t c = blockIdx.x * 32ll + lane;
+  float s = 0.0f;
+  if (c < t.width) {
+    int64_t k = group;
+    for (; k + 56 < rows; k += 64) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = in[(k + 8 * j) * stride + c];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    for (; k < rows; k += 8) s += in[k * stride + c];
+  }
+  by_group[group][lane] = s;
+  __syncthreads();
+  if (group == 0 && c < t.width) {
+    s = 0.0f;
+    for (int k = 0; k < 8; ++k) s += by_group[k][lane];
+    out[c] = from_float<T>(s);
+  }
 }
 
-__global__ void sum_parts_kernel(const float* __restrict__ parts, int64_t count, float* out) {
-  double s = 0.0;
-  for (int64_t i = 0; i < count; ++i) s += parts[i];
-  *out = static_cast<float>(s);
-}
-
+// ---- launches ----
 NormArgs arguments(const fhb_norm_problem& p) {
-  return {p.residual, p.branch, p.pre_weight, p.post_weight, p.gate, p.rows, p.width,
-          p.residual_stride, p.branch_stride, p.gate != nullptr ? p.gate_rows : (p.rows > 0 ? p.rows : 1),
-          p.residual_scale_ptr, p.residual_scale, p.eps};
+  return {p.residual, p.branch, p.pre_weight, p.post_weight, p.gate, p.rows, p.residual_stride,
+          p.branch_stride, p.gate != nullptr ? p.gate_rows : std::max<int64_t>(p.rows, 1),
+          static_cast<int>(p.width), p.residual_scale_ptr, p.residual_scale, p.eps};
+}
+
+bool wide_rows(const void* p, int64_t stride, int dtype) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 &&
+         stride * static_cast<int64_t>(dtype_bytes(dtype)) % 16 == 0;
+}
+bool wide_inputs(const fhb_norm_problem& p) {
+  return p.width % kVector == 0 && wide_rows(p.residual, p.residual_stride, p.residual_dtype) &&
+         wide_rows(p.branch, p.branch_stride, p.dtype) && wide_rows(p.pre_weight, 0, p.dtype) &&
+         wide_rows(p.post_weight, 0, p.dtype) && wide_rows(p.gate, p.width, p.dtype);
+}
+
+// Threads of a row: 8 values each, a power of 2 of them, at most 1,024 (rows wider than 8,192
+// take four vectors a thread).
+int row_threads(int64_t width) {
+  const int64_t need = (width + kVector - 1) / kVector;
+  int n = 8;
+  while (n < need && n < 1024) n *= 2;
+  return n;
+}
+int slots_of(int threads) { return threads <= 32 ? 256 / threads : 1; }
+int block_of(int threads) { return threads <= 32 ? 256 : threads; }
+
+// CTAs: enough for 1,536 threads on every SM in the forward, 1,024 in the backward (its sums
+// take registers, and every CTA leaves a row of column sums).
+int64_t ctas(int threads, int per_sm_threads, const DeviceInfo& dev) {
+  return static_cast<int64_t>(dev.sms) * std::max(1, per_sm_threads / block_of(threads));
+}
+
+Units units_of(const fhb_norm_problem& p, const DeviceInfo& dev) {
+  const int threads = row_threads(p.width);
+  Units u;
+  u.group_rows = p.gate != nullptr ? std::min(p.gate_rows, std::max<int64_t>(p.rows, 1))
+                                   : std::max<int64_t>(p.rows, 1);
+  u.groups = std::max<int64_t>(1, (p.rows + u.group_rows - 1) / u.group_rows);
+  u.slots = ctas(threads, 1024, dev) * slots_of(threads);
+  u.parts = std::min(std::max<int64_t>(1, u.slots / u.groups), u.group_rows);
+  u.part_rows = (u.group_rows + u.parts - 1) / u.parts;
+  u.parts = (u.group_rows + u.part_rows - 1) / u.part_rows;
+  const int64_t count = u.groups * u.parts;
+  u.grid = std::min((count + slots_of(threads) - 1) / slots_of(threads), ctas(threads, 1024, dev));
+  return u;
+}
+
+// Calls body(Layout) with the layout for the width.
+template <bool Wide, typename Body>
+cudaError_t with_layout(int64_t width, Body body) {
+  const int threads = row_threads(width);
+  if (width > 1024 * kVector) return body(Layout<0, 1024, 4, Wide>{});
+  switch (threads) {
+    case 8: return body(Layout<8, 256, 1, Wide>{});
+    case 16: return body(Layout<16, 256, 1, Wide>{});
+    case 32: return body(Layout<32, 256, 1, Wide>{});
+    case 512: return body(Layout<0, 512, 1, Wide>{});
+    case 1024: return body(Layout<0, 1024, 1, Wide>{});
+    default: return body(Layout<0, 256, 1, Wide>{});
+  }
+}
+template <typename Body>
+cudaError_t with_layout(bool wide, int64_t width, Body body) {
+  return wide ? with_layout<true>(width, body) : with_layout<false>(width, body);
 }
 
 template <typename TR, typename T>
 cudaError_t forward(const fhb_norm_problem& p, void* total, void* normed, float* stats,
                     const DeviceInfo& dev, cudaStream_t stream) {
-  const int64_t most = 8ll * dev.sms;
-  norm_kernel<TR, T><<<static_cast<unsigned>(p.rows < most ? p.rows : most), kThreads, 0, stream>>>(
-      arguments(p), static_cast<TR*>(total), static_cast<T*>(normed), stats);
-  return cudaGetLastError();
+  const bool wide = wide_inputs(p) && wide_rows(total, p.width, p.residual_dtype) &&
+                    wide_rows(normed, p.width, p.dtype);
+  const int threads = row_threads(p.width);
+  const int64_t need = (p.rows + slots_of(threads) - 1) / slots_of(threads);
+  const unsigned grid = static_cast<unsigned>(std::min(need, ctas(threads, 1536, dev)));
+  return with_layout(wide, p.width, [&](auto layout) {
+    norm_kernel<decltype(layout), TR, T><<<grid, block_of(threads), 0, stream>>>(
+        arguments(p), static_cast<TR*>(total), static_cast<T*>(normed), stats);
+    return cudaGetLastError();
+  });
+}
+
+struct Room {
+  float *columns, *gate_parts, *scale_parts;
+  size_t bytes;
+};
+Room room_of(const fhb_norm_problem& p, const Units& u, void* base) {
+  float* at = static_cast<float*>(base);
+  const int64_t columns = (u.grid * 3 * p.width + 31) / 32 * 32;
+  const int64_t gates = u.groups > 1 && u.parts > 1 ? (u.groups * u.parts * p.width + 31) / 32 * 32 : 0;
+  return {at, at + columns, at + columns + gates,
+          static_cast<size_t>(columns + gates + (u.grid + 31) / 32 * 32) * 4};
 }
 
 template <typename TR, typename T>
-cudaError_t backward(const fhb_norm_problem& p, const NormGrads& g, const fhb_norm_grads& out,
-                     const float* stats, float* parts, const DeviceInfo& dev, cudaStream_t stream) {
-  const int64_t most = 8ll * dev.sms;
-  if (p.rows > 0)
-    norm_backward_kernel<TR, T><<<static_cast<unsigned>(p.rows < most ? p.rows : most), kThreads, 0, stream>>>(
-        arguments(p), g, stats);
-  const int64_t blocks = (p.width + kThreads - 1) / kThreads;
-  norm_columns_kernel<TR, T><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-      arguments(p), g, stats, static_cast<T*>(out.pre_weight), static_cast<T*>(out.post_weight),
-      static_cast<T*>(out.gate), parts);
-  if (out.residual_scale != nullptr)
-    sum_parts_kernel<<<1, 1, 0, stream>>>(parts, blocks, out.residual_scale);
+cudaError_t backward(const fhb_norm_problem& p, const NormGrads& g, const Units& u, const Totals& t,
+                     const float* stats, bool wide, cudaStream_t stream) {
+  const int threads = row_threads(p.width);
+  const size_t smem = threads <= 32 ? static_cast<size_t>(slots_of(threads)) * p.width * 4 : 0;
+  const cudaError_t e = with_layout(wide, p.width, [&](auto layout) {
+    norm_backward_kernel<decltype(layout), TR, T>
+        <<<static_cast<unsigned>(u.grid), block_of(threads), smem, stream>>>(arguments(p), g, u, stats);
+    return cudaGetLastError();
+  });
+  if (e != cudaSuccess || !(g.want_pre || g.want_post || g.want_gate || g.want_scale)) return e;
+  const bool groups = t.by_group && g.want_gate && u.parts > 1;
+  const dim3 grid(static_cast<unsigned>((p.width + 31) / 32), static_cast<unsigned>(4 + (groups ? u.groups : 0)));
+  norm_totals_kernel<T><<<grid, 256, 0, stream>>>(t);
   return cudaGetLastError();
-}
-
-int64_t parts_bytes(const fhb_norm_problem& p) {
-  return ((p.width + kThreads - 1) / kThreads * 4 + 15) & ~15ll;
 }
 
 }  // namespace
@@ -237,8 +541,8 @@ cudaError_t launch_residual_norm(const fhb_norm_problem& p, void* total, void* n
   return forward<bf16, bf16>(p, total, normed, stats, dev, stream);
 }
 
-size_t residual_norm_workspace_bytes(const fhb_norm_problem& p, const DeviceInfo&) {
-  return parts_bytes(p) + p.rows * p.width * 4;
+size_t residual_norm_workspace_bytes(const fhb_norm_problem& p, const DeviceInfo& dev) {
+  return room_of(p, units_of(p, dev), nullptr).bytes;
 }
 
 cudaError_t launch_residual_norm_backward(const fhb_norm_problem& p, const void* grad_total,
@@ -246,14 +550,23 @@ cudaError_t launch_residual_norm_backward(const fhb_norm_problem& p, const void*
                                           int64_t grad_normed_stride, const float* stats,
                                           const fhb_norm_grads& out, void* workspace,
                                           const DeviceInfo& dev, cudaStream_t stream) {
-  float* parts = static_cast<float*>(workspace);
+  const Units u = units_of(p, dev);
+  const Room room = room_of(p, u, workspace);
   const NormGrads g{grad_total, grad_normed, grad_total_stride, grad_normed_stride, out.residual,
-                    out.branch,
-                    reinterpret_cast<float*>(static_cast<char*>(workspace) + parts_bytes(p))};
+                    out.branch, out.gate, room.columns, room.gate_parts, room.scale_parts,
+                    out.pre_weight != nullptr, out.post_weight != nullptr, out.gate != nullptr,
+                    out.residual_scale != nullptr};
+  const Totals t{room.columns, room.gate_parts, room.scale_parts, u.grid, u.parts, p.width,
+                 out.pre_weight, out.post_weight, out.gate, out.residual_scale,
+                 p.gate != nullptr && u.groups > 1};
+  const bool wide = wide_inputs(p) && wide_rows(grad_total, grad_total_stride, p.residual_dtype) &&
+                    wide_rows(grad_normed, grad_normed_stride, p.dtype) &&
+                    wide_rows(out.residual, p.width, p.residual_dtype) &&
+                    wide_rows(out.branch, p.width, p.dtype) && wide_rows(out.gate, p.width, p.dtype);
   if (p.residual_dtype == FHB_DTYPE_F32)
-    return p.dtype == FHB_DTYPE_F32 ? backward<float, float>(p, g, out, stats, parts, dev, stream)
-                                    : backward<float, bf16>(p, g, out, stats, parts, dev, stream);
-  return backward<bf16, bf16>(p, g, out, stats, parts, dev, stream);
+    return p.dtype == FHB_DTYPE_F32 ? backward<float, float>(p, g, u, t, stats, wide, stream)
+                                    : backward<float, bf16>(p, g, u, t, stats, wide, stream);
+  return backward<bf16, bf16>(p, g, u, t, stats, wide, stream);
 }
 
 }  // namespace fhb

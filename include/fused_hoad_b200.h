@@ -354,6 +354,7 @@ int fhb_ffn_backward(const fhb_ffn_problem* problem, const void* grad_y, int64_t
  * post_weight are NULL too). gate (NULL: 1) has one contiguous row of `width` values for every
  * gate_rows consecutive rows (`rows` of them share row 0 of a per-channel gate; 1: a full one).
  * scale is *residual_scale_ptr (device, float) where that is given, else residual_scale.
+ * width is at most 32,768 (FHB_ERR_TOO_LARGE beyond).
  */
 typedef struct fhb_norm_problem {
   int64_t rows, width;
