@@ -1,7 +1,15 @@
 // One AdamW step over many tensors, moments in FP32 or in 8 bits (e4m3 codes of m and sqrt(v)
-// with one scale per block of 256 values). The arithmetic on the moments is the formula's,
-// operation by operation (no contraction into fused multiply-adds), so the moments and codes
-// are those of the same formula in any IEEE FP32 arithmetic.
+// with one scale per block of 256 values).
+//
+// Bound by memory: 28 bytes a value with FP32 parameters and states, 10 with bfloat16 parameters
+// and 8-bit states. A warp takes a block of 256 values, 8 neighbours a lane, so every array is
+// moved in whole sectors and an 8-bit block's largest value is one warp maximum away. The
+// moments are the formula's, operation by operation (no contraction into fused multiply-adds;
+// quotients and roots correctly rounded), so moments, codes and scales are those of the same
+// formula in any IEEE FP32 arithmetic; the parameter's update uses approximate quotients (2^-22
+// of the update). The tensors' addresses travel as kernel arguments: nothing is copied to the
+// device before the launch, and the step counter is advanced by the last CTA to finish.
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -12,144 +20,298 @@ namespace fhb {
 namespace {
 
 constexpr int kBlock = FHB_ADAMW_BLOCK;
-constexpr int kMaxTensors = 32;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+// Tensors of one launch: its arguments hold 4 KB cheaply and 32 KB at most.
+constexpr int kFewTensors = 40, kManyTensors = 400;
+// The step counter's upper bits count the CTAs that are done (0 between launches).
+constexpr int kStepBits = 40;
+constexpr unsigned long long kStepMask = (1ull << kStepBits) - 1;
 
-struct AdamwConstants {
-  double beta1, beta2, lr;  // for the bias corrections
+struct Constants {
+  double beta1, beta2, lr;           // for the bias corrections
   float b1, c1, b2, c2, decay, eps;  // beta, 1 - beta, 1 - lr weight_decay
 };
-struct AdamwBatch {
-  fhb_adamw_tensor tensor[kMaxTensors];
-  int64_t first_block[kMaxTensors + 1];  // running count of 256-value blocks
+template <int Capacity>
+struct Batch {
+  fhb_adamw_tensor tensor[Capacity];
+  int64_t first_block[Capacity + 1];  // running count of 256-value blocks
+  unsigned char wide[Capacity];       // every array of the tensor is aligned for 8 values
   int tensors;
+  int advances;  // the last launch of the step
 };
 
-// The maximum of two magnitudes; NaN wins.
-__device__ __forceinline__ float max_or_nan(float a, float b) {
-  return a != a ? a : (b != b ? b : fmaxf(a, b));
-}
-__device__ __forceinline__ float warp_max_or_nan(float v) {
+// ---- 8 neighbours of an array ----
+__device__ __forceinline__ void load8(const float* p, bool wide, int left, float (&x)[8]) {
+  if (wide && left >= 8) {
+    uint32_t w[8];
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]),
+                   "=r"(w[6]), "=r"(w[7])
+                 : "l"(p)
+                 : "memory");
 #pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) v = max_or_nan(v, __shfl_xor_sync(0xffffffffu, v, m));
-  return v;
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = i < left ? p[i] : 0.0f;
+}
+__device__ __forceinline__ void store8(float* p, bool wide, int left, const float (&x)[8]) {
+  if (wide && left >= 8) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p),
+                 "r"(__float_as_uint(x[0])), "r"(__float_as_uint(x[1])), "r"(__float_as_uint(x[2])),
+                 "r"(__float_as_uint(x[3])), "r"(__float_as_uint(x[4])), "r"(__float_as_uint(x[5])),
+                 "r"(__float_as_uint(x[6])), "r"(__float_as_uint(x[7]))
+                 : "memory");
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < left) p[i] = x[i];
+}
+__device__ __forceinline__ void load8(const bf16* p, bool wide, int left, float (&x)[8]) {
+  if (wide && left >= 8) {
+    const uint4 w = *reinterpret_cast<const uint4*>(p);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(u[i] << 16);
+      x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = i < left ? to_float(p[i]) : 0.0f;
+}
+__device__ __forceinline__ void store8(bf16* p, bool wide, int left, const float (&x)[8]) {
+  if (wide && left >= 8) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
+    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < left) p[i] = from_float<bf16>(x[i]);
+}
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, bool wide, int left) {
+  if (wide && left >= 8) return *reinterpret_cast<const uint2*>(p);
+  unsigned long long w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < left) w |= static_cast<unsigned long long>(p[i]) << (8 * i);
+  return make_uint2(static_cast<uint32_t>(w), static_cast<uint32_t>(w >> 32));
+}
+__device__ __forceinline__ void decode8(uint2 codes, float scale, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t pair = ((i < 2 ? codes.x : codes.y) >> (16 * (i & 1))) & 0xFFFFu;
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3);
+    const float2 v = __half22float2(__half2(h));
+    x[2 * i] = __fmul_rn(v.x, scale);
+    x[2 * i + 1] = __fmul_rn(v.y, scale);
+  }
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, bool wide, int left, const float (&units)[8]) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i / 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(units[2 * i], units[2 * i + 1]),
+                                                               __NV_SATFINITE, __NV_E4M3))
+                << (16 * (i & 1));
+  if (wide && left >= 8) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < left) p[i] = static_cast<uint8_t>(w[i / 4] >> (8 * (i & 3)));
+}
+
+// Largest of non-negative values over the warp; NaN (whatever its sign bit was) wins: as bit
+// patterns, NaN > infinity > numbers in order.
+__device__ __forceinline__ float warp_largest(const float (&x)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, top));
 }
 __device__ __forceinline__ float block_scale(float largest) {
-  if (largest == INFINITY) return NAN;  // as a NaN in the block: all of it decodes to NaN
+  if (!(largest < INFINITY)) return NAN;  // a block with a NaN or infinity decodes to NaN
   const float s = __fmul_rn(largest, 1.0f / 448.0f);
-  return s < 0x1p-126f ? 0x1p-126f : s;  // a NaN stays
+  return s < 0x1p-126f ? 0x1p-126f : s;
 }
-__device__ __forceinline__ uint8_t encode(float x) {
-  return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
-}
-__device__ __forceinline__ float decode(uint8_t c) {
-  __nv_fp8_e4m3 v;
-  v.__x = c;
-  return static_cast<float>(v);
-}
-
-// One warp per block of 256 values, eight per lane.
-template <bool Eight>
-__global__ void __launch_bounds__(256)
-    adamw_kernel(const __grid_constant__ AdamwBatch batch, AdamwConstants k,
-                 const int64_t* __restrict__ step) {
-  const int64_t block = (blockIdx.x * 256ll + threadIdx.x) / 32;
-  const int lane = threadIdx.x % 32;
-  if (block >= batch.first_block[batch.tensors]) return;
-  int at = 0;
-  while (block >= batch.first_block[at + 1]) ++at;
-  const fhb_adamw_tensor& t = batch.tensor[at];
-  const int64_t own = block - batch.first_block[at], base = own * kBlock;
-  const double now = static_cast<double>(*step + 1);
-  const float step_size = static_cast<float>(k.lr / (1.0 - pow(k.beta1, now)));
-  const float root = static_cast<float>(sqrt(1.0 - pow(k.beta2, now)));
-  float sm = 0.0f, sv = 0.0f;
-  if (Eight) {
-    sm = t.exp_avg_scale[own];
-    sv = t.exp_avg_sq_scale[own];
+// x[i] / scale, correctly rounded. One reciprocal for the block and a remainder step each:
+// with r the correctly rounded 1 / s, q = x r is off by an ulp at most and q + (x - q s) r is
+// the correctly rounded quotient, as long as the remainder does not underflow -- blocks whose
+// largest value is that small divide.
+__device__ __forceinline__ void divide8(float (&x)[8], float scale) {
+  if (scale < 0x1p-90f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __fdiv_rn(x[i], scale);
+    return;
   }
-  float m[8], v[8];
-  float top_m = 0.0f, top_v = 0.0f;
+  const float r = __frcp_rn(scale);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int64_t j = base + lane + 32 * i;
-    m[i] = v[i] = 0.0f;
-    if (j >= t.count) continue;
-    const bool wide = t.dtype == FHB_DTYPE_F32;
-    const float g = wide ? static_cast<const float*>(t.grad)[j]
-                         : to_float(static_cast<const bf16*>(t.grad)[j]);
-    const float p = wide ? static_cast<float*>(t.param)[j] : to_float(static_cast<bf16*>(t.param)[j]);
-    float m0, v0;
-    if (Eight) {
-      m0 = __fmul_rn(decode(static_cast<uint8_t*>(t.exp_avg)[j]), sm);
-      const float s = __fmul_rn(decode(static_cast<uint8_t*>(t.exp_avg_sq)[j]), sv);
-      v0 = __fmul_rn(s, s);
-    } else {
-      m0 = static_cast<float*>(t.exp_avg)[j];
-      v0 = static_cast<float*>(t.exp_avg_sq)[j];
-    }
-    m[i] = __fadd_rn(__fmul_rn(m0, k.b1), __fmul_rn(g, k.c1));
-    v[i] = __fadd_rn(__fmul_rn(v0, k.b2), __fmul_rn(__fmul_rn(g, g), k.c2));
-    const float denominator = sqrtf(v[i]) / root + k.eps;
-    const float next = p * k.decay - step_size * (m[i] / denominator);
-    if (wide) static_cast<float*>(t.param)[j] = next;
-    else static_cast<bf16*>(t.param)[j] = from_float<bf16>(next);
+    const float q = __fmul_rn(x[i], r);
+    x[i] = __fmaf_rn(__fmaf_rn(-q, scale, x[i]), r, q);
+  }
+}
+
+template <bool Eight, typename T>
+__device__ __forceinline__ void update_block(const fhb_adamw_tensor& t, bool wide, int64_t own,
+                                             int lane, const Constants& k, float step_size,
+                                             float inverse_root) {
+  const int64_t at = own * kBlock + lane * 8;
+  const int left = static_cast<int>(min(t.count - at, int64_t{8}));  // may be negative
+  float g[8], p[8], m[8], v[8];
+  load8(static_cast<const T*>(t.grad) + at, wide, left, g);
+  load8(static_cast<const T*>(t.param) + at, wide, left, p);
+  if (Eight) {
+    const uint2 cm = load_codes(static_cast<const uint8_t*>(t.exp_avg) + at, wide, left);
+    const uint2 cv = load_codes(static_cast<const uint8_t*>(t.exp_avg_sq) + at, wide, left);
+    decode8(cm, t.exp_avg_scale[own], m);
+    decode8(cv, t.exp_avg_sq_scale[own], v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], v[i]);
+  } else {
+    load8(static_cast<const float*>(t.exp_avg) + at, wide, left, m);
+    load8(static_cast<const float*>(t.exp_avg_sq) + at, wide, left, v);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    m[i] = __fadd_rn(__fmul_rn(m[i], k.b1), __fmul_rn(g[i], k.c1));
+    v[i] = __fadd_rn(__fmul_rn(v[i], k.b2), __fmul_rn(__fmul_rn(g[i], g[i]), k.c2));
+  }
+  if (!Eight) {
+    store8(static_cast<float*>(t.exp_avg) + at, wide, left, m);
+    store8(static_cast<float*>(t.exp_avg_sq) + at, wide, left, v);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
     if (Eight) {
       v[i] = __fsqrt_rn(v[i]);
-      top_m = max_or_nan(top_m, fabsf(m[i]));
-      top_v = max_or_nan(top_v, v[i]);
     } else {
-      static_cast<float*>(t.exp_avg)[j] = m[i];
-      static_cast<float*>(t.exp_avg_sq)[j] = v[i];
+      asm("sqrt.approx.f32 %0, %0;" : "+f"(v[i]));
     }
+    const float denominator = fmaf(v[i], inverse_root, k.eps);
+    // the denominator may be 0 (eps 0): 0 / 0 and x / 0 as IEEE has them
+    p[i] = fmaf(-step_size, __fdividef(m[i], denominator), p[i] * k.decay);
   }
+  store8(static_cast<T*>(t.param) + at, wide, left, p);
   if (!Eight) return;
-  const float new_sm = block_scale(warp_max_or_nan(top_m));
-  const float new_sv = block_scale(warp_max_or_nan(top_v));
+  const float scale_m = block_scale(warp_largest(m)), scale_v = block_scale(warp_largest(v));
+  divide8(m, scale_m);
+  float units[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t j = base + lane + 32 * i;
-    if (j >= t.count) continue;
-    float units = __fdiv_rn(v[i], new_sv);
-    if (v[i] > 0.0f) units = units < 0x1p-9f ? 0x1p-9f : units;
-    static_cast<uint8_t*>(t.exp_avg)[j] = encode(__fdiv_rn(m[i], new_sm));
-    static_cast<uint8_t*>(t.exp_avg_sq)[j] = encode(units);
-  }
+  for (int i = 0; i < 8; ++i) units[i] = v[i];
+  divide8(units, scale_v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (v[i] > 0.0f && units[i] < 0x1p-9f) units[i] = 0x1p-9f;  // not zero stays not zero
+  store_codes(static_cast<uint8_t*>(t.exp_avg) + at, wide, left, m);
+  store_codes(static_cast<uint8_t*>(t.exp_avg_sq) + at, wide, left, units);
   if (lane == 0) {
-    t.exp_avg_scale[own] = new_sm;
-    t.exp_avg_sq_scale[own] = new_sv;
+    t.exp_avg_scale[own] = scale_m;
+    t.exp_avg_sq_scale[own] = scale_v;
   }
 }
 
-__global__ void advance_kernel(int64_t* step) { *step += 1; }
+template <bool Eight, int Capacity>
+__global__ void __launch_bounds__(kThreads)
+    adamw_kernel(const __grid_constant__ Batch<Capacity> batch, const Constants k,
+                 unsigned long long* step) {
+  __shared__ float corrections[2];
+  __shared__ unsigned long long now;
+  if (threadIdx.x == 0) {
+    // volatile: other CTAs add to the upper bits
+    now = (*const_cast<volatile unsigned long long*>(step) & kStepMask) + 1;
+    const double t = static_cast<double>(now);
+    corrections[0] = static_cast<float>(k.lr / (1.0 - pow(k.beta1, t)));
+    corrections[1] = static_cast<float>(1.0 / sqrt(1.0 - pow(k.beta2, t)));
+  }
+  __syncthreads();
+  const float step_size = corrections[0], inverse_root = corrections[1];
+  const int lane = threadIdx.x % 32;
+  const int64_t blocks = batch.first_block[batch.tensors];
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kWarps;
+  int at = 0;
+  for (int64_t block = blockIdx.x * static_cast<int64_t>(kWarps) + threadIdx.x / 32; block < blocks;
+       block += stride) {
+    // the tensor: the last one whose first block is not past this (blocks only go up)
+    int low = at, high = batch.tensors;
+    while (high - low > 1) {
+      const int mid = (low + high) / 2;
+      if (batch.first_block[mid] <= block) low = mid;
+      else high = mid;
+    }
+    at = low;
+    const fhb_adamw_tensor& t = batch.tensor[at];
+    const int64_t own = block - batch.first_block[at];
+    if (t.dtype == FHB_DTYPE_F32)
+      update_block<Eight, float>(t, batch.wide[at] != 0, own, lane, k, step_size, inverse_root);
+    else
+      update_block<Eight, bf16>(t, batch.wide[at] != 0, own, lane, k, step_size, inverse_root);
+  }
+  if (!batch.advances) return;
+  __syncthreads();
+  if (threadIdx.x == 0 && atomicAdd(step, 1ull << kStepBits) >> kStepBits == gridDim.x - 1)
+    *step = now;  // every CTA has read the counter
+}
+
+bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+template <int Capacity>
+cudaError_t launch(const fhb_adamw_tensor* tensors, int64_t count, bool eight, bool advances,
+                   unsigned long long* step, const Constants& k, const DeviceInfo& dev,
+                   cudaStream_t stream) {
+  Batch<Capacity> batch{};
+  batch.tensors = static_cast<int>(count);
+  batch.advances = advances;
+  for (int i = 0; i < batch.tensors; ++i) {
+    const fhb_adamw_tensor& t = tensors[i];
+    batch.tensor[i] = t;
+    batch.first_block[i + 1] = batch.first_block[i] + (t.count + kBlock - 1) / kBlock;
+    const uintptr_t of_param = 8 * dtype_bytes(t.dtype), of_state = eight ? 8 : 32;
+    batch.wide[i] = aligned(t.param, of_param) && aligned(t.grad, of_param) &&
+                    aligned(t.exp_avg, of_state) && aligned(t.exp_avg_sq, of_state);
+  }
+  const int64_t need = (batch.first_block[count] + kWarps - 1) / kWarps;
+  if (need == 0 && !advances) return cudaSuccess;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(need, 1), 6ll * dev.sms));
+  if (eight)
+    adamw_kernel<true, Capacity><<<grid, kThreads, 0, stream>>>(batch, k, step);
+  else
+    adamw_kernel<false, Capacity><<<grid, kThreads, 0, stream>>>(batch, k, step);
+  return cudaGetLastError();
+}
 
 }  // namespace
 
 cudaError_t launch_adamw(const fhb_adamw_tensor* tensors, int64_t n_tensors, int state_bits,
                          int64_t* step, double lr, double beta1, double beta2, double eps,
-                         double weight_decay, cudaStream_t stream) {
-  const AdamwConstants k{beta1, beta2, lr, static_cast<float>(beta1), static_cast<float>(1.0 - beta1),
-                         static_cast<float>(beta2), static_cast<float>(1.0 - beta2),
-                         static_cast<float>(1.0 - lr * weight_decay), static_cast<float>(eps)};
-  for (int64_t first = 0; first < n_tensors; first += kMaxTensors) {
-    AdamwBatch batch{};
-    batch.tensors = static_cast<int>(std::min<int64_t>(kMaxTensors, n_tensors - first));
-    for (int i = 0; i < batch.tensors; ++i) {
-      batch.tensor[i] = tensors[first + i];
-      batch.first_block[i + 1] = batch.first_block[i] + (tensors[first + i].count + kBlock - 1) / kBlock;
-    }
-    const int64_t blocks = batch.first_block[batch.tensors];
-    if (blocks == 0) continue;
-    const int64_t grid = (blocks + 7) / 8;
-    if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
-    if (state_bits == 8)
-      adamw_kernel<true><<<static_cast<unsigned>(grid), 256, 0, stream>>>(batch, k, step);
-    else
-      adamw_kernel<false><<<static_cast<unsigned>(grid), 256, 0, stream>>>(batch, k, step);
-    const cudaError_t e = cudaGetLastError();
+                         double weight_decay, const DeviceInfo& dev, cudaStream_t stream) {
+  const Constants k{beta1, beta2, lr, static_cast<float>(beta1), static_cast<float>(1.0 - beta1),
+                    static_cast<float>(beta2), static_cast<float>(1.0 - beta2),
+                    static_cast<float>(1.0 - lr * weight_decay), static_cast<float>(eps)};
+  auto* counter = reinterpret_cast<unsigned long long*>(step);
+  int64_t first = 0;
+  do {
+    const int64_t left = n_tensors - first;
+    const int64_t count = std::min<int64_t>(left, kManyTensors);
+    const bool last = count == left;
+    const cudaError_t e =
+        count <= kFewTensors
+            ? launch<kFewTensors>(tensors + first, count, state_bits == 8, last, counter, k, dev, stream)
+            : launch<kManyTensors>(tensors + first, count, state_bits == 8, last, counter, k, dev, stream);
     if (e != cudaSuccess) return e;
-  }
-  advance_kernel<<<1, 1, 0, stream>>>(step);
-  return cudaGetLastError();
+    first += count;
+  } while (first < n_tensors);
+  return cudaSuccess;
 }
 
 }  // namespace fhb

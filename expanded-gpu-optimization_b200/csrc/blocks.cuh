@@ -65,6 +65,6 @@ cudaError_t launch_residual_norm_backward(const fhb_norm_problem& p, const void*
 // ---- adamw.cu ----
 cudaError_t launch_adamw(const fhb_adamw_tensor* tensors, int64_t n_tensors, int state_bits,
                          int64_t* step, double lr, double beta1, double beta2, double eps,
-                         double weight_decay, cudaStream_t stream);
+                         double weight_decay, const DeviceInfo& dev, cudaStream_t stream);
 
 }  // namespace fhb

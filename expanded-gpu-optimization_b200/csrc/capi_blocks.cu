@@ -226,7 +226,7 @@ int fhb_adamw_step(const fhb_adamw_tensor* tensors, int64_t n_tensors, int state
   const int code = fhb::current_device_info(&dev);
   if (code != FHB_OK) return code;
   return fhb::record_cuda_error(fhb::launch_adamw(tensors, n_tensors, state_bits, step, lr, beta1,
-                                                  beta2, eps, weight_decay, stream));
+                                                  beta2, eps, weight_decay, *dev, stream));
 }
 
 }  // extern "C"

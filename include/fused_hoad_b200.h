@@ -394,8 +394,9 @@ int fhb_residual_norm_backward(const fhb_norm_problem* problem, const void* grad
  *     scale = max(max|value| * (1/448), 2^-126),  code = e4m3(value / scale), nearest even;
  * a sqrt(v) that is not zero takes at least the smallest code, 2^-9. The update uses m and v
  * before they are coded. A block with a NaN or infinite value decodes to NaN throughout.
- * `step` is a device int64 counter of the steps taken so far, read (t = step + 1) and then
- * advanced on the stream, so the call can be replayed from a CUDA graph.
+ * `step` is a device int64 counter of the steps taken so far (0 to 2^40 - 2), read (t = step +
+ * 1) and then advanced on the stream, so the call can be replayed from a CUDA graph; while the
+ * call runs its upper bits count finished CTAs, so nothing else may read or write it then.
  */
 #define FHB_ADAMW_BLOCK 256
 typedef struct fhb_adamw_tensor {
