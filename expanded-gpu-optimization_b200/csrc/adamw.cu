@@ -15,6 +15,7 @@
 #include <algorithm>
 
 #include "blocks.cuh"
+#include "common.cuh"
 
 namespace fhb {
 namespace {
@@ -22,6 +23,7 @@ namespace {
 constexpr int kBlock = FHB_ADAMW_BLOCK;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kResident = 4, kResidentEight = 3;  // CTAs an SM holds
 // Tensors of one launch: its arguments hold 4 KB cheaply and 32 KB at most.
 constexpr int kFewTensors = 40, kManyTensors = 400;
 // The step counter's upper bits count the CTAs that are done (0 between launches).
@@ -42,23 +44,13 @@ struct Batch {
 };
 
 // ---- 8 neighbours of an array ----
-__device__ __forceinline__ void load8(const float* p, bool wide, int left, float (&x)[8]) {
-  if (wide && left >= 8) {
-    uint32_t w[8];
-    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]),
-                   "=r"(w[6]), "=r"(w[7])
-                 : "l"(p)
-                 : "memory");
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int left, float (&x)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = i < left ? p[i] : 0.0f;
+  for (int i = 0; i < 8; ++i) x[i] = i < left ? to_float(p[i]) : 0.0f;
 }
-__device__ __forceinline__ void store8(float* p, bool wide, int left, const float (&x)[8]) {
-  if (wide && left >= 8) {
+__device__ __forceinline__ void store8(float* p, bool full, int left, const float (&x)[8]) {
+  if (full) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p),
                  "r"(__float_as_uint(x[0])), "r"(__float_as_uint(x[1])), "r"(__float_as_uint(x[2])),
                  "r"(__float_as_uint(x[3])), "r"(__float_as_uint(x[4])), "r"(__float_as_uint(x[5])),
@@ -70,22 +62,8 @@ __device__ __forceinline__ void store8(float* p, bool wide, int left, const floa
   for (int i = 0; i < 8; ++i)
     if (i < left) p[i] = x[i];
 }
-__device__ __forceinline__ void load8(const bf16* p, bool wide, int left, float (&x)[8]) {
-  if (wide && left >= 8) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(u[i] << 16);
-      x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = i < left ? to_float(p[i]) : 0.0f;
-}
-__device__ __forceinline__ void store8(bf16* p, bool wide, int left, const float (&x)[8]) {
-  if (wide && left >= 8) {
+__device__ __forceinline__ void store8(bf16* p, bool full, int left, const float (&x)[8]) {
+  if (full) {
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -97,8 +75,7 @@ __device__ __forceinline__ void store8(bf16* p, bool wide, int left, const float
   for (int i = 0; i < 8; ++i)
     if (i < left) p[i] = from_float<bf16>(x[i]);
 }
-__device__ __forceinline__ uint2 load_codes(const uint8_t* p, bool wide, int left) {
-  if (wide && left >= 8) return *reinterpret_cast<const uint2*>(p);
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int left) {
   unsigned long long w = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -111,18 +88,17 @@ __device__ __forceinline__ void decode8(uint2 codes, float scale, float (&x)[8])
     const uint32_t pair = ((i < 2 ? codes.x : codes.y) >> (16 * (i & 1))) & 0xFFFFu;
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3);
     const float2 v = __half22float2(__half2(h));
-    x[2 * i] = __fmul_rn(v.x, scale);
-    x[2 * i + 1] = __fmul_rn(v.y, scale);
+    mul2o(x[2 * i], x[2 * i + 1], v.x, v.y, scale, scale);
   }
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, bool wide, int left, const float (&units)[8]) {
+__device__ __forceinline__ void store_codes(uint8_t* p, bool full, int left, const float (&units)[8]) {
   uint32_t w[2] = {0, 0};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     w[i / 2] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(units[2 * i], units[2 * i + 1]),
                                                                __NV_SATFINITE, __NV_E4M3))
                 << (16 * (i & 1));
-  if (wide && left >= 8) {
+  if (full) {
     *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     return;
   }
@@ -144,10 +120,10 @@ __device__ __forceinline__ float block_scale(float largest) {
   const float s = __fmul_rn(largest, 1.0f / 448.0f);
   return s < 0x1p-126f ? 0x1p-126f : s;
 }
-// x[i] / scale, correctly rounded. One reciprocal for the block and a remainder step each:
-// with r the correctly rounded 1 / s, q = x r is off by an ulp at most and q + (x - q s) r is
-// the correctly rounded quotient, as long as the remainder does not underflow -- blocks whose
-// largest value is that small divide.
+// x[i] / scale, correctly rounded: one reciprocal for the block and Markstein's remainder step
+// for each value. With r the correctly rounded 1 / s, q = x r is off by an ulp at most and
+// q + (x - q s) r is the correctly rounded quotient, as long as the remainder does not
+// underflow -- blocks whose largest value is that small divide.
 __device__ __forceinline__ void divide8(float (&x)[8], float scale) {
   if (scale < 0x1p-90f) {
 #pragma unroll
@@ -156,53 +132,127 @@ __device__ __forceinline__ void divide8(float (&x)[8], float scale) {
   }
   const float r = __frcp_rn(scale);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q = __fmul_rn(x[i], r);
-    x[i] = __fmaf_rn(__fmaf_rn(-q, scale, x[i]), r, q);
+  for (int i = 0; i < 8; i += 2) {
+    float q0, q1, d0, d1;
+    mul2o(q0, q1, x[i], x[i + 1], r, r);
+    fma2o(d0, d1, q0, q1, -scale, -scale, x[i], x[i + 1]);
+    fma2o(x[i], x[i + 1], d0, d1, r, r, q0, q1);
   }
 }
 
+// What a lane loads of its block, as it lies in memory: the next block's is on its way while
+// this one's is worked on.
 template <bool Eight, typename T>
-__device__ __forceinline__ void update_block(const fhb_adamw_tensor& t, bool wide, int64_t own,
-                                             int lane, const Constants& k, float step_size,
-                                             float inverse_root) {
+struct Raw {
+  uint32_t g[2 * sizeof(T)], p[2 * sizeof(T)], m[Eight ? 2 : 8], v[Eight ? 2 : 8];
+  float sm, sv;
+};
+template <int Words>
+__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[Words]) {
+  if constexpr (Words == 8)
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]),
+                   "=r"(w[6]), "=r"(w[7])
+                 : "l"(p)
+                 : "memory");
+  else if constexpr (Words == 4)
+    asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "l"(p)
+                 : "memory");
+  else
+    asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p) : "memory");
+}
+template <bool Eight, typename T>
+__device__ __forceinline__ void load_raw(const fhb_adamw_tensor& t, int64_t own, int lane, Raw<Eight, T>& w) {
+  const int64_t at = own * kBlock + lane * 8;
+  load_words(static_cast<const T*>(t.grad) + at, w.g);
+  load_words(static_cast<const T*>(t.param) + at, w.p);
+  if constexpr (Eight) {
+    load_words(static_cast<const uint8_t*>(t.exp_avg) + at, w.m);
+    load_words(static_cast<const uint8_t*>(t.exp_avg_sq) + at, w.v);
+    w.sm = t.exp_avg_scale[own];
+    w.sv = t.exp_avg_sq_scale[own];
+  } else {
+    load_words(static_cast<const float*>(t.exp_avg) + at, w.m);
+    load_words(static_cast<const float*>(t.exp_avg_sq) + at, w.v);
+  }
+}
+template <int Words>
+__device__ __forceinline__ void unpack(const uint32_t (&w)[Words], float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < Words; ++i) {
+    if constexpr (Words == 8) {
+      x[i] = __uint_as_float(w[i]);
+    } else {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+}
+
+// The values of a last block or an unaligned tensor, one by one.
+template <bool Eight, typename T>
+__device__ __forceinline__ void load_single(const fhb_adamw_tensor& t, int64_t own, int lane,
+                                            float (&g)[8], float (&p)[8], float (&m)[8],
+                                            float (&v)[8]) {
   const int64_t at = own * kBlock + lane * 8;
   const int left = static_cast<int>(min(t.count - at, int64_t{8}));  // may be negative
-  float g[8], p[8], m[8], v[8];
-  load8(static_cast<const T*>(t.grad) + at, wide, left, g);
-  load8(static_cast<const T*>(t.param) + at, wide, left, p);
-  if (Eight) {
-    const uint2 cm = load_codes(static_cast<const uint8_t*>(t.exp_avg) + at, wide, left);
-    const uint2 cv = load_codes(static_cast<const uint8_t*>(t.exp_avg_sq) + at, wide, left);
-    decode8(cm, t.exp_avg_scale[own], m);
-    decode8(cv, t.exp_avg_sq_scale[own], v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], v[i]);
+  load8(static_cast<const T*>(t.grad) + at, left, g);
+  load8(static_cast<const T*>(t.param) + at, left, p);
+  if constexpr (Eight) {
+    decode8(load_codes(static_cast<const uint8_t*>(t.exp_avg) + at, left), t.exp_avg_scale[own], m);
+    decode8(load_codes(static_cast<const uint8_t*>(t.exp_avg_sq) + at, left), t.exp_avg_sq_scale[own], v);
   } else {
-    load8(static_cast<const float*>(t.exp_avg) + at, wide, left, m);
-    load8(static_cast<const float*>(t.exp_avg_sq) + at, wide, left, v);
+    load8(static_cast<const float*>(t.exp_avg) + at, left, m);
+    load8(static_cast<const float*>(t.exp_avg_sq) + at, left, v);
   }
+}
+
+// One block by one warp, from its gradient, parameter, m, and v (8 bits: sqrt(v)). Full: all
+// 256 values exist and every array is aligned for 8 of them.
+template <bool Eight, typename T, bool full>
+__device__ __forceinline__ void update_block(const fhb_adamw_tensor& t, int64_t own, int lane,
+                                             const Constants& k, float step_size,
+                                             float inverse_root, const float (&g)[8], float (&p)[8],
+                                             float (&m)[8], float (&v)[8]) {
+  const int64_t at = own * kBlock + lane * 8;
+  const int left = full ? 8 : static_cast<int>(min(t.count - at, int64_t{8}));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    m[i] = __fadd_rn(__fmul_rn(m[i], k.b1), __fmul_rn(g[i], k.c1));
-    v[i] = __fadd_rn(__fmul_rn(v[i], k.b2), __fmul_rn(__fmul_rn(g[i], g[i]), k.c2));
+  for (int i = 0; i < 8; i += 2) {
+    float a0, a1, c0, c1;
+    if (Eight) mul2o(v[i], v[i + 1], v[i], v[i + 1], v[i], v[i + 1]);
+    mul2o(a0, a1, m[i], m[i + 1], k.b1, k.b1);
+    mul2o(c0, c1, g[i], g[i + 1], k.c1, k.c1);
+    // single additions: a packed one would be contracted with the packed products before it
+    m[i] = __fadd_rn(a0, c0);
+    m[i + 1] = __fadd_rn(a1, c1);
+    mul2o(a0, a1, v[i], v[i + 1], k.b2, k.b2);
+    mul2o(c0, c1, g[i], g[i + 1], g[i], g[i + 1]);
+    mul2o(c0, c1, c0, c1, k.c2, k.c2);
+    v[i] = __fadd_rn(a0, c0);
+    v[i + 1] = __fadd_rn(a1, c1);
   }
   if (!Eight) {
-    store8(static_cast<float*>(t.exp_avg) + at, wide, left, m);
-    store8(static_cast<float*>(t.exp_avg_sq) + at, wide, left, v);
+    store8(static_cast<float*>(t.exp_avg) + at, full, left, m);
+    store8(static_cast<float*>(t.exp_avg_sq) + at, full, left, v);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 8; i += 2) {
     if (Eight) {
       v[i] = __fsqrt_rn(v[i]);
+      v[i + 1] = __fsqrt_rn(v[i + 1]);
     } else {
       asm("sqrt.approx.f32 %0, %0;" : "+f"(v[i]));
+      asm("sqrt.approx.f32 %0, %0;" : "+f"(v[i + 1]));
     }
-    const float denominator = fmaf(v[i], inverse_root, k.eps);
-    // the denominator may be 0 (eps 0): 0 / 0 and x / 0 as IEEE has them
-    p[i] = fmaf(-step_size, __fdividef(m[i], denominator), p[i] * k.decay);
+    float d0, d1, w0, w1;
+    fma2o(d0, d1, v[i], v[i + 1], inverse_root, inverse_root, k.eps, k.eps);
+    mul2o(w0, w1, p[i], p[i + 1], k.decay, k.decay);
+    // a denominator of 0 (eps 0): 0 / 0 and x / 0 as IEEE has them
+    fma2o(p[i], p[i + 1], __fdividef(m[i], d0), __fdividef(m[i + 1], d1), -step_size, -step_size, w0, w1);
   }
-  store8(static_cast<T*>(t.param) + at, wide, left, p);
+  store8(static_cast<T*>(t.param) + at, full, left, p);
   if (!Eight) return;
   const float scale_m = block_scale(warp_largest(m)), scale_v = block_scale(warp_largest(v));
   divide8(m, scale_m);
@@ -212,18 +262,61 @@ __device__ __forceinline__ void update_block(const fhb_adamw_tensor& t, bool wid
   divide8(units, scale_v);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (v[i] > 0.0f && units[i] < 0x1p-9f) units[i] = 0x1p-9f;  // not zero stays not zero
-  store_codes(static_cast<uint8_t*>(t.exp_avg) + at, wide, left, m);
-  store_codes(static_cast<uint8_t*>(t.exp_avg_sq) + at, wide, left, units);
+    units[i] = fmaxf(units[i], v[i] > 0.0f ? 0x1p-9f : 0.0f);  // not zero stays not zero
+  store_codes(static_cast<uint8_t*>(t.exp_avg) + at, full, left, m);
+  store_codes(static_cast<uint8_t*>(t.exp_avg_sq) + at, full, left, units);
   if (lane == 0) {
     t.exp_avg_scale[own] = scale_m;
     t.exp_avg_sq_scale[own] = scale_v;
   }
 }
 
+// The rest: last blocks of a tensor and unaligned tensors, kept out of the others' registers.
+template <bool Eight, typename T>
+__device__ __noinline__ void update_partial(const fhb_adamw_tensor& t, int64_t own, int lane,
+                                            const Constants& k, float step_size,
+                                            float inverse_root) {
+  float g[8], p[8], m[8], v[8];
+  load_single<Eight, T>(t, own, lane, g, p, m, v);
+  update_block<Eight, T, false>(t, own, lane, k, step_size, inverse_root, g, p, m, v);
+}
+template <bool Eight, typename T>
+__device__ __forceinline__ int64_t update_tensor(const fhb_adamw_tensor& t, bool wide, int64_t block,
+                                                 int64_t first, int64_t end, int64_t stride, int lane,
+                                                 const Constants& k, float step_size,
+                                                 float inverse_root) {
+  // blocks before `whole` are full
+  const int64_t whole = first + (wide ? t.count / kBlock : 0);
+  if (block < whole) {
+    Raw<Eight, T> w;
+    load_raw(t, block - first, lane, w);
+    while (true) {
+      float g[8], p[8], m[8], v[8];
+      unpack(w.g, g);
+      unpack(w.p, p);
+      if constexpr (Eight) {
+        decode8(make_uint2(w.m[0], w.m[1]), w.sm, m);
+        decode8(make_uint2(w.v[0], w.v[1]), w.sv, v);
+      } else {
+        unpack(w.m, m);
+        unpack(w.v, v);
+      }
+      const int64_t own = block - first;
+      block += stride;
+      if (Eight && block < whole) load_raw(t, block - first, lane, w);
+      update_block<Eight, T, true>(t, own, lane, k, step_size, inverse_root, g, p, m, v);
+      if (block >= whole) break;
+      if (!Eight) load_raw(t, block - first, lane, w);
+    }
+  }
+  for (; block < end; block += stride)
+    update_partial<Eight, T>(t, block - first, lane, k, step_size, inverse_root);
+  return block;
+}
+
 template <bool Eight, int Capacity>
-__global__ void __launch_bounds__(kThreads)
-    adamw_kernel(const __grid_constant__ Batch<Capacity> batch, const Constants k,
+__global__ void __launch_bounds__(kThreads, Eight ? kResidentEight : kResident)
+    adamw_kernel(const __grid_constant__ Batch<Capacity> batch, const __grid_constant__ Constants k,
                  unsigned long long* step) {
   __shared__ float corrections[2];
   __shared__ unsigned long long now;
@@ -239,9 +332,9 @@ __global__ void __launch_bounds__(kThreads)
   const int lane = threadIdx.x % 32;
   const int64_t blocks = batch.first_block[batch.tensors];
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kWarps;
+  int64_t block = blockIdx.x * static_cast<int64_t>(kWarps) + threadIdx.x / 32;
   int at = 0;
-  for (int64_t block = blockIdx.x * static_cast<int64_t>(kWarps) + threadIdx.x / 32; block < blocks;
-       block += stride) {
+  while (block < blocks) {
     // the tensor: the last one whose first block is not past this (blocks only go up)
     int low = at, high = batch.tensors;
     while (high - low > 1) {
@@ -251,11 +344,11 @@ __global__ void __launch_bounds__(kThreads)
     }
     at = low;
     const fhb_adamw_tensor& t = batch.tensor[at];
-    const int64_t own = block - batch.first_block[at];
-    if (t.dtype == FHB_DTYPE_F32)
-      update_block<Eight, float>(t, batch.wide[at] != 0, own, lane, k, step_size, inverse_root);
-    else
-      update_block<Eight, bf16>(t, batch.wide[at] != 0, own, lane, k, step_size, inverse_root);
+    const bool wide = batch.wide[at] != 0;
+    const int64_t first = batch.first_block[at], end = batch.first_block[at + 1];
+    block = t.dtype == FHB_DTYPE_F32
+                ? update_tensor<Eight, float>(t, wide, block, first, end, stride, lane, k, step_size, inverse_root)
+                : update_tensor<Eight, bf16>(t, wide, block, first, end, stride, lane, k, step_size, inverse_root);
   }
   if (!batch.advances) return;
   __syncthreads();
@@ -282,7 +375,7 @@ cudaError_t launch(const fhb_adamw_tensor* tensors, int64_t count, bool eight, b
   }
   const int64_t need = (batch.first_block[count] + kWarps - 1) / kWarps;
   if (need == 0 && !advances) return cudaSuccess;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(need, 1), 6ll * dev.sms));
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(need, 1), static_cast<int64_t>(eight ? kResidentEight : kResident) * dev.sms));
   if (eight)
     adamw_kernel<true, Capacity><<<grid, kThreads, 0, stream>>>(batch, k, step);
   else
