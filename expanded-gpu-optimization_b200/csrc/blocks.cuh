@@ -29,16 +29,31 @@ __device__ __forceinline__ bf16 from_float<bf16>(float x) {
   return __float2bfloat16_rn(x);
 }
 
-// The block's activation and its derivative at g: tanh, or silu = g sigma(g) with derivative
-// sigma (1 + g (1 - sigma)).
-__device__ __forceinline__ void block_activation(int activation, float g, float& a, float& slope) {
-  if (activation == FHB_ACTIVATION_TANH) {
-    a = tanhf(g);
-    slope = 1.0f - a * a;
+// The block's activation a and its derivative at g, on the special-function unit (ex2, rcp: a
+// few ulp). silu: a = g s, a' = s (1 + g (1 - s)), s = 1 / (1 + e^-g). tanh: with r = 1 / (1 +
+// e^2g), a = 1 - 2 r and a' = 4 r (1 - r), which has no cancellation where tanh saturates;
+// below 1/4, where 1 - 2 r loses digits, the Taylor series (next term below 2^-26 of a).
+__device__ __forceinline__ float reciprocal_of_one_plus_exp2(float x) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
+  return r;
+}
+template <bool Tanh>
+__device__ __forceinline__ void block_activation(float g, float& a, float& slope) {
+  if (Tanh) {
+    const float r = reciprocal_of_one_plus_exp2(g * 2.8853900817779268f);  // 2 / ln 2
+    const float q = g * g;
+    float t = fmaf(q, 62.0f / 2835.0f, -17.0f / 315.0f);
+    t = fmaf(q, t, 2.0f / 15.0f);
+    t = fmaf(q, t, -1.0f / 3.0f);
+    t = fmaf(g * q, t, g);
+    a = fabsf(g) < 0.25f ? t : fmaf(-2.0f, r, 1.0f);
+    slope = 4.0f * r * (1.0f - r);
   } else {
-    const float s = 1.0f / (1.0f + expf(-g));
+    const float s = reciprocal_of_one_plus_exp2(g * -1.4426950408889634f);  // 1 / ln 2
     a = g * s;
-    slope = s * (1.0f + g * (1.0f - s));
+    slope = fmaf(a, 1.0f - s, s);
   }
 }
 #endif

@@ -39,45 +39,55 @@ Saved saved_in(const fhb_ffn_problem& p, Room& room) {
 }
 
 // ---- column sums (the biases' gradients) ----
-// Rows of one part: 512, more where there would be over 2,048 parts.
-int64_t part_rows_of(int64_t rows) { return std::max<int64_t>(512, (rows + 2047) / 2048); }
+// dg's and du's come as sums over 32 rows from the product that makes them, dy's from itself.
+// One part: 64 columns of up to part_rows rows over 8 warps; then the parts, in order.
 struct ColumnSource {
-  const void* p;  // T, or a TcMatrix's planes
-  int64_t stride, plane, columns;
-  bool operand;
+  const void* p;
+  int64_t stride, columns, rows;
+  bool sums;  // FP32 sums, else values of the block's type
   void* out;
 };
 struct ColumnSources {
   ColumnSource source[3];
-  int64_t rows, part_rows, widest;
+  int64_t part_rows, part_count, widest;
   float* parts;  // [source][part][widest]
-  int64_t part_count;
 };
+// Rows of one part: 256, more where there would be over 1,024 parts.
+int64_t part_rows_of(int64_t rows) { return std::max<int64_t>(256, (rows + 1023) / 1024); }
 
-// One part: 64 columns, its rows over 8 warps, then the warps' sums in order.
+template <typename S>
+__device__ __forceinline__ void add_rows(const S* p, int64_t stride, int64_t first, int64_t last,
+                                         const int64_t (&c)[2], int64_t columns, float (&sum)[2]) {
+  int64_t r = first;
+  for (; r + 56 < last; r += 64) {  // eight rows in flight
+    float v[8][2];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) v[k][j] = c[j] < columns ? to_float(p[(r + 8 * k) * stride + c[j]]) : 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) sum[j] += v[k][j];
+  }
+  for (; r < last; r += 8)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (c[j] < columns) sum[j] += to_float(p[r * stride + c[j]]);
+}
+
 template <typename T>
-__global__ void __launch_bounds__(256) column_parts_kernel(ColumnSources s) {
+__global__ void __launch_bounds__(256) column_parts_kernel(const __grid_constant__ ColumnSources s) {
   const ColumnSource& src = s.source[blockIdx.z];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int64_t c0 = blockIdx.x * 64ll;
+  const int64_t c0 = blockIdx.x * 64ll, c[2] = {c0 + lane, c0 + lane + 32};
   if (c0 >= src.columns) return;
-  const int64_t first = blockIdx.y * s.part_rows;
-  const int64_t last = min(first + s.part_rows, s.rows);
+  const int64_t first = blockIdx.y * s.part_rows, last = min(first + s.part_rows, src.rows);
   float sum[2] = {};
-  for (int64_t r = first + warp; r < last; r += 8)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int64_t c = c0 + lane + 32 * j, at = r * src.stride + c;
-      if (c >= src.columns) continue;
-      if (src.operand) {
-        const bf16* p = static_cast<const bf16*>(src.p) + at;
-        float v = to_float(p[0]);
-        if (sizeof(T) == 4) v += to_float(p[src.plane]) + to_float(p[2 * src.plane]);
-        sum[j] += v;
-      } else {
-        sum[j] += to_float(static_cast<const T*>(src.p)[at]);
-      }
-    }
+  if (src.sums)
+    add_rows(static_cast<const float*>(src.p), src.stride, first + warp, last, c, src.columns, sum);
+  else
+    add_rows(static_cast<const T*>(src.p), src.stride, first + warp, last, c, src.columns, sum);
   __shared__ float by_warp[8][64];
   by_warp[warp][lane] = sum[0];
   by_warp[warp][lane + 32] = sum[1];
@@ -90,22 +100,30 @@ __global__ void __launch_bounds__(256) column_parts_kernel(ColumnSources s) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(64) column_totals_kernel(ColumnSources s) {
+__global__ void __launch_bounds__(256) column_totals_kernel(const __grid_constant__ ColumnSources s) {
   const ColumnSource& src = s.source[blockIdx.y];
-  const int64_t c = blockIdx.x * 64ll + threadIdx.x;
-  if (c >= src.columns) return;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t c = blockIdx.x * 32ll + lane;
+  const int64_t parts = (src.rows + s.part_rows - 1) / s.part_rows;
   float total = 0.0f;
-  for (int64_t part = 0; part < s.part_count; ++part)
-    total += s.parts[(blockIdx.y * s.part_count + part) * s.widest + c];
+  if (c < src.columns)
+    for (int64_t part = warp; part < parts; part += 8)
+      total += s.parts[(blockIdx.y * s.part_count + part) * s.widest + c];
+  __shared__ float by_warp[8][32];
+  by_warp[warp][lane] = total;
+  __syncthreads();
+  if (warp != 0 || c >= src.columns) return;
+  total = 0.0f;
+  for (int w = 0; w < 8; ++w) total += by_warp[w][lane];
   static_cast<T*>(src.out)[c] = from_float<T>(total);
 }
 
 template <typename T>
-cudaError_t column_sums(ColumnSources& s, int count, cudaStream_t stream) {
+cudaError_t column_sums(const ColumnSources& s, int count, cudaStream_t stream) {
   if (count == 0) return cudaSuccess;
-  const unsigned columns = static_cast<unsigned>((s.widest + 63) / 64);
-  column_parts_kernel<T><<<dim3(columns, static_cast<unsigned>(s.part_count), count), 256, 0, stream>>>(s);
-  column_totals_kernel<T><<<dim3(columns, count), 64, 0, stream>>>(s);
+  column_parts_kernel<T><<<dim3(static_cast<unsigned>((s.widest + 63) / 64),
+                                static_cast<unsigned>(s.part_count), count), 256, 0, stream>>>(s);
+  column_totals_kernel<T><<<dim3(static_cast<unsigned>((s.widest + 31) / 32), count), 256, 0, stream>>>(s);
   return cudaGetLastError();
 }
 
@@ -114,29 +132,24 @@ struct Operands {
   TcMatrix x, w_gate, w_up, w_down, dy;
 };
 
-// Operand forms of the inputs, copied into `room` where they have to be (and where it is real).
-cudaError_t operands_in(const fhb_ffn_problem& p, const void* dy, int64_t dy_stride, Room& room,
-                        Operands& o, cudaStream_t stream) {
-  struct {
-    const void* p;
-    int64_t rows, cols, stride;
-    TcMatrix* out;
-  } const inputs[] = {{p.x, p.tokens, p.width, p.x_stride, &o.x},
-                      {p.w_gate, p.hidden, p.width, p.w_gate_stride, &o.w_gate},
-                      {p.w_up, p.hidden, p.width, p.w_up_stride, &o.w_up},
-                      {p.w_down, p.out_width, p.hidden, p.w_down_stride, &o.w_down},
-                      {dy, p.tokens, p.out_width, dy_stride, &o.dy}};
-  for (const auto& in : inputs) {
-    if (in.p == nullptr) continue;
-    void* place = room.take(tc_operand_bytes(in.p, in.rows, in.cols, in.stride, p.dtype));
-    if (room.base == nullptr) {
-      *in.out = tc_result(nullptr, in.rows, in.cols, p.dtype);
-      continue;
-    }
-    const cudaError_t e = tc_operand(in.p, in.rows, in.cols, in.stride, p.dtype, place, in.out, stream);
-    if (e != cudaSuccess) return e;
+// Operand forms of the inputs; those that have to be copied take their place in `room`.
+struct Inputs {
+  TcInput in[5];
+  TcMatrix out[5];
+};
+Inputs inputs_in(const fhb_ffn_problem& p, const void* dy, int64_t dy_stride, Room& room, Operands& o) {
+  Inputs x{{{p.x, p.tokens, p.width, p.x_stride},
+            {p.w_gate, p.hidden, p.width, p.w_gate_stride},
+            {p.w_up, p.hidden, p.width, p.w_up_stride},
+            {p.w_down, p.out_width, p.hidden, p.w_down_stride},
+            {dy, p.tokens, p.out_width, dy_stride}}, {}};
+  TcMatrix* const to[] = {&o.x, &o.w_gate, &o.w_up, &o.w_down, &o.dy};
+  for (int i = 0; i < 5; ++i) {
+    if (x.in[i].p == nullptr) continue;
+    void* place = room.take(tc_operand_bytes(x.in[i], p.dtype));
+    *to[i] = x.out[i] = tc_operand(x.in[i], p.dtype, place);
   }
-  return cudaSuccess;
+  return x;
 }
 
 TcProduct gate_product(const fhb_ffn_problem& p, const Operands& o, const Saved& s, bool keep) {
@@ -185,6 +198,11 @@ Backward backward_of(const fhb_ffn_problem& p, const Operands& o, const Saved& s
   b.hidden.epilogue = TcEpilogue::kGateGrad;
   b.hidden.gated[0] = b.dg, b.hidden.gated[1] = b.du;
   b.hidden.factors = s.factors;
+  if (out.b_gate != nullptr || out.b_up != nullptr) {
+    b.hidden.row_sums_stride = round_up(p.hidden, 32);
+    b.hidden.row_sums = static_cast<float*>(room.take(
+        static_cast<size_t>((p.tokens + 31) / 32 * 2 * b.hidden.row_sums_stride * 4)));
+  }
   b.want_x = out.x != nullptr;
   b.x = store_product(p, p.tokens, p.width, p.hidden, out.x);
   b.x.a[0] = b.dg, b.x.a[1] = b.du, b.x.b[0] = o.w_gate, b.x.b[1] = o.w_up;
@@ -229,14 +247,14 @@ size_t ffn_workspace_bytes(const fhb_ffn_problem& p, bool backward, const Device
   Operands o;
   if (p.tokens == 0) return 0;
   if (!backward) {
-    operands_in(p, nullptr, 0, room, o, nullptr);
+    inputs_in(p, nullptr, 0, room, o);
     const Saved s = saved_in(p, room);
     const size_t parts = gemm_tc_workspace_bytes(down_product(p, o, s, nullptr), dev);
     room.take(parts);
     return room.used;
   }
   // the upstream gradient may need a copy: the size asked for does not depend on it
-  operands_in(p, nullptr, 0, room, o, nullptr);
+  inputs_in(p, nullptr, 0, room, o);
   room.take(tc_result_bytes(p.tokens, p.out_width, p.dtype));
   Room aside{nullptr};
   const Saved s = saved_in(p, aside);
@@ -255,7 +273,8 @@ cudaError_t launch_ffn_forward(const fhb_ffn_problem& p, void* y, void* saved, v
                                const DeviceInfo& dev, cudaStream_t stream) {
   Room room{static_cast<char*>(workspace)}, kept{static_cast<char*>(saved)};
   Operands o;
-  cudaError_t e = operands_in(p, nullptr, 0, room, o, stream);
+  const Inputs x = inputs_in(p, nullptr, 0, room, o);
+  cudaError_t e = launch_pack(x.in, x.out, 5, p.dtype, stream);
   if (e != cudaSuccess) return e;
   const Saved s = saved_in(p, saved != nullptr ? kept : room);
   e = launch_gemm_tc(gate_product(p, o, s, saved != nullptr), nullptr, dev, stream);
@@ -284,7 +303,8 @@ cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, in
   }
   Room room{static_cast<char*>(workspace)}, kept{static_cast<char*>(const_cast<void*>(saved))};
   Operands o;
-  cudaError_t e = operands_in(p, grad_y, grad_y_stride, room, o, stream);
+  const Inputs x = inputs_in(p, grad_y, grad_y_stride, room, o);
+  cudaError_t e = launch_pack(x.in, x.out, 5, p.dtype, stream);
   if (e != cudaSuccess) return e;
   const Saved s = saved_in(p, kept);
   const Backward b = backward_of(p, o, s, out, room);
@@ -300,13 +320,16 @@ cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, in
   if (e != cudaSuccess) return e;
   ColumnSources columns{};
   int count = 0;
-  if (out.b_gate != nullptr) columns.source[count++] = {b.dg.p, b.dg.stride, b.dg.plane, p.hidden, true, out.b_gate};
-  if (out.b_up != nullptr) columns.source[count++] = {b.du.p, b.du.stride, b.du.plane, p.hidden, true, out.b_up};
-  if (out.b_down != nullptr) columns.source[count++] = {grad_y, grad_y_stride, 0, p.out_width, false, out.b_down};
-  columns.rows = p.tokens;
+  const int64_t row_sums = (p.tokens + 31) / 32, sums_stride = b.hidden.row_sums_stride;
+  if (out.b_gate != nullptr)
+    columns.source[count++] = {b.hidden.row_sums, 2 * sums_stride, p.hidden, row_sums, true, out.b_gate};
+  if (out.b_up != nullptr)
+    columns.source[count++] = {b.hidden.row_sums + sums_stride, 2 * sums_stride, p.hidden, row_sums, true, out.b_up};
+  if (out.b_down != nullptr)
+    columns.source[count++] = {grad_y, grad_y_stride, p.out_width, p.tokens, false, out.b_down};
   columns.part_rows = part_rows_of(p.tokens);
-  columns.widest = std::max(p.hidden, p.out_width);
   columns.part_count = column_part_count(p);
+  columns.widest = std::max(p.hidden, p.out_width);
   columns.parts = static_cast<float*>(room.take(0));
   return p.dtype == FHB_DTYPE_F32 ? column_sums<float>(columns, count, stream)
                                   : column_sums<bf16>(columns, count, stream);

@@ -10,6 +10,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -25,6 +26,7 @@ constexpr int kThreads = 32 * (kEpilogueWarps + 2);
 constexpr int kMaxSlots = 10;
 constexpr int kRingBytes = 208 * 1024;
 constexpr int kMaxTerms = 12;
+constexpr int kMaxOperands = 5;  // of a block's products
 constexpr int kATileBytes = kRows * kKBlock * 2;  // 16 KB
 
 struct Maps {
@@ -52,6 +54,8 @@ struct Args {
   int activation;
   float* partial;
   int64_t partial_stride;
+  float* row_sums;            // [32 rows][dg, du][row_sums_stride]: their column sums, or null
+  int64_t row_sums_stride;
   unsigned int* status;
 };
 
@@ -309,28 +313,53 @@ __device__ __forceinline__ void store_factors(const TcFactors& f, int64_t place,
     for (int i = 0; i < 4; ++i) store32(p + 8 * i, w + 8 * i);
   }
 }
-// v[i] *= factor i.
+// The factors of one kind of a group of 32, as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void times_factors(const TcFactors& f, int64_t place, float (&v)[32]) {
-  uint32_t w[32];
-  if (sizeof(T) == 2) {
-    const __half* p = static_cast<const __half*>(f.values) + place * kFactorGroup;
-    load32(p, w);
-    load32(p + 16, w + 8);
-    const float unscale = group_unscale(f.exponents[place]);
+struct FactorWords {
+  uint32_t w[8 * sizeof(T)];
+  uint32_t exponent;
+};
+template <typename T>
+__device__ __forceinline__ void load_factors(const TcFactors& f, int64_t place, FactorWords<T>& x) {
+  const char* p = static_cast<const char*>(f.values) + place * (kFactorGroup * sizeof(T));
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) load32(p + 32 * i, x.w + 8 * i);
+  if (sizeof(T) == 2) x.exponent = f.exponents[place];
+}
+// out[i] = v[i] times factor i
+template <typename T>
+__device__ __forceinline__ void times_factors(const FactorWords<T>& x, const float (&v)[32], float (&out)[32]) {
+  if constexpr (sizeof(T) == 2) {
+    const float unscale = group_unscale(x.exponent);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      v[2 * i] *= x.x * unscale;
-      v[2 * i + 1] *= x.y * unscale;
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x.w[i]));
+      out[2 * i] = v[2 * i] * (f.x * unscale);
+      out[2 * i + 1] = v[2 * i + 1] * (f.y * unscale);
     }
   } else {
-    const float* p = static_cast<const float*>(f.values) + place * kFactorGroup;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load32(p + 8 * i, w + 8 * i);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] *= __uint_as_float(w[i]);
+    for (int i = 0; i < 32; ++i) out[i] = v[i] * __uint_as_float(x.w[i]);
   }
+}
+
+// Column sums over the warp's 32 rows (one row a lane): lane i gets column i's, by halving the
+// columns and doubling the rows five times, in a fixed order.
+__device__ __forceinline__ float sum_rows(const float (&v)[32], int lane) {
+  float s[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float keep = lane & 16 ? v[i + 16] : v[i], give = lane & 16 ? v[i] : v[i + 16];
+    s[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+  }
+#pragma unroll
+  for (int half = 8; half >= 1; half /= 2)
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const float keep = lane & half ? s[i + half] : s[i], give = lane & half ? s[i] : s[i + half];
+      s[i] = keep + __shfl_xor_sync(0xffffffffu, give, half);
+    }
+  return s[0];
 }
 
 // One item of work: a tile of one group's result and one part of K.
@@ -519,100 +548,163 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Item it = item_at<Cg, kGateTile>(p, index);
       const int chunks = chunk_count<T>(it.blocks);
       const int64_t row = it.m0 + rank * kRows + quadrant * 32 + lane;
-      // two groups of 32 columns at a time: a gate tile's g and u, else neighbours
-      const auto finish = [&](int pair, float (&v0)[32], float (&v1)[32]) {
-        if (row >= p.m) return;
-        if constexpr (E == TcEpilogue::kGate) {
-          const int64_t n0 = it.n0 + 32 * pair;
-          if (n0 >= p.n) return;
-          add_bias<T>(p.bias[0], n0, p.n, v0);
-          add_bias<T>(p.bias[1], n0, p.n, v1);
-          float h[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float a, slope;
-            block_activation(p.activation, v0[i], a, slope);
-            h[i] = a * v1[i];
-            v0[i] = a;
-            v1[i] *= slope;
-          }
-          store_operand<T>(p.gated[0] + row * p.gated_stride + n0, p.gated_plane, h);
-          if (p.factors.values != nullptr) {
-            const int64_t place = (row * p.factors.groups + n0 / kFactorGroup) * 2;
-            store_factors<T>(p.factors, place, v0);
-            store_factors<T>(p.factors, place + 1, v1);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float(&v)[32] = j == 0 ? v0 : v1;
-            const int64_t n0 = it.n0 + 64 * pair + 32 * j;
-            if (n0 >= p.n) break;
-            if constexpr (E == TcEpilogue::kGateGrad) {
-              const int64_t place = (row * p.factors.groups + n0 / kFactorGroup) * 2;
-              float d[32];
-#pragma unroll
-              for (int i = 0; i < 32; ++i) d[i] = v[i];
-              times_factors<T>(p.factors, place, d);  // du = dh act(g)
-              times_factors<T>(p.factors, place + 1, v);
-              const int64_t at = row * p.gated_stride + n0;
-              store_operand<T>(p.gated[0] + at, p.gated_plane, v);
-              store_operand<T>(p.gated[1] + at, p.gated_plane, d);
-            } else if constexpr (E == TcEpilogue::kPartial) {
-              float* out = p.partial + ((static_cast<int64_t>(it.group) * p.parts + it.part) * p.m + row) * p.partial_stride;
-              store_results<float>(out, n0, p.partial_stride, true, v);
-            } else {
-              add_bias<T>(p.bias[0], n0, p.n, v);
-              store_results<T>(static_cast<T*>(p.out[it.group]) + row * p.out_stride, n0, p.n, p.out_wide != 0, v);
-            }
-          }
+      const auto release_sums = [&](int buffer) {
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if (Cg == 2) arrive_remote(release + buffer * 8);
+          else mbar_arrive(&sum_empty[buffer]);
         }
       };
-      float acc0[32], acc1[32];
-      for (int c = 0; c < chunks; ++c, ++sums) {
-        const int buffer = static_cast<int>(sums & 1);
+      // waits for the sums of a chunk of K; the warps agree, since what follows is for whole warps
+      const auto wait_sums = [&](int buffer) {
         ok = mbar_wait_bounded(&sum_full[buffer], static_cast<uint32_t>((sums >> 1) & 1), p.status,
                                FHB_STATUS_MMA_TIMEOUT);
-        // a wait that gave up: the warps agree, since what follows is for whole warps
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         tc::fence_after_sync();
-        const uint32_t from = tmem + buffer * kMaxColumns + (static_cast<uint32_t>(quadrant * 32) << 16);
-        for (int pair = half; pair < pairs; pair += 2) {
-          __syncwarp();
-          const uint32_t c0 = from + (kGateTile ? 32 * pair : 64 * pair);
-          const uint32_t c1 = kGateTile ? from + p.columns / 2 + 32 * pair : c0 + 32;
-          if (kChunked && c > 0) {
-            float v[32];
-            load_columns(c0, v);
-            tc::wait_ld();
+        return ok;
+      };
+      const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
+      // 32 columns of the sums over K: FP32 blocks add up their chunks
+      const auto add_columns = [&](uint32_t at, bool first, float (&v)[32]) {
+        __syncwarp();
+        if (first) {
+          load_columns(at, v);
+          tc::wait_ld();
+        } else {
+          float more[32];
+          load_columns(at, more);
+          tc::wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) acc0[i] += v[i];
-            load_columns(c1, v);
-            tc::wait_ld();
+          for (int i = 0; i < 32; ++i) v[i] += more[i];
+        }
+      };
+
+      if constexpr (E == TcEpilogue::kGateGrad) {
+        // group by group of 32 columns; a group's factors are on their way while the sums (for
+        // the first) or the group before are worked on
+        FactorWords<T> f1, f2;
+        const auto prefetch = [&](int group) {
+          const int64_t n0 = it.n0 + 64 * (half + 2 * (group / 2)) + 32 * (group % 2);
+          if (row >= p.m || n0 >= p.n) return;
+          const int64_t place = (row * p.factors.groups + n0 / kFactorGroup) * 2;
+          load_factors<T>(p.factors, place, f1);
+          load_factors<T>(p.factors, place + 1, f2);
+        };
+        const auto finish = [&](int group, const float (&v)[32]) {
+          const int64_t n0 = it.n0 + 64 * (half + 2 * (group / 2)) + 32 * (group % 2);
+          if (n0 >= p.n) return;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) acc1[i] += v[i];
-          } else {
-            load_columns(c0, acc0);
-            load_columns(c1, acc1);
-            tc::wait_ld();
-          }
-          if (pair + 2 >= pairs) {  // the accumulator has been read
-            tc::fence_before_sync();
+          for (int which = 0; which < 2; ++which) {  // dg = dh f2, then du = dh f1
+            float d[32];
+            times_factors<T>(which == 0 ? f2 : f1, v, d);
+            if (row < p.m)
+              store_operand<T>(p.gated[which] + row * p.gated_stride + n0, p.gated_plane, d);
+            if (p.row_sums == nullptr) continue;
+            if (row >= p.m) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) d[i] = 0.0f;
+            }
             __syncwarp();
-            if (lane == 0) {
-              if (Cg == 2) arrive_remote(release + buffer * 8);
-              else mbar_arrive(&sum_empty[buffer]);
+            const float sum = sum_rows(d, lane);
+            const int64_t rows = it.m0 + rank * kRows + quadrant * 32;
+            if (rows < p.m) p.row_sums[(rows / 32 * 2 + which) * p.row_sums_stride + n0 + lane] = sum;
+          }
+        };
+        const int groups = half < pairs ? 2 * ((pairs - half + 1) / 2) : 0;
+        if (!kChunked && groups > 0) prefetch(0);  // FP32 has no registers for it
+        if constexpr (kChunked) {
+          float v0[32], v1[32];  // at most 128 columns: two groups a warp
+          for (int c = 0; c < chunks; ++c, ++sums) {
+            const int buffer = static_cast<int>(sums & 1);
+            if (!wait_sums(buffer)) break;
+            if (groups > 0) {
+              const uint32_t from = tmem + buffer * kMaxColumns + lanes + 64 * half;
+              add_columns(from, c == 0, v0);
+              add_columns(from + 32, c == 0, v1);
+            }
+            release_sums(buffer);
+          }
+          if (ok && groups > 0) {
+            prefetch(0);
+            finish(0, v0);
+            prefetch(1);
+            finish(1, v1);
+          }
+        } else {
+          const int buffer = static_cast<int>(sums & 1);
+          if (!wait_sums(buffer)) break;
+          ++sums;
+          const uint32_t from = tmem + buffer * kMaxColumns + lanes;
+          for (int group = 0; group < groups; ++group) {
+            float v[32];
+            add_columns(from + 64 * (half + 2 * (group / 2)) + 32 * (group % 2), true, v);
+            if (group + 1 == groups) release_sums(buffer);
+            finish(group, v);
+            if (group + 1 < groups) prefetch(group + 1);
+          }
+          if (groups == 0) release_sums(buffer);
+        }
+      } else {
+        // two groups of 32 columns at a time: a gate tile's g and u, else neighbours
+        const auto finish = [&](int pair, float (&v0)[32], float (&v1)[32]) {
+          if (row >= p.m) return;
+          if constexpr (kGateTile) {
+            const int64_t n0 = it.n0 + 32 * pair;
+            if (n0 >= p.n) return;
+            add_bias<T>(p.bias[0], n0, p.n, v0);
+            add_bias<T>(p.bias[1], n0, p.n, v1);
+            float h[32];
+            const auto gate = [&](auto tanh) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                float a, slope;
+                block_activation<decltype(tanh)::value>(v0[i], a, slope);
+                h[i] = a * v1[i];
+                v0[i] = a;
+                v1[i] *= slope;
+              }
+            };
+            if (p.activation == FHB_ACTIVATION_TANH) gate(std::true_type{});
+            else gate(std::false_type{});
+            store_operand<T>(p.gated[0] + row * p.gated_stride + n0, p.gated_plane, h);
+            if (p.factors.values != nullptr) {
+              const int64_t place = (row * p.factors.groups + n0 / kFactorGroup) * 2;
+              store_factors<T>(p.factors, place, v0);
+              store_factors<T>(p.factors, place + 1, v1);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float(&v)[32] = j == 0 ? v0 : v1;
+              const int64_t n0 = it.n0 + 64 * pair + 32 * j;
+              if (n0 >= p.n) break;
+              if constexpr (E == TcEpilogue::kPartial) {
+                float* out = p.partial + ((static_cast<int64_t>(it.group) * p.parts + it.part) * p.m + row) * p.partial_stride;
+                store_results<float>(out, n0, p.partial_stride, true, v);
+              } else {
+                add_bias<T>(p.bias[0], n0, p.n, v);
+                store_results<T>(static_cast<T*>(p.out[it.group]) + row * p.out_stride, n0, p.n, p.out_wide != 0, v);
+              }
             }
           }
-          if (!kChunked || c + 1 == chunks) finish(pair, acc0, acc1);
-        }
-        if (half >= pairs) {  // a tile of 64 columns leaves the second half of the warps idle
-          __syncwarp();
-          if (lane == 0) {
-            if (Cg == 2) arrive_remote(release + buffer * 8);
-            else mbar_arrive(&sum_empty[buffer]);
+        };
+        float acc0[32], acc1[32];
+        for (int c = 0; c < chunks; ++c, ++sums) {
+          const int buffer = static_cast<int>(sums & 1);
+          if (!wait_sums(buffer)) break;
+          const uint32_t from = tmem + buffer * kMaxColumns + lanes;
+          // FP32 blocks have at most 128 columns: a pair a warp, kept over the chunks
+          for (int pair = half; pair < pairs; pair += 2) {
+            const uint32_t c0 = from + (kGateTile ? 32 * pair : 64 * pair);
+            const uint32_t c1 = kGateTile ? from + p.columns / 2 + 32 * pair : c0 + 32;
+            add_columns(c0, !kChunked || c == 0, acc0);
+            add_columns(c1, !kChunked || c == 0, acc1);
+            if (pair + 2 >= pairs) release_sums(buffer);
+            if (!kChunked || c + 1 == chunks) finish(pair, acc0, acc1);
           }
+          // a tile of 64 columns leaves the second half of the warps idle
+          if (half >= pairs) release_sums(buffer);
         }
       }
     }
@@ -649,41 +741,48 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Rows of `cols` values into rows of `stride` bf16 (a multiple of 8, the rest zero): a copy, or
-// the three planes of FP32 values.
+// Rows of `cols` values into rows of `stride` bf16 (a multiple of 8, the rest zero): copies, or
+// the three planes of FP32 values. One matrix per blockIdx.y.
+struct PackJob {
+  const void* in;
+  bf16* out;
+  int64_t rows, cols, in_stride, stride, plane;
+};
+struct PackJobs {
+  PackJob job[kMaxOperands];
+};
 template <typename T>
-__global__ void __launch_bounds__(256)
-    pack_kernel(const T* __restrict__ in, int64_t rows, int64_t cols, int64_t in_stride,
-                bf16* __restrict__ out, int64_t stride, int64_t plane) {
-  const int64_t pieces = stride / 8;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * pieces; i += gridDim.x * 256ll) {
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJobs jobs) {
+  const PackJob& j = jobs.job[blockIdx.y];
+  const int64_t pieces = j.stride / 8;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < j.rows * pieces; i += gridDim.x * 256ll) {
     const int64_t row = i / pieces, c = (i % pieces) * 8;
-    const T* src = in + row * in_stride + c;
+    const T* src = static_cast<const T*>(j.in) + row * j.in_stride + c;
     float v[8];
-    if (sizeof(T) == 4 && c + 8 <= cols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+    if (sizeof(T) == 4 && c + 8 <= j.cols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
       const float4 x = reinterpret_cast<const float4*>(src)[0], y = reinterpret_cast<const float4*>(src)[1];
       v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_float(src[j]) : 0.0f;
+      for (int k = 0; k < 8; ++k) v[k] = c + k < j.cols ? to_float(src[k]) : 0.0f;
     }
-    bf16* dst = out + row * stride + c;
+    bf16* dst = j.out + row * j.stride + c;
     uint32_t w[3][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int k = 0; k < 4; ++k) {
       if (sizeof(T) == 2) {
-        w[0][j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+        w[0][k] = pack_bf16(v[2 * k], v[2 * k + 1]);
       } else {
         float x[3], y[3];
-        split_f32(v[2 * j], x[0], x[1], x[2]);
-        split_f32(v[2 * j + 1], y[0], y[1], y[2]);
+        split_f32(v[2 * k], x[0], x[1], x[2]);
+        split_f32(v[2 * k + 1], y[0], y[1], y[2]);
 #pragma unroll
-        for (int q = 0; q < 3; ++q) w[q][j] = pack_bf16(x[q], y[q]);
+        for (int q = 0; q < 3; ++q) w[q][k] = pack_bf16(x[q], y[q]);
       }
     }
 #pragma unroll
     for (int q = 0; q < (sizeof(T) == 2 ? 1 : 3); ++q)
-      *reinterpret_cast<uint4*>(dst + q * plane) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+      *reinterpret_cast<uint4*>(dst + q * j.plane) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
   }
 }
 
@@ -893,6 +992,8 @@ cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, const DeviceInfo
   args.activation = p.activation;
   args.partial = static_cast<float*>(workspace);
   args.partial_stride = plan.partial_stride;
+  args.row_sums = p.row_sums;
+  args.row_sums_stride = p.row_sums_stride;
   args.status = dev.status;
 
   Maps maps{};
@@ -931,26 +1032,31 @@ TcMatrix tc_result(void* room, int64_t rows, int64_t cols, int dtype) {
   return {static_cast<const bf16*>(room), rows, cols, stride, rows * stride, dtype == FHB_DTYPE_F32 ? 3 : 1};
 }
 
-size_t tc_operand_bytes(const void* p, int64_t rows, int64_t cols, int64_t stride, int dtype) {
-  return copies_by_tile(p, stride, dtype) ? 0 : tc_result_bytes(rows, cols, dtype);
+size_t tc_operand_bytes(const TcInput& in, int dtype) {
+  return copies_by_tile(in.p, in.stride, dtype) ? 0 : tc_result_bytes(in.rows, in.cols, dtype);
 }
 
-cudaError_t tc_operand(const void* p, int64_t rows, int64_t cols, int64_t stride, int dtype,
-                       void* room, TcMatrix* out, cudaStream_t stream) {
-  if (copies_by_tile(p, stride, dtype)) {
-    *out = {static_cast<const bf16*>(p), rows, cols, stride, 0, 1};
-    return cudaSuccess;
+TcMatrix tc_operand(const TcInput& in, int dtype, void* room) {
+  if (copies_by_tile(in.p, in.stride, dtype))
+    return {static_cast<const bf16*>(in.p), in.rows, in.cols, in.stride, 0, 1};
+  return tc_result(room, in.rows, in.cols, dtype);
+}
+
+cudaError_t launch_pack(const TcInput* in, const TcMatrix* out, int count, int dtype,
+                        cudaStream_t stream) {
+  PackJobs jobs{};
+  int used = 0;
+  int64_t most = 0;
+  for (int i = 0; i < count; ++i) {
+    if (in[i].p == nullptr || out[i].p == in[i].p || in[i].rows == 0) continue;
+    jobs.job[used++] = {in[i].p, const_cast<bf16*>(out[i].p), in[i].rows, in[i].cols, in[i].stride,
+                        out[i].stride, out[i].plane};
+    most = std::max(most, in[i].rows * (out[i].stride / 8));
   }
-  *out = tc_result(room, rows, cols, dtype);
-  const int64_t pieces = rows * (out->stride / 8);
-  if (pieces == 0) return cudaSuccess;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(blocks_of(pieces, 256), 2368));
-  if (dtype == FHB_DTYPE_F32)
-    pack_kernel<float><<<grid, 256, 0, stream>>>(static_cast<const float*>(p), rows, cols, stride,
-                                                 static_cast<bf16*>(room), out->stride, out->plane);
-  else
-    pack_kernel<bf16><<<grid, 256, 0, stream>>>(static_cast<const bf16*>(p), rows, cols, stride,
-                                                static_cast<bf16*>(room), out->stride, out->plane);
+  if (used == 0) return cudaSuccess;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks_of(most, 256), 2368)), used);
+  if (dtype == FHB_DTYPE_F32) pack_kernel<float><<<grid, 256, 0, stream>>>(jobs);
+  else pack_kernel<bf16><<<grid, 256, 0, stream>>>(jobs);
   return cudaGetLastError();
 }
 

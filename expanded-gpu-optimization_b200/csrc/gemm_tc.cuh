@@ -56,6 +56,9 @@ struct TcProduct {
   TcMatrix gated[2];
   TcFactors factors;
   int activation = 0;
+  // kGateGrad: the column sums of dg and du over every 32 rows, [m / 32][2][row_sums_stride]
+  float* row_sums = nullptr;
+  int64_t row_sums_stride = 0;
 };
 
 // Workspace of a product: the FP32 partial sums of its parts of K (0 where it has one).
@@ -63,12 +66,17 @@ size_t gemm_tc_workspace_bytes(const TcProduct& p, const DeviceInfo& dev);
 cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, const DeviceInfo& dev,
                            cudaStream_t stream);
 
-// `rows` x `cols` elements of type `dtype` with row stride `stride` as tensor-core operand:
-// the matrix itself where it can be copied by TMA, else its copy in `room` (bytes:
-// tc_operand_bytes; 0 where no copy is needed).
-size_t tc_operand_bytes(const void* p, int64_t rows, int64_t cols, int64_t stride, int dtype);
-cudaError_t tc_operand(const void* p, int64_t rows, int64_t cols, int64_t stride, int dtype,
-                       void* room, TcMatrix* out, cudaStream_t stream);
+// A caller's matrix: `rows` x `cols` elements of the block's type, rows `stride` apart.
+struct TcInput {
+  const void* p;
+  int64_t rows, cols, stride;
+};
+// The input as tensor-core operand: itself where TMA can copy its tiles, else its copy in `room`
+// (bytes: tc_operand_bytes, 0 where no copy is needed), which launch_pack makes.
+size_t tc_operand_bytes(const TcInput& in, int dtype);
+TcMatrix tc_operand(const TcInput& in, int dtype, void* room);
+cudaError_t launch_pack(const TcInput* in, const TcMatrix* out, int count, int dtype,
+                        cudaStream_t stream);
 // A matrix of the block's type in operand form at `room`, to be written by a product.
 size_t tc_result_bytes(int64_t rows, int64_t cols, int dtype);
 TcMatrix tc_result(void* room, int64_t rows, int64_t cols, int dtype);
