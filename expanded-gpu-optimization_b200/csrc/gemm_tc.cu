@@ -24,8 +24,8 @@ constexpr int kMaxColumns = 256;                 // result columns of a tile
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 32 * (kEpilogueWarps + 2);
 constexpr int kMaxSlots = 10;
-constexpr int kRingBytes = 208 * 1024;
-constexpr int kMaxTerms = 12;
+constexpr int kRingBytes = 216 * 1024;
+constexpr int kPlanes = 3;                       // of an FP32 operand
 constexpr int kMaxOperands = 5;  // of a block's products
 constexpr int kATileBytes = kRows * kKBlock * 2;  // 16 KB
 
@@ -38,8 +38,8 @@ struct Args {
   int tiles_m, tiles_n, groups, parts;
   int k_blocks, part_blocks;  // of K, and of each part of K
   int columns;                // columns of a tile (both halves of a gate tile)
-  int slots, terms;
-  uint8_t a_map[kMaxTerms], b_map[kMaxTerms], a_plane[kMaxTerms], b_plane[kMaxTerms];
+  int slots, slot_blocks;     // of the ring; blocks of K in a slot
+  int sum_terms;
   int a_k_major, b_k_major;
   int a_rows;                 // rows of one A copy (fewer than 128 where m is small)
   uint32_t idesc;
@@ -386,10 +386,14 @@ __device__ __forceinline__ Item item_at(const Args& p, int64_t index) {
   return it;
 }
 
-// FP32 blocks: the tensor core cuts each sum to FP32 instead of rounding it, an error that
-// grows with the number of additions and has a sign. K is summed in chunks of kChunkBlocks
-// ring slots per term, and the chunks in registers, rounded.
+// FP32 blocks. A slot holds the three planes of 64 of K of both operands, for six of their nine
+// products (the others are below 2^-24 of the whole): the large one has an accumulator of its
+// own and the five small ones share another, kSmallColumns on. The tensor core cuts each sum to
+// FP32 instead of rounding it, an error that grows with the number of additions and has a sign:
+// the small products do not add to it that way, and K is summed in chunks of kChunkBlocks slots
+// per term, the chunks in registers, rounded.
 constexpr int kChunkBlocks = 2;
+constexpr int kSmallColumns = 128;
 template <typename T>
 __device__ __forceinline__ int chunk_count(int blocks) {
   return sizeof(T) == 4 ? (blocks + kChunkBlocks - 1) / kChunkBlocks : 1;
@@ -400,6 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     gemm_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
   constexpr bool kGateTile = E == TcEpilogue::kGate;
   constexpr bool kChunked = sizeof(T) == 4;
+  constexpr int kCopies = kChunked ? kPlanes : 1;  // planes that come with one copy
   extern __shared__ unsigned char raw[];
   __shared__ uint64_t full[kMaxSlots], empty[kMaxSlots], sum_full[2], sum_empty[2];
   __shared__ uint32_t tmem_at;
@@ -407,7 +412,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = Cg == 2 ? cluster_rank() : 0;
   const int b_rows = p.columns / Cg;  // rows of this CTA's B tile
-  const uint32_t slot_bytes = kATileBytes + static_cast<uint32_t>(b_rows) * kKBlock * 2;
+  const uint32_t b_tile_bytes = static_cast<uint32_t>(b_rows) * kKBlock * 2;
+  const uint32_t block_bytes = kCopies * (kATileBytes + b_tile_bytes);  // of one block of K
+  const uint32_t slot_bytes = block_bytes * p.slot_blocks;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.slots; ++s) {
@@ -438,48 +445,51 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       int64_t issued = 0;
       const uint32_t a_bytes = p.a_k_major ? static_cast<uint32_t>(p.a_rows) * kKBlock * 2 : kATileBytes;
-      const uint32_t bytes = Cg * (a_bytes + static_cast<uint32_t>(b_rows) * kKBlock * 2);
+      const uint32_t bytes = Cg * kCopies * (a_bytes + b_tile_bytes);
+      const uint32_t first_bar = Cg == 2 ? in_cta(smem_u32(&full[0]), 0) : smem_u32(&full[0]);
       for (int64_t index = first; ok && index < items; index += stride) {
         const Item it = item_at<Cg, kGateTile>(p, index);
         const int chunks = chunk_count<T>(it.blocks);
-        const int64_t a0 = it.m0 + rank * kRows;
+        const int a0 = static_cast<int>(it.m0 + rank * kRows);
+        const int b0 = static_cast<int>(it.n0) + (kGateTile ? 0 : static_cast<int>(rank) * b_rows);
         for (int c = 0; ok && c < chunks; ++c) {
           const int low = it.first_block + (kChunked ? c * kChunkBlocks : 0);
           const int high = kChunked ? min(low + kChunkBlocks, it.first_block + it.blocks)
                                     : it.first_block + it.blocks;
-          for (int t = 0; ok && t < p.terms; ++t) {
-            const CUtensorMap* am = &maps.a[p.a_map[t] + (p.groups == 2 ? it.group : 0)];
-            const CUtensorMap* bm = &maps.b[p.b_map[t]];
-            for (int kb = low; kb < high; ++kb) {
+          for (int t = 0; ok && t < p.sum_terms; ++t) {
+            const CUtensorMap* am = &maps.a[p.groups == 2 ? it.group : t];
+            const CUtensorMap* bm = &maps.b[kGateTile && Cg == 2 ? static_cast<int>(rank) : t];
+            for (int kb = low; kb < high; kb += p.slot_blocks) {
               if (!mbar_wait_bounded(&empty[slot], phase ^ 1, p.status, FHB_STATUS_MMA_TIMEOUT)) {
                 ok = false;
                 break;
               }
-              if (rank == 0) mbar_arrive_expect_tx(&full[slot], bytes);
-              const uint32_t bar = Cg == 2 ? in_cta(smem_u32(&full[slot]), 0) : smem_u32(&full[slot]);
-              const uint32_t at = ring + slot * slot_bytes, bt = at + kATileBytes;
-              const int k0 = kb * kKBlock;
-              if (p.a_k_major) {
-                copy_tile<Cg>(at, am, k0, static_cast<int>(a0), p.a_plane[t], bar);
-              } else {
-                copy_tile<Cg>(at, am, static_cast<int>(a0), k0, p.a_plane[t], bar);
-                copy_tile<Cg>(at + 8192, am, static_cast<int>(a0) + 64, k0, p.a_plane[t], bar);
-              }
-              if (kGateTile) {
-                // one half of the columns from each weight (always K-major)
-                if (Cg == 2) {
-                  copy_tile<Cg>(bt, &maps.b[rank], k0, static_cast<int>(it.n0), p.b_plane[t], bar);
+              const int blocks = min(p.slot_blocks, high - kb);
+              if (rank == 0) mbar_arrive_expect_tx(&full[slot], bytes * blocks);
+              const uint32_t bar = first_bar + slot * 8;
+              for (int j = 0; j < blocks; ++j) {
+                const uint32_t at = ring + slot * slot_bytes + j * block_bytes;
+                const uint32_t bt = at + kCopies * kATileBytes;
+                const int k0 = (kb + j) * kKBlock;
+                if (p.a_k_major) {
+                  copy_tile<Cg>(at, am, k0, a0, 0, bar);
                 } else {
-                  copy_tile<Cg>(bt, &maps.b[0], k0, static_cast<int>(it.n0), p.b_plane[t], bar);
-                  copy_tile<Cg>(bt + b_rows * kKBlock, &maps.b[1], k0, static_cast<int>(it.n0), p.b_plane[t], bar);
+                  copy_tile<Cg>(at, am, a0, k0, 0, bar);
+                  copy_tile<Cg>(at + kCopies * 8192, am, a0 + 64, k0, 0, bar);
                 }
-              } else {
-                const int b0 = static_cast<int>(it.n0) + static_cast<int>(rank) * b_rows;
-                if (p.b_k_major)
-                  copy_tile<Cg>(bt, bm, k0, b0, p.b_plane[t], bar);
-                else
+                if (kGateTile && Cg == 1) {
+                  // half of the columns from each weight; FP32: plane by plane, so that the
+                  // halves of a plane are neighbours
+                  for (int q = 0; q < kCopies; ++q) {
+                    copy_tile<Cg>(bt + q * b_tile_bytes, &maps.b[0], k0, b0, q, bar);
+                    copy_tile<Cg>(bt + q * b_tile_bytes + b_tile_bytes / 2, &maps.b[1], k0, b0, q, bar);
+                  }
+                } else if (p.b_k_major) {
+                  copy_tile<Cg>(bt, bm, k0, b0, 0, bar);
+                } else {
                   for (int i = 0; i < b_rows; i += 64)
-                    copy_tile<Cg>(bt + i * kKBlock * 2, bm, b0 + i, k0, p.b_plane[t], bar);
+                    copy_tile<Cg>(bt + i * kCopies * 128, bm, b0 + i, k0, 0, bar);
+                }
               }
               ++issued;
               if (++slot == p.slots) {
@@ -508,6 +518,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       int64_t sums = 0;
       bool ok = true;
       const uint32_t a_step = p.a_k_major ? 2 : 128, b_step = p.b_k_major ? 2 : 128;  // 16 of K
+      // bytes from plane to plane and (operand across K) from one block of 64 rows to the next
+      const uint32_t a_plane = p.a_k_major ? static_cast<uint32_t>(p.a_rows) * 128 : 8192;
+      const uint32_t b_plane = p.b_k_major ? b_tile_bytes : 8192;
+      const uint64_t a_desc = tile_descriptor(0, kCopies * 8192), b_desc = a_desc;
       for (int64_t index = first; ok && index < items; index += stride) {
         const Item it = item_at<Cg, kGateTile>(p, index);
         const int chunks = chunk_count<T>(it.blocks);
@@ -519,20 +533,43 @@ __global__ void __launch_bounds__(kThreads, 1)
                                  p.status, FHB_STATUS_MMA_TIMEOUT);
           if (!ok) break;
           tc::fence_after_sync();
-          const int steps = blocks * p.terms;
-          for (int i = 0; i < steps; ++i) {
-            ok = mbar_wait_bounded(&full[slot], phase, p.status, FHB_STATUS_MMA_TIMEOUT);
-            if (!ok) break;
-            tc::fence_after_sync();
-            const uint32_t at = ring + slot * slot_bytes;
-            mma_slot<Cg>(tmem + buffer * kMaxColumns, tile_descriptor(at, 8192),
-                         tile_descriptor(at + kATileBytes, 8192), a_step, b_step, p.idesc, i != 0);
-            commit<Cg>(&empty[slot]);
-            if (++slot == p.slots) {
-              slot = 0;
-              phase ^= 1;
+          const uint32_t d = tmem + buffer * kMaxColumns;
+          uint32_t accumulate = 0;
+          for (int t = 0; ok && t < p.sum_terms; ++t)
+            for (int kb = 0; kb < blocks; kb += p.slot_blocks) {
+              ok = mbar_wait_bounded(&full[slot], phase, p.status, FHB_STATUS_MMA_TIMEOUT);
+              if (!ok) break;
+              tc::fence_after_sync();
+              const uint32_t at = ring + slot * slot_bytes;
+              if constexpr (kChunked) {
+                const uint32_t bt = at + kCopies * kATileBytes;
+                const uint64_t a0 = a_desc | (at >> 4), b0 = b_desc | (bt >> 4);
+                const uint64_t a1 = a0 + (a_plane >> 4), b1 = b0 + (b_plane >> 4);
+                const uint64_t a2 = a1 + (a_plane >> 4), b2 = b1 + (b_plane >> 4);
+                const uint32_t small = d + kSmallColumns;
+                mma_slot<Cg>(small, a2, b0, a_step, b_step, p.idesc, accumulate);
+                mma_slot<Cg>(d, a0, b0, a_step, b_step, p.idesc, accumulate);
+                mma_slot<Cg>(small, a0, b2, a_step, b_step, p.idesc, 1);
+                mma_slot<Cg>(small, a1, b1, a_step, b_step, p.idesc, 1);
+                mma_slot<Cg>(small, a1, b0, a_step, b_step, p.idesc, 1);
+                mma_slot<Cg>(small, a0, b1, a_step, b_step, p.idesc, 1);
+                accumulate = 1;
+              } else {
+                const int here = min(p.slot_blocks, blocks - kb);
+                uint64_t a0 = a_desc | (at >> 4), b0 = b_desc | ((at + kATileBytes) >> 4);
+                for (int j = 0; j < here; ++j) {
+                  mma_slot<Cg>(d, a0, b0, a_step, b_step, p.idesc, accumulate);
+                  accumulate = 1;
+                  a0 += block_bytes >> 4;
+                  b0 += block_bytes >> 4;
+                }
+              }
+              commit<Cg>(&empty[slot]);
+              if (++slot == p.slots) {
+                slot = 0;
+                phase ^= 1;
+              }
             }
-          }
           if (ok) commit<Cg>(&sum_full[buffer]);
         }
       }
@@ -565,18 +602,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         return ok;
       };
       const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
-      // 32 columns of the sums over K: FP32 blocks add up their chunks
+      // 32 columns of the sums over K: FP32 blocks add both accumulators and their chunks
       const auto add_columns = [&](uint32_t at, bool first, float (&v)[32]) {
         __syncwarp();
-        if (first) {
+        if constexpr (kChunked) {
+          float more[32];
+          load_columns(at + kSmallColumns, more);
+          if (first) {
+            load_columns(at, v);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += more[i];
+          } else {
+            float large[32];
+            load_columns(at, large);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] += large[i] + more[i];
+          }
+        } else {
           load_columns(at, v);
           tc::wait_ld();
-        } else {
-          float more[32];
-          load_columns(at, more);
-          tc::wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] += more[i];
         }
       };
 
@@ -791,37 +837,42 @@ int64_t blocks_of(int64_t x, int64_t size) { return (x + size - 1) / size; }
 
 // ---- the plan of a product: tile, pairing, parts of K ----
 struct Plan {
-  int cg, columns, parts, part_blocks, k_blocks, tiles_m, tiles_n, terms, slots, grid;
+  int cg, columns, parts, part_blocks, k_blocks, tiles_m, tiles_n, slots, slot_blocks, grid;
   int64_t partial_stride;
 };
+// Bytes of the ring that one block of K takes.
+int block_bytes_of(bool wide, int cg, int columns) {
+  return (wide ? kPlanes : 1) * (kATileBytes + columns / cg * kKBlock * 2);
+}
 
-// Chooses by an estimate of the launch's cycles. A ring slot costs its MMAs (4 x columns / 2
-// cycles a CTA, the same work in a pair with half the B tile each) or the copies of its bytes
-// (about 64 a cycle), whichever is longer; an item costs about 2,000 cycles more (its first
-// copies, its last results), and a second launch that adds the parts about 3,000 and its bytes.
+// Chooses by an estimate of the launch's cycles. A block of K costs its MMAs (4 x columns / 2
+// cycles a product of planes, the same in a pair with half the B tile each) or the copies of its
+// bytes (about 64 a cycle), whichever is longer; an item costs about 2,000 cycles more (its
+// first copies, its last results), and a second launch that adds the parts about 3,000 and its
+// bytes.
 Plan plan_of(const TcProduct& p, const DeviceInfo& dev) {
   const bool wide = p.dtype == FHB_DTYPE_F32, gate = p.epilogue == TcEpilogue::kGate;
-  const int terms = p.sum_terms * (wide ? 6 : 1);
   const int k_blocks = static_cast<int>(blocks_of(p.k, kKBlock));
   const int64_t n_columns = gate ? 2 * p.n : p.n;
   Plan best{};
   double least = 0.0;
   for (int cg = 1; cg <= 2; ++cg)
-    for (int columns = 64; columns <= (wide ? 128 : kMaxColumns); columns *= 2) {
+    for (int columns = 64; columns <= (wide ? kSmallColumns : kMaxColumns); columns *= 2) {
       if (cg == 2 && columns < 128) continue;  // an operand across K comes in blocks of 64
       if (cg == 2 && p.m <= kRows) continue;
       const int64_t tiles_m = blocks_of(p.m, kRows * cg);
       const int64_t tiles_n = blocks_of(n_columns, columns);
       const int64_t tiles = tiles_m * tiles_n * p.groups;
       const int64_t units = dev.sms / cg;
-      const int most = p.epilogue == TcEpilogue::kStore ? std::min(k_blocks, 64) : 1;
-      for (int parts = 1; parts <= most; ++parts) {
-        if (parts > 1 && tiles * (parts - 1) >= 4 * units) break;
-        const int part_blocks = static_cast<int>(blocks_of(k_blocks, parts));
-        if (blocks_of(k_blocks, part_blocks) != parts) continue;
-        const double mma = 2.0 * columns, copy = (kATileBytes + 128.0 * columns / cg) / 64.0;
-        const double item = 2000.0 + static_cast<double>(part_blocks) * terms * std::max(mma, copy);
-        double cycles = static_cast<double>(blocks_of(tiles * parts, units)) * item;
+      const double mma = 2.0 * columns * (wide ? 6 : 1);
+      const double block = p.sum_terms * std::max(mma, block_bytes_of(wide, cg, columns) / 64.0);
+      // parts that fill one, two, three or four rounds of the SMs
+      for (int rounds = 0; rounds <= (p.epilogue == TcEpilogue::kStore ? 4 : 0); ++rounds) {
+        const int64_t wanted = rounds == 0 ? 1 : units * rounds / tiles;
+        if (rounds > 0 && (wanted < 2 || wanted > 128)) continue;
+        const int part_blocks = static_cast<int>(blocks_of(k_blocks, wanted));
+        const int parts = static_cast<int>(blocks_of(k_blocks, part_blocks));
+        double cycles = static_cast<double>(blocks_of(tiles * parts, units)) * (2000.0 + part_blocks * block);
         if (parts > 1)
           cycles += 3000.0 + 8.0 * static_cast<double>(p.m) * n_columns * p.groups * parts / (64.0 * dev.sms);
         if (least == 0.0 || cycles < least) {
@@ -837,8 +888,10 @@ Plan plan_of(const TcProduct& p, const DeviceInfo& dev) {
       }
     }
   best.k_blocks = k_blocks;
-  best.terms = terms;
-  best.slots = std::min(kMaxSlots, kRingBytes / (kATileBytes + best.columns / best.cg * kKBlock * 2));
+  // two blocks of K a slot halve the waits between MMAs, where at least three slots remain
+  const int block_bytes = block_bytes_of(wide, best.cg, best.columns);
+  best.slot_blocks = !wide && best.part_blocks > 1 && kRingBytes / (2 * block_bytes) >= 3 ? 2 : 1;
+  best.slots = std::min(kMaxSlots, kRingBytes / (best.slot_blocks * block_bytes));
   best.partial_stride = round_up(p.n, 32);
   return best;
 }
@@ -850,13 +903,14 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiled g_encode = nullptr;
 
-// Tiles of 64 columns (128 bytes, swizzled) by `box_rows` rows of one plane.
-bool tile_map(const TcMatrix& x, int box_rows, CUtensorMap* out) {
+// Tiles of 64 columns (128 bytes, swizzled) by `box_rows` rows of `box_planes` planes.
+bool tile_map(const TcMatrix& x, int box_rows, int box_planes, CUtensorMap* out) {
   const cuuint64_t size[3] = {static_cast<cuuint64_t>(x.cols), static_cast<cuuint64_t>(x.rows),
                               static_cast<cuuint64_t>(x.planes)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(x.stride) * 2,
                                  static_cast<cuuint64_t>(x.planes > 1 ? x.plane : x.stride) * 2};
-  const cuuint32_t box[3] = {kKBlock, static_cast<cuuint32_t>(box_rows), 1}, step[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {kKBlock, static_cast<cuuint32_t>(box_rows),
+                             static_cast<cuuint32_t>(box_planes)}, step[3] = {1, 1, 1};
   const auto encode = [&] {
     return g_encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<bf16*>(x.p), size, strides,
                     box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -869,8 +923,8 @@ bool tile_map(const TcMatrix& x, int box_rows, CUtensorMap* out) {
   return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && encode();
 }
 
-size_t smem_bytes(const Plan& plan) {
-  return static_cast<size_t>(plan.slots) * (kATileBytes + plan.columns / plan.cg * kKBlock * 2) + 1024;
+size_t smem_bytes(const Plan& plan, bool wide) {
+  return static_cast<size_t>(plan.slots) * plan.slot_blocks * block_bytes_of(wide, plan.cg, plan.columns) + 1024;
 }
 
 template <int Cg, TcEpilogue E, typename T>
@@ -882,7 +936,7 @@ cudaError_t launch(const Maps& maps, const Args& args, const Plan& plan, cudaStr
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(plan.grid);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem_bytes(plan);
+  cfg.dynamicSmemBytes = smem_bytes(plan, sizeof(T) == 4);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = Cg == 2 ? 1 : 0;
@@ -960,16 +1014,8 @@ cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, const DeviceInfo
   args.part_blocks = plan.part_blocks;
   args.columns = plan.columns;
   args.slots = plan.slots;
-  // FP32: the products of planes whose sizes multiply to 2^-16 of the whole or more, smallest
-  // first (the dropped ones are below 2^-24)
-  constexpr uint8_t planes[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
-  for (int q = 0; q < (wide ? 6 : 1); ++q)
-    for (int s = 0; s < p.sum_terms; ++s) {
-      const int t = args.terms++;
-      args.a_map[t] = args.b_map[t] = static_cast<uint8_t>(s);
-      args.a_plane[t] = wide ? planes[q][0] : 0;
-      args.b_plane[t] = wide ? planes[q][1] : 0;
-    }
+  args.slot_blocks = plan.slot_blocks;
+  args.sum_terms = p.sum_terms;
   args.a_k_major = p.a_k_major;
   args.b_k_major = p.b_k_major;
   args.a_rows = static_cast<int>(std::min<int64_t>(kRows, round_up(p.m, 8)));
@@ -998,11 +1044,12 @@ cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, const DeviceInfo
 
   Maps maps{};
   const int b_rows = plan.columns / plan.cg;
+  const int planes = wide ? kPlanes : 1;
   const int a_box = p.a_k_major ? args.a_rows : kKBlock;
   const int b_box = !p.b_k_major ? kKBlock : gate ? plan.columns / 2 : b_rows;
   for (int i = 0; i < 2; ++i) {
-    if (!tile_map(p.a[p.a[i].p != nullptr ? i : 0], a_box, &maps.a[i]) ||
-        !tile_map(p.b[p.b[i].p != nullptr ? i : 0], b_box, &maps.b[i]))
+    if (!tile_map(p.a[p.a[i].p != nullptr ? i : 0], a_box, planes, &maps.a[i]) ||
+        !tile_map(p.b[p.b[i].p != nullptr ? i : 0], b_box, gate && plan.cg == 1 ? 1 : planes, &maps.b[i]))
       return cudaErrorInvalidValue;
   }
   switch (p.epilogue) {
