@@ -75,7 +75,9 @@ __device__ __forceinline__ uint32_t in_cta(uint32_t smem, uint32_t rank) {
   return r;
 }
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  // relaxed: what it orders are TMEM reads, by the tcgen05 fence before it; a release would wait
+  // for the thread's stores to memory (3,000 cycles a tile)
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 template <int Cg>
@@ -267,12 +269,34 @@ __device__ __forceinline__ void store_results(T* row, int64_t n0, int64_t n, boo
     if (n0 + i < n) p[i] = from_float<T>(v[i]);
 }
 
+// Adds bias[n0 + i], the same for all lanes: in 16-byte loads where all 32 exist.
 template <typename T>
 __device__ __forceinline__ void add_bias(const void* bias, int64_t n0, int64_t n, float (&v)[32]) {
   if (bias == nullptr) return;
+  const T* p = static_cast<const T*>(bias) + n0;
+  if (n0 + 32 <= n && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    constexpr int kEach = 16 / sizeof(T);
+    uint4 w[32 / kEach];
+#pragma unroll
+    for (int i = 0; i < 32 / kEach; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+#pragma unroll
+    for (int i = 0; i < 32 / kEach; ++i) {
+      const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (sizeof(T) == 4) {
+          v[4 * i + j] += __uint_as_float(u[j]);
+        } else {
+          v[8 * i + 2 * j] += __uint_as_float(u[j] << 16);
+          v[8 * i + 2 * j + 1] += __uint_as_float(u[j] & 0xFFFF0000u);
+        }
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 32; ++i)
-    if (n0 + i < n) v[i] += to_float(static_cast<const T*>(bias)[n0 + i]);
+    if (n0 + i < n) v[i] += to_float(p[i]);
 }
 
 // The power of 2 that brings a group's largest magnitude into [2^14, 2^15), the top of f16's
@@ -367,20 +391,22 @@ struct Item {
   int group, part, first_block, blocks;
   int64_t m0, n0;  // first row of the tile (of the pair), first column (gate: feature)
 };
+// (32-bit divisions: there are fewer than 2^31 items, and 64-bit ones took 3,000 cycles an item)
 template <int Cg, bool Gate>
-__device__ __forceinline__ Item item_at(const Args& p, int64_t index) {
-  const int tiles = p.tiles_m * p.tiles_n;
+__device__ __forceinline__ Item item_at(const Args& p, uint32_t index) {
+  const uint32_t tiles = static_cast<uint32_t>(p.tiles_m) * static_cast<uint32_t>(p.tiles_n);
   Item it;
-  const int rest = static_cast<int>(index / tiles);
-  int tile = static_cast<int>(index % tiles);
-  it.part = rest % p.parts;
-  it.group = rest / p.parts;
+  const uint32_t rest = index / tiles;
+  uint32_t tile = index - rest * tiles;
+  it.group = static_cast<int>(rest / p.parts);
+  it.part = static_cast<int>(rest) - it.group * p.parts;
   // bands of 8 tile rows, column by column: the tiles in flight share their operands in L2
-  const int band = tile / (8 * p.tiles_n);
-  const int rows = min(8, p.tiles_m - 8 * band);
-  tile -= band * 8 * p.tiles_n;
-  it.m0 = static_cast<int64_t>(8 * band + tile % rows) * (kRows * Cg);
-  it.n0 = static_cast<int64_t>(tile / rows) * (Gate ? p.columns / 2 : p.columns);
+  const uint32_t band_tiles = 8u * static_cast<uint32_t>(p.tiles_n), band = tile / band_tiles;
+  const uint32_t rows = min(8u, static_cast<uint32_t>(p.tiles_m) - 8u * band);
+  tile -= band * band_tiles;
+  const uint32_t column = tile / rows;
+  it.m0 = static_cast<int64_t>(8u * band + (tile - column * rows)) * (kRows * Cg);
+  it.n0 = static_cast<int64_t>(column) * (Gate ? p.columns / 2 : p.columns);
   it.first_block = it.part * p.part_blocks;
   it.blocks = min(p.part_blocks, p.k_blocks - it.first_block);
   return it;
@@ -434,8 +460,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after_sync();
   const uint32_t tmem = tmem_at;
 
-  const int64_t items = static_cast<int64_t>(p.tiles_m) * p.tiles_n * p.parts * p.groups;
-  const int64_t first = blockIdx.x / Cg, stride = gridDim.x / Cg;
+  const uint32_t items = static_cast<uint32_t>(p.tiles_m) * p.tiles_n * p.parts * p.groups;
+  const uint32_t first = blockIdx.x / Cg, stride = gridDim.x / Cg;
 
   if (warp == kEpilogueWarps) {
     // ---- copies ----
@@ -447,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t a_bytes = p.a_k_major ? static_cast<uint32_t>(p.a_rows) * kKBlock * 2 : kATileBytes;
       const uint32_t bytes = Cg * kCopies * (a_bytes + b_tile_bytes);
       const uint32_t first_bar = Cg == 2 ? in_cta(smem_u32(&full[0]), 0) : smem_u32(&full[0]);
-      for (int64_t index = first; ok && index < items; index += stride) {
+      for (uint32_t index = first; ok && index < items; index += stride) {
         const Item it = item_at<Cg, kGateTile>(p, index);
         const int chunks = chunk_count<T>(it.blocks);
         const int a0 = static_cast<int>(it.m0 + rank * kRows);
@@ -522,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t a_plane = p.a_k_major ? static_cast<uint32_t>(p.a_rows) * 128 : 8192;
       const uint32_t b_plane = p.b_k_major ? b_tile_bytes : 8192;
       const uint64_t a_desc = tile_descriptor(0, kCopies * 8192), b_desc = a_desc;
-      for (int64_t index = first; ok && index < items; index += stride) {
+      for (uint32_t index = first; ok && index < items; index += stride) {
         const Item it = item_at<Cg, kGateTile>(p, index);
         const int chunks = chunk_count<T>(it.blocks);
         for (int c = 0; ok && c < chunks; ++c, ++sums) {
@@ -581,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t release = Cg == 2 ? in_cta(smem_u32(&sum_empty[0]), 0) : smem_u32(&sum_empty[0]);
     int64_t sums = 0;
     bool ok = true;
-    for (int64_t index = first; ok && index < items; index += stride) {
+    for (uint32_t index = first; ok && index < items; index += stride) {
       const Item it = item_at<Cg, kGateTile>(p, index);
       const int chunks = chunk_count<T>(it.blocks);
       const int64_t row = it.m0 + rank * kRows + quadrant * 32 + lane;
@@ -1003,6 +1029,9 @@ cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, const DeviceInfo
                            cudaStream_t stream) {
   const Plan plan = plan_of(p, dev);
   const bool wide = p.dtype == FHB_DTYPE_F32, gate = p.epilogue == TcEpilogue::kGate;
+  // items are counted in 32 bits, with room for a last stride beyond them
+  if (static_cast<int64_t>(plan.tiles_m) * plan.tiles_n > 0x70000000 / (plan.parts * p.groups))
+    return cudaErrorInvalidValue;
   Args args{};
   args.m = p.m;
   args.n = p.n;
