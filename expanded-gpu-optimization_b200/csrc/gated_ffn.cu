@@ -106,9 +106,18 @@ __global__ void __launch_bounds__(256) column_totals_kernel(const __grid_constan
   const int64_t c = blockIdx.x * 32ll + lane;
   const int64_t parts = (src.rows + s.part_rows - 1) / s.part_rows;
   float total = 0.0f;
-  if (c < src.columns)
-    for (int64_t part = warp; part < parts; part += 8)
-      total += s.parts[(blockIdx.y * s.part_count + part) * s.widest + c];
+  if (c < src.columns) {
+    const float* in = s.parts + blockIdx.y * s.part_count * s.widest + c;
+    int64_t part = warp;
+    for (; part + 56 < parts; part += 64) {  // eight parts in flight
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = in[(part + 8 * k) * s.widest];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) total += v[k];
+    }
+    for (; part < parts; part += 8) total += in[part * s.widest];
+  }
   __shared__ float by_warp[8][32];
   by_warp[warp][lane] = total;
   __syncthreads();

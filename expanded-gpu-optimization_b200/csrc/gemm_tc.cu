@@ -1,9 +1,9 @@
 // Matrix products of the gated feed-forward block on the tensor cores (tcgen05, TMEM, TMA).
 //
-// One persistent CTA per SM (or a pair of CTAs on two SMs that share a 256-row tile): warp 8
-// copies operand tiles of 64 of K into a ring in shared memory (TMA, 128-byte swizzle), warp 9
-// issues the MMAs into one of two TMEM accumulators, and warps 0-7 turn the other accumulator
-// into results. Operands may lie along K or across it in memory: the tile copies and the MMA
+// One persistent CTA per SM (or a pair of CTAs on two SMs that share a 256-row tile): warp 16
+// copies operand tiles of 64 of K into a ring in shared memory (TMA, 128-byte swizzle), warp 17
+// issues the MMAs into one of two TMEM accumulators, and warps 0-15 turn the other accumulator
+// into results, 16 columns of 32 rows at a time. Operands may lie along K or across it in memory: the tile copies and the MMA
 // descriptors follow, nothing is transposed in a pass of its own.
 #include "gemm_tc.cuh"
 
@@ -21,7 +21,8 @@ namespace {
 constexpr int kKBlock = 64;                      // K of one ring slot: 128 bytes of bf16
 constexpr int kRows = 128;                       // result rows of one CTA
 constexpr int kMaxColumns = 256;                 // result columns of a tile
-constexpr int kEpilogueWarps = 8;
+constexpr int kEpilogueWarps = 16;
+constexpr int kGroup = 16;                       // columns that a thread works on together
 constexpr int kThreads = 32 * (kEpilogueWarps + 2);
 constexpr int kMaxSlots = 10;
 constexpr int kRingBytes = 216 * 1024;
@@ -163,24 +164,6 @@ __device__ __forceinline__ void free_tmem(uint32_t tmem) {
     tc::tmem_dealloc(tmem, 512);
 }
 
-// 32 consecutive TMEM columns of the warp's 32 rows: one row per lane.
-__device__ __forceinline__ void load_columns(uint32_t tmem, float (&v)[32]) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(tmem)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-
 // 32 bytes in one access, 32-byte aligned: a whole memory sector per thread.
 __device__ __forceinline__ void store32(void* p, const uint32_t* v) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]),
@@ -215,19 +198,18 @@ __device__ __forceinline__ void split_f32(float x, float& a, float& b, float& c)
   c = (x - a) - b;
 }
 
-// 32 values of a row in operand form (bf16, or three planes), 32-byte aligned.
+// 16 values of a row in operand form (bf16, or three planes), 32-byte aligned.
 template <typename T>
-__device__ __forceinline__ void store_operand(bf16* p, int64_t plane, const float (&v)[32]) {
-  uint32_t w[16];
+__device__ __forceinline__ void store_operand(bf16* p, int64_t plane, const float (&v)[kGroup]) {
+  uint32_t w[8];
   if (sizeof(T) == 2) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+    for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
     store32(p, w);
-    store32(p + 16, w + 8);
   } else {
-    uint32_t w1[16], w2[16];
+    uint32_t w1[8], w2[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
       float a[2], b[2], c[2];
       split_f32(v[2 * i], a[0], b[0], c[0]);
       split_f32(v[2 * i + 1], a[1], b[1], c[1]);
@@ -236,51 +218,47 @@ __device__ __forceinline__ void store_operand(bf16* p, int64_t plane, const floa
       w2[i] = pack_bf16(c[0], c[1]);
     }
     store32(p, w);
-    store32(p + 16, w + 8);
     store32(p + plane, w1);
-    store32(p + plane + 16, w1 + 8);
     store32(p + 2 * plane, w2);
-    store32(p + 2 * plane + 16, w2 + 8);
   }
 }
 
-// 32 results of a row from column n0 on, those below n.
+// 16 results of a row from column n0 on, those below n.
 template <typename T>
 __device__ __forceinline__ void store_results(T* row, int64_t n0, int64_t n, bool wide,
-                                              const float (&v)[32]) {
+                                              const float (&v)[kGroup]) {
   T* p = row + n0;
-  if (wide && n0 + 32 <= n) {
-    uint32_t w[32];
+  if (wide && n0 + kGroup <= n) {
+    uint32_t w[16];
     if (sizeof(T) == 2) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+      for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
       store32(p, w);
-      store32(p + 16, w + 8);
     } else {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) store32(p + 8 * i, w + 8 * i);
+      for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i]);
+      store32(p, w);
+      store32(p + 8, w + 8);
     }
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
+  for (int i = 0; i < kGroup; ++i)
     if (n0 + i < n) p[i] = from_float<T>(v[i]);
 }
 
-// Adds bias[n0 + i], the same for all lanes: in 16-byte loads where all 32 exist.
+// Adds bias[n0 + i], the same for all lanes: in 16-byte loads where all 16 exist.
 template <typename T>
-__device__ __forceinline__ void add_bias(const void* bias, int64_t n0, int64_t n, float (&v)[32]) {
+__device__ __forceinline__ void add_bias(const void* bias, int64_t n0, int64_t n, float (&v)[kGroup]) {
   if (bias == nullptr) return;
   const T* p = static_cast<const T*>(bias) + n0;
-  if (n0 + 32 <= n && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+  if (n0 + kGroup <= n && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
     constexpr int kEach = 16 / sizeof(T);
-    uint4 w[32 / kEach];
+    uint4 w[kGroup / kEach];
 #pragma unroll
-    for (int i = 0; i < 32 / kEach; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    for (int i = 0; i < kGroup / kEach; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
 #pragma unroll
-    for (int i = 0; i < 32 / kEach; ++i) {
+    for (int i = 0; i < kGroup / kEach; ++i) {
       const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -295,7 +273,7 @@ __device__ __forceinline__ void add_bias(const void* bias, int64_t n0, int64_t n
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
+  for (int i = 0; i < kGroup; ++i)
     if (n0 + i < n) v[i] += to_float(p[i]);
 }
 
@@ -310,80 +288,78 @@ __device__ __forceinline__ float group_unscale(uint32_t e) {
   return __uint_as_float((e - 14u) << 23);
 }
 
-// 32 factors of one kind into their place (see TcFactors).
+// 16 factors of one kind into their place (see TcFactors).
 template <typename T>
-__device__ __forceinline__ void store_factors(const TcFactors& f, int64_t place, const float (&v)[32]) {
-  uint32_t w[32];
+__device__ __forceinline__ void store_factors(const TcFactors& f, int64_t place, const float (&v)[kGroup]) {
+  uint32_t w[16];
   if (sizeof(T) == 2) {
     float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(v[i]));
+    for (int i = 0; i < kGroup; ++i) top = fmaxf(top, fabsf(v[i]));
     uint32_t e;
     const float scale = group_scale(top, e);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const __half2 h = __floats2half2_rn(v[2 * i] * scale, v[2 * i + 1] * scale);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    __half* p = static_cast<__half*>(f.values) + place * kFactorGroup;
-    store32(p, w);
-    store32(p + 16, w + 8);
+    store32(static_cast<__half*>(f.values) + place * kFactorGroup, w);
     f.exponents[place] = static_cast<unsigned char>(e);
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
+    for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i]);
     float* p = static_cast<float*>(f.values) + place * kFactorGroup;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) store32(p + 8 * i, w + 8 * i);
+    store32(p, w);
+    store32(p + 8, w + 8);
   }
 }
-// The factors of one kind of a group of 32, as they lie in memory.
+// The factors of one kind of a group, as they lie in memory.
 template <typename T>
 struct FactorWords {
-  uint32_t w[8 * sizeof(T)];
+  uint32_t w[4 * sizeof(T)];
   uint32_t exponent;
 };
 template <typename T>
 __device__ __forceinline__ void load_factors(const TcFactors& f, int64_t place, FactorWords<T>& x) {
   const char* p = static_cast<const char*>(f.values) + place * (kFactorGroup * sizeof(T));
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) load32(p + 32 * i, x.w + 8 * i);
+  load32(p, x.w);
+  if (sizeof(T) == 4) load32(p + 32, x.w + 8);
   if (sizeof(T) == 2) x.exponent = f.exponents[place];
 }
 // out[i] = v[i] times factor i
 template <typename T>
-__device__ __forceinline__ void times_factors(const FactorWords<T>& x, const float (&v)[32], float (&out)[32]) {
+__device__ __forceinline__ void times_factors(const FactorWords<T>& x, const float (&v)[kGroup], float (&out)[kGroup]) {
   if constexpr (sizeof(T) == 2) {
     const float unscale = group_unscale(x.exponent);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x.w[i]));
       out[2 * i] = v[2 * i] * (f.x * unscale);
       out[2 * i + 1] = v[2 * i + 1] * (f.y * unscale);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) out[i] = v[i] * __uint_as_float(x.w[i]);
+    for (int i = 0; i < kGroup; ++i) out[i] = v[i] * __uint_as_float(x.w[i]);
   }
 }
 
-// Column sums over the warp's 32 rows (one row a lane): lane i gets column i's, by halving the
-// columns and doubling the rows five times, in a fixed order.
-__device__ __forceinline__ float sum_rows(const float (&v)[32], int lane) {
-  float s[16];
+// Column sums over the warp's 32 rows (one row a lane): lanes i and i + 16 get column i's, by
+// halving the columns and doubling the rows, in a fixed order.
+__device__ __forceinline__ float sum_rows(const float (&v)[kGroup], int lane) {
+  float s[8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float keep = lane & 16 ? v[i + 16] : v[i], give = lane & 16 ? v[i] : v[i + 16];
-    s[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+  for (int i = 0; i < 8; ++i) {
+    const float keep = lane & 8 ? v[i + 8] : v[i], give = lane & 8 ? v[i] : v[i + 8];
+    s[i] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
   }
 #pragma unroll
-  for (int half = 8; half >= 1; half /= 2)
+  for (int half = 4; half >= 1; half /= 2)
 #pragma unroll
     for (int i = 0; i < half; ++i) {
       const float keep = lane & half ? s[i + half] : s[i], give = lane & half ? s[i] : s[i + half];
       s[i] = keep + __shfl_xor_sync(0xffffffffu, give, half);
     }
-  return s[0];
+  return s[0] + __shfl_xor_sync(0xffffffffu, s[0], 16);
 }
 
 // One item of work: a tile of one group's result and one part of K.
@@ -602,8 +578,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else {
-    // ---- results: each warp has 32 rows; the two halves of the warps share the columns ----
-    const int quadrant = warp % 4, half = warp / 4, pairs = p.columns / 64;
+    // ---- results: each warp has 32 rows; four warps share the columns ----
+    const int quadrant = warp % 4, quarter = warp / 4, pairs = p.columns / 32;
     const uint32_t release = Cg == 2 ? in_cta(smem_u32(&sum_empty[0]), 0) : smem_u32(&sum_empty[0]);
     int64_t sums = 0;
     bool ok = true;
@@ -628,77 +604,76 @@ __global__ void __launch_bounds__(kThreads, 1)
         return ok;
       };
       const uint32_t lanes = static_cast<uint32_t>(quadrant * 32) << 16;
-      // 32 columns of the sums over K: FP32 blocks add both accumulators and their chunks
-      const auto add_columns = [&](uint32_t at, bool first, float (&v)[32]) {
+      // 16 columns of the sums over K: FP32 blocks add both accumulators and their chunks
+      const auto add_columns = [&](uint32_t at, bool first, float (&v)[kGroup]) {
         __syncwarp();
         if constexpr (kChunked) {
-          float more[32];
-          load_columns(at + kSmallColumns, more);
+          float more[kGroup];
+          tc::ld_x16(at + kSmallColumns, more);
           if (first) {
-            load_columns(at, v);
+            tc::ld_x16(at, v);
             tc::wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += more[i];
+            for (int i = 0; i < kGroup; ++i) v[i] += more[i];
           } else {
-            float large[32];
-            load_columns(at, large);
+            float large[kGroup];
+            tc::ld_x16(at, large);
             tc::wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += large[i] + more[i];
+            for (int i = 0; i < kGroup; ++i) v[i] += large[i] + more[i];
           }
         } else {
-          load_columns(at, v);
+          tc::ld_x16(at, v);
           tc::wait_ld();
         }
       };
 
       if constexpr (E == TcEpilogue::kGateGrad) {
-        // group by group of 32 columns; a group's factors are on their way while the sums (for
+        // group by group of 16 columns; a group's factors are on their way while the sums (for
         // the first) or the group before are worked on
         FactorWords<T> f1, f2;
         const auto prefetch = [&](int group) {
-          const int64_t n0 = it.n0 + 64 * (half + 2 * (group / 2)) + 32 * (group % 2);
+          const int64_t n0 = it.n0 + 32 * (quarter + 4 * (group / 2)) + 16 * (group % 2);
           if (row >= p.m || n0 >= p.n) return;
           const int64_t place = (row * p.factors.groups + n0 / kFactorGroup) * 2;
           load_factors<T>(p.factors, place, f1);
           load_factors<T>(p.factors, place + 1, f2);
         };
-        const auto finish = [&](int group, const float (&v)[32]) {
-          const int64_t n0 = it.n0 + 64 * (half + 2 * (group / 2)) + 32 * (group % 2);
+        const auto finish = [&](int group, const float (&v)[kGroup]) {
+          const int64_t n0 = it.n0 + 32 * (quarter + 4 * (group / 2)) + 16 * (group % 2);
           if (n0 >= p.n) return;
 #pragma unroll
           for (int which = 0; which < 2; ++which) {  // dg = dh f2, then du = dh f1
-            float d[32];
+            float d[kGroup];
             times_factors<T>(which == 0 ? f2 : f1, v, d);
             if (row < p.m)
               store_operand<T>(p.gated[which] + row * p.gated_stride + n0, p.gated_plane, d);
             if (p.row_sums == nullptr) continue;
             if (row >= p.m) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) d[i] = 0.0f;
+              for (int i = 0; i < kGroup; ++i) d[i] = 0.0f;
             }
             __syncwarp();
             const float sum = sum_rows(d, lane);
             const int64_t rows = it.m0 + rank * kRows + quadrant * 32;
-            if (rows < p.m) p.row_sums[(rows / 32 * 2 + which) * p.row_sums_stride + n0 + lane] = sum;
+            if (rows < p.m && lane < kGroup) p.row_sums[(rows / 32 * 2 + which) * p.row_sums_stride + n0 + lane] = sum;
           }
         };
-        const int groups = half < pairs ? 2 * ((pairs - half + 1) / 2) : 0;
-        if (!kChunked && groups > 0) prefetch(0);  // FP32 has no registers for it
+        const int groups = quarter < pairs ? 2 * ((pairs - quarter + 3) / 4) : 0;
+        if (groups > 0) prefetch(0);
         if constexpr (kChunked) {
-          float v0[32], v1[32];  // at most 128 columns: two groups a warp
+          float v0[kGroup], v1[kGroup];  // at most 128 columns: two groups a warp
           for (int c = 0; c < chunks; ++c, ++sums) {
             const int buffer = static_cast<int>(sums & 1);
             if (!wait_sums(buffer)) break;
             if (groups > 0) {
-              const uint32_t from = tmem + buffer * kMaxColumns + lanes + 64 * half;
+              const uint32_t from = tmem + buffer * kMaxColumns + lanes + 32 * quarter;
               add_columns(from, c == 0, v0);
-              add_columns(from + 32, c == 0, v1);
+              add_columns(from + 16, c == 0, v1);
             }
             release_sums(buffer);
           }
           if (ok && groups > 0) {
-            prefetch(0);
             finish(0, v0);
             prefetch(1);
             finish(1, v1);
@@ -709,8 +684,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++sums;
           const uint32_t from = tmem + buffer * kMaxColumns + lanes;
           for (int group = 0; group < groups; ++group) {
-            float v[32];
-            add_columns(from + 64 * (half + 2 * (group / 2)) + 32 * (group % 2), true, v);
+            float v[kGroup];
+            add_columns(from + 32 * (quarter + 4 * (group / 2)) + 16 * (group % 2), true, v);
             if (group + 1 == groups) release_sums(buffer);
             finish(group, v);
             if (group + 1 < groups) prefetch(group + 1);
@@ -718,18 +693,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (groups == 0) release_sums(buffer);
         }
       } else {
-        // two groups of 32 columns at a time: a gate tile's g and u, else neighbours
-        const auto finish = [&](int pair, float (&v0)[32], float (&v1)[32]) {
+        // two groups of 16 columns at a time: a gate tile's g and u, else neighbours
+        const auto finish = [&](int pair, float (&v0)[kGroup], float (&v1)[kGroup]) {
           if (row >= p.m) return;
           if constexpr (kGateTile) {
-            const int64_t n0 = it.n0 + 32 * pair;
+            const int64_t n0 = it.n0 + 16 * pair;
             if (n0 >= p.n) return;
             add_bias<T>(p.bias[0], n0, p.n, v0);
             add_bias<T>(p.bias[1], n0, p.n, v1);
-            float h[32];
+            float h[kGroup];
             const auto gate = [&](auto tanh) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
+              for (int i = 0; i < kGroup; ++i) {
                 float a, slope;
                 block_activation<decltype(tanh)::value>(v0[i], a, slope);
                 h[i] = a * v1[i];
@@ -748,8 +723,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              float(&v)[32] = j == 0 ? v0 : v1;
-              const int64_t n0 = it.n0 + 64 * pair + 32 * j;
+              float(&v)[kGroup] = j == 0 ? v0 : v1;
+              const int64_t n0 = it.n0 + 32 * pair + 16 * j;
               if (n0 >= p.n) break;
               if constexpr (E == TcEpilogue::kPartial) {
                 float* out = p.partial + ((static_cast<int64_t>(it.group) * p.parts + it.part) * p.m + row) * p.partial_stride;
@@ -761,22 +736,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         };
-        float acc0[32], acc1[32];
+        float acc0[kGroup], acc1[kGroup];
         for (int c = 0; c < chunks; ++c, ++sums) {
           const int buffer = static_cast<int>(sums & 1);
           if (!wait_sums(buffer)) break;
           const uint32_t from = tmem + buffer * kMaxColumns + lanes;
           // FP32 blocks have at most 128 columns: a pair a warp, kept over the chunks
-          for (int pair = half; pair < pairs; pair += 2) {
-            const uint32_t c0 = from + (kGateTile ? 32 * pair : 64 * pair);
-            const uint32_t c1 = kGateTile ? from + p.columns / 2 + 32 * pair : c0 + 32;
+          for (int pair = quarter; pair < pairs; pair += 4) {
+            const uint32_t c0 = from + (kGateTile ? 16 * pair : 32 * pair);
+            const uint32_t c1 = kGateTile ? from + p.columns / 2 + 16 * pair : c0 + 16;
             add_columns(c0, !kChunked || c == 0, acc0);
             add_columns(c1, !kChunked || c == 0, acc1);
-            if (pair + 2 >= pairs) release_sums(buffer);
+            if (pair + 4 >= pairs) release_sums(buffer);
             if (!kChunked || c + 1 == chunks) finish(pair, acc0, acc1);
           }
-          // a tile of 64 columns leaves the second half of the warps idle
-          if (half >= pairs) release_sums(buffer);
+          // a tile of 64 columns leaves half of the warps idle
+          if (quarter >= pairs) release_sums(buffer);
         }
       }
     }
@@ -787,23 +762,34 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kEpilogueWarps) free_tmem<Cg>(tmem);
 }
 
-// out[m][n] = the sum of the parts in order + bias[n].
+// out[m][n] = the sum of the parts in order + bias[n]; one group of the product per blockIdx.y.
+template <typename T>
+struct Outputs {
+  T* group[2];
+};
 template <typename T>
 __global__ void __launch_bounds__(256)
     add_parts_kernel(const float* __restrict__ partial, int64_t part_values, int64_t stride, int parts,
-                     int64_t m, int64_t n, const T* __restrict__ bias, T* __restrict__ out,
+                     int64_t m, int64_t n, const T* __restrict__ bias, Outputs<T> outputs,
                      int64_t out_stride) {
-  const int64_t quads = stride / 4;
+  const int64_t quads = stride / 4, step = part_values / 4;
+  T* const out = outputs.group[blockIdx.y];
+  partial += blockIdx.y * parts * part_values;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < m * quads; i += gridDim.x * 256ll) {
-    const int64_t row = i / quads, c = (i % quads) * 4;
+    const int64_t row = i / quads, c = (i - row * quads) * 4;
     const float4* src = reinterpret_cast<const float4*>(partial + row * stride + c);
     float4 s = src[0];
-    for (int k = 1; k < parts; ++k) {
-      const float4 v = src[k * (part_values / 4)];
-      s.x += v.x;
-      s.y += v.y;
-      s.z += v.z;
-      s.w += v.w;
+    int k = 1;
+    for (; k + 4 <= parts; k += 4) {  // four parts in flight
+      float4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = src[(k + j) * step];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s = make_float4(s.x + v[j].x, s.y + v[j].y, s.z + v[j].z, s.w + v[j].w);
+    }
+    for (; k < parts; ++k) {
+      const float4 v = src[k * step];
+      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
     }
     const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
@@ -991,15 +977,11 @@ template <typename T>
 cudaError_t add_parts(const TcProduct& p, const Plan& plan, const float* partial, const DeviceInfo& dev,
                       cudaStream_t stream) {
   const int64_t values = p.m * plan.partial_stride;
-  const int64_t blocks = std::min<int64_t>(blocks_of(values / 4, 256), 8ll * dev.sms);
-  for (int g = 0; g < p.groups; ++g) {
-    add_parts_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
-        partial + g * plan.parts * values, values, plan.partial_stride, plan.parts, p.m, p.n,
-        static_cast<const T*>(p.bias[0]), static_cast<T*>(p.out[g]), p.out_stride);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-  }
-  return cudaSuccess;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks_of(values / 4, 256), 8ll * dev.sms)), p.groups);
+  add_parts_kernel<T><<<grid, 256, 0, stream>>>(
+      partial, values, plan.partial_stride, plan.parts, p.m, p.n, static_cast<const T*>(p.bias[0]),
+      Outputs<T>{{static_cast<T*>(p.out[0]), static_cast<T*>(p.out[1])}}, p.out_stride);
+  return cudaGetLastError();
 }
 
 }  // namespace

@@ -27,14 +27,14 @@ enum class TcEpilogue {
   kGateGrad,  // the gradients of g and u from that of h
 };
 
-// What the forward keeps of the activation for the backward, for 32 consecutive hidden features
+// What the forward keeps of the activation for the backward, for 16 consecutive hidden features
 // of one token: f1 = act(g) and f2 = u act'(g), so that du = dh f1 and dg = dh f2.
-// bf16 block: f16 values times one power of 2 for each of the two groups of 32 (an exponent
+// bf16 block: f16 values times one power of 2 for each of the two groups of 16 (an exponent
 // byte each), so the range is FP32's and the rounding 2^-12 of the group's largest value --
 // 16 times below the bf16 rounding of dg and du that follows. FP32 block: FP32 values.
-constexpr int kFactorGroup = 32;
+constexpr int kFactorGroup = 16;
 struct TcFactors {
-  void* values = nullptr;          // [token][group][2][32], __half or float
+  void* values = nullptr;          // [token][group][2][16], __half or float
   unsigned char* exponents = nullptr;  // [token][group][2]
   int64_t groups = 0;
 };
