@@ -1,6 +1,8 @@
 // Torch binding of the gated residual trunk's operators (include/fused_hoad_b200.h): part of
 // the module fused_hoad._C. Outputs, workspaces and what the backward keeps come from the ATen
 // caching allocator on the current stream, so the ops stay asynchronous and graph-capturable.
+// Gradients are autograd nodes in C++: autograd's threads need no Python for them (a node in
+// Python costs about 70 us a backward pass).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime.h>
@@ -78,6 +80,27 @@ torch::Tensor bytes_for(size_t bytes, const torch::Tensor& like) {
 void* data_of(const torch::Tensor& t) { return t.numel() ? t.data_ptr() : nullptr; }
 void* data_of(const OptionalTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+OptionalTensor given(const torch::Tensor& t) {
+  return t.defined() ? OptionalTensor(t) : OptionalTensor();
+}
+torch::Tensor or_undefined(const OptionalTensor& t) { return t ? *t : torch::Tensor(); }
+
+bool records_gradients(const variable_list& tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const torch::Tensor& t : tensors)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+// The backwards are not differentiable themselves. Recording a graph of one (create_graph) would
+// cut it off there, and gradients of gradients would silently lack a part: it raises instead.
+void check_differentiated_once(const char* op) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), op,
+              " is differentiable once: its backward does not support create_graph");
+}
+
 // ---- gated feed-forward block ----
 
 // The problem, and the row views that its pointers belong to.
@@ -134,63 +157,70 @@ Ffn ffn_of(const torch::Tensor& x, const torch::Tensor& w_gate, const torch::Ten
   return f;
 }
 
-// (y [..., out_width], what the backward needs or an empty tensor)
-std::tuple<torch::Tensor, torch::Tensor> gated_feed_forward(
-    torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up, torch::Tensor w_down,
-    OptionalTensor b_gate, OptionalTensor b_up, OptionalTensor b_down,
-    const std::string& activation, bool want_saved) {
-  const Ffn f = ffn_of(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation);
+// y [..., out_width]; `saved`, where given, becomes what the backward needs.
+torch::Tensor ffn_forward(const Ffn& f, const torch::Tensor& x, torch::Tensor* saved) {
   const c10::cuda::CUDAGuard device_guard(x.device());
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = f.problem.out_width;
   auto y = torch::empty(shape, x.options());
-  auto saved = bytes_for(want_saved ? fhb_ffn_saved_bytes(&f.problem) : 0, x);
-  if (f.problem.tokens == 0) return {y, saved};
+  if (saved != nullptr) *saved = bytes_for(fhb_ffn_saved_bytes(&f.problem), x);
+  if (f.problem.tokens == 0) return y;
   auto workspace = bytes_for(fhb_ffn_workspace_bytes(&f.problem, 0), x);
-  check_status(fhb_ffn_forward(&f.problem, y.data_ptr(), want_saved ? saved.data_ptr() : nullptr,
-                               data_of(workspace), static_cast<size_t>(workspace.numel()),
+  check_status(fhb_ffn_forward(&f.problem, y.data_ptr(),
+                               saved != nullptr ? saved->data_ptr() : nullptr, data_of(workspace),
+                               static_cast<size_t>(workspace.numel()),
                                at::cuda::getCurrentCUDAStream()),
                "gated_feed_forward");
-  return {y, saved};
+  return y;
 }
 
-// Gradients of x, w_gate, w_up, w_down, b_gate, b_up, b_down, in that order; an undefined
-// tensor (None) where wants[i] is false.
-std::vector<OptionalTensor> gated_feed_forward_backward(
-    torch::Tensor grad_y, torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up,
-    torch::Tensor w_down, OptionalTensor b_gate, OptionalTensor b_up, OptionalTensor b_down,
-    const std::string& activation, torch::Tensor saved, std::vector<bool> wants) {
-  const Ffn f = ffn_of(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation);
-  const fhb_ffn_problem& p = f.problem;
-  TORCH_CHECK(wants.size() == 7, "wants must have 7 entries");
-  check_like(grad_y, x, "grad_y", "x");
-  TORCH_CHECK(grad_y.dim() >= 1 && grad_y.size(-1) == p.out_width &&
-                  grad_y.numel() == p.tokens * p.out_width,
-              "grad_y must have shape [..., ", text(p.out_width), "]");
-  const c10::cuda::CUDAGuard device_guard(x.device());
-  TORCH_CHECK(saved.is_cuda() && saved.is_contiguous() && saved.scalar_type() == torch::kUInt8 &&
-                  static_cast<size_t>(saved.numel()) >= fhb_ffn_saved_bytes(&p),
-              "saved must be what gated_feed_forward returned for these arguments");
-  const torch::Tensor dy = as_rows(grad_y);
-  const auto like = [&](bool want, at::IntArrayRef shape) -> OptionalTensor {
-    if (!want) return c10::nullopt;
-    return torch::empty(shape, x.options());
-  };
-  std::vector<OptionalTensor> out{like(wants[0], x.sizes()),
-                                  like(wants[1], w_gate.sizes()),
-                                  like(wants[2], w_up.sizes()),
-                                  like(wants[3], w_down.sizes()),
-                                  like(wants[4] && b_gate, {p.hidden}),
-                                  like(wants[5] && b_up, {p.hidden}),
-                                  like(wants[6] && b_down, {p.out_width})};
-  const fhb_ffn_grads grads{data_of(out[0]), data_of(out[1]), data_of(out[2]), data_of(out[3]),
-                            data_of(out[4]), data_of(out[5]), data_of(out[6])};
-  auto workspace = bytes_for(fhb_ffn_workspace_bytes(&p, 1), x);
-  check_status(fhb_ffn_backward(&p, data_of(dy), row_stride(dy), data_of(saved), &grads,
-                                data_of(workspace), static_cast<size_t>(workspace.numel()),
-                                at::cuda::getCurrentCUDAStream()),
-               "gated_feed_forward_backward");
-  return out;
+class FfnNode : public torch::autograd::Function<FfnNode> {
+ public:
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& x,
+                               const torch::Tensor& w_gate, const torch::Tensor& w_up,
+                               const torch::Tensor& w_down, const OptionalTensor& b_gate,
+                               const OptionalTensor& b_up, const OptionalTensor& b_down,
+                               const std::string& activation) {
+    const Ffn f = ffn_of(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation);
+    torch::Tensor saved;
+    auto y = ffn_forward(f, x, &saved);
+    ctx->saved_data["activation"] = activation;
+    ctx->save_for_backward({saved, x, w_gate, w_up, w_down, or_undefined(b_gate), or_undefined(b_up),
+                            or_undefined(b_down)});
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list upstream) {
+    check_differentiated_once("gated_feed_forward");
+    const variable_list t = ctx->get_saved_variables();
+    const torch::Tensor &saved = t[0], &x = t[1], &grad_y = upstream[0];
+    const Ffn f = ffn_of(x, t[2], t[3], t[4], given(t[5]), given(t[6]), given(t[7]),
+                         ctx->saved_data["activation"].toStringRef());
+    const fhb_ffn_problem& p = f.problem;
+    check_like(grad_y, x, "grad_y", "x");
+    variable_list out(8);
+    const c10::cuda::CUDAGuard device_guard(x.device());
+    const torch::Tensor dy = as_rows(grad_y);
+    for (int i = 0, edge = 0; i < 7; ++i)  // only tensors that were given have an edge
+      if (t[i + 1].defined() && ctx->needs_input_grad(edge++)) out[i] = torch::empty(t[i + 1].sizes(), x.options());
+    const auto place = [&](int i) { return out[i].defined() ? data_of(out[i]) : nullptr; };
+    const fhb_ffn_grads grads{place(0), place(1), place(2), place(3), place(4), place(5), place(6)};
+    auto workspace = bytes_for(fhb_ffn_workspace_bytes(&p, 1), x);
+    check_status(fhb_ffn_backward(&p, data_of(dy), row_stride(dy), data_of(saved), &grads,
+                                  data_of(workspace), static_cast<size_t>(workspace.numel()),
+                                  at::cuda::getCurrentCUDAStream()),
+                 "gated_feed_forward's backward");
+    return out;
+  }
+};
+
+torch::Tensor gated_feed_forward(torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up,
+                                 torch::Tensor w_down, OptionalTensor b_gate, OptionalTensor b_up,
+                                 OptionalTensor b_down, const std::string& activation) {
+  if (records_gradients({x, w_gate, w_up, w_down, or_undefined(b_gate), or_undefined(b_up),
+                         or_undefined(b_down)}))
+    return FfnNode::apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation);
+  return ffn_forward(ffn_of(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation), x, nullptr);
 }
 
 // ---- norms with gate and residual scale ----
@@ -272,74 +302,90 @@ Norm norm_of(const torch::Tensor& residual, const OptionalTensor& branch,
   return n;
 }
 
-// (total or an empty tensor, normed, stats or an empty tensor)
-std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> residual_norm(
-    torch::Tensor residual, OptionalTensor branch, torch::Tensor pre_weight,
-    OptionalTensor post_weight, OptionalTensor gate, OptionalTensor scale_tensor, double scale,
-    double eps, bool want_total, bool want_stats) {
-  const Norm n = norm_of(residual, branch, pre_weight, post_weight, gate, scale_tensor, scale, eps);
+// (total or an undefined tensor, normed); `stats`, where given, becomes what the backward needs.
+std::pair<torch::Tensor, torch::Tensor> norm_forward(const Norm& n, const torch::Tensor& residual,
+                                                     const torch::Tensor& pre_weight,
+                                                     bool want_total, torch::Tensor* stats) {
   const c10::cuda::CUDAGuard device_guard(residual.device());
-  auto total = want_total ? torch::empty(residual.sizes(), residual.options())
-                          : torch::empty({0}, residual.options());
+  torch::Tensor total;
+  if (want_total) total = torch::empty(residual.sizes(), residual.options());
   auto normed = torch::empty(residual.sizes(), pre_weight.options());
-  auto stats = torch::empty({want_stats ? 2 * n.problem.rows : 0},
-                            residual.options().dtype(torch::kFloat32));
-  check_status(fhb_residual_norm(&n.problem, data_of(total), data_of(normed),
-                                 static_cast<float*>(data_of(stats)),
+  if (stats != nullptr)
+    *stats = torch::empty({2 * n.problem.rows}, residual.options().dtype(torch::kFloat32));
+  check_status(fhb_residual_norm(&n.problem, want_total ? data_of(total) : nullptr, data_of(normed),
+                                 stats != nullptr ? static_cast<float*>(data_of(*stats)) : nullptr,
                                  at::cuda::getCurrentCUDAStream()),
                "residual_norm");
-  return {total, normed, stats};
+  return {total, normed};
 }
 
-// Gradients of residual, branch, pre_weight, post_weight, gate, residual_scale; None where
-// wants[i] is false.
-std::vector<OptionalTensor> residual_norm_backward(
-    OptionalTensor grad_total, OptionalTensor grad_normed, torch::Tensor residual,
-    OptionalTensor branch, torch::Tensor pre_weight, OptionalTensor post_weight,
-    OptionalTensor gate, OptionalTensor scale_tensor, double scale, double eps,
-    torch::Tensor stats, std::vector<bool> wants) {
+// Without a branch it is the norm alone, and there is no total.
+class NormNode : public torch::autograd::Function<NormNode> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& residual,
+                               const OptionalTensor& branch, const torch::Tensor& pre_weight,
+                               const OptionalTensor& post_weight, const OptionalTensor& gate,
+                               const OptionalTensor& scale_tensor, double scale, double eps) {
+    const Norm n = norm_of(residual, branch, pre_weight, post_weight, gate, scale_tensor, scale, eps);
+    torch::Tensor stats;
+    auto [total, normed] = norm_forward(n, residual, pre_weight, branch.has_value(), &stats);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["eps"] = eps;
+    ctx->save_for_backward({stats, residual, or_undefined(branch), pre_weight, or_undefined(post_weight),
+                            or_undefined(gate), or_undefined(scale_tensor)});
+    ctx->set_materialize_grads(false);
+    if (branch) return {total, normed};
+    return {normed};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list upstream) {
+    check_differentiated_once("residual_norm");
+    const variable_list t = ctx->get_saved_variables();
+    const torch::Tensor &stats = t[0], &residual = t[1], &branch = t[2], &pre_weight = t[3];
+    const Norm n = norm_of(residual, given(branch), pre_weight, given(t[4]), given(t[5]), given(t[6]),
+                           ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble());
+    const fhb_norm_problem& p = n.problem;
+    const torch::Tensor grad_total = branch.defined() ? upstream[0] : torch::Tensor();
+    const torch::Tensor grad_normed = upstream.back();
+    variable_list out(8);
+    const c10::cuda::CUDAGuard device_guard(residual.device());
+    torch::Tensor dt, dn;
+    if (grad_total.defined()) {
+      check_like(grad_total, residual, "grad_total", "residual");
+      dt = as_rows(grad_total);
+    }
+    if (grad_normed.defined()) {
+      check_like(grad_normed, pre_weight, "grad_normed", "pre_weight");
+      dn = as_rows(grad_normed);
+    }
+    for (int i = 0, edge = 0; i < 6; ++i)
+      if (t[i + 1].defined() && ctx->needs_input_grad(edge++)) out[i] = torch::empty(t[i + 1].sizes(), t[i + 1].options());
+    const auto place = [&](int i) { return out[i].defined() ? data_of(out[i]) : nullptr; };
+    const fhb_norm_grads grads{place(0), place(1), place(2), place(3), place(4),
+                               static_cast<float*>(place(5))};
+    auto workspace = bytes_for(fhb_residual_norm_workspace_bytes(&p), residual);
+    check_status(
+        fhb_residual_norm_backward(
+            &p, dt.defined() ? data_of(dt) : nullptr, dt.defined() ? row_stride(dt) : 0,
+            dn.defined() ? data_of(dn) : nullptr, dn.defined() ? row_stride(dn) : 0,
+            static_cast<const float*>(data_of(stats)), &grads, data_of(workspace),
+            static_cast<size_t>(workspace.numel()), at::cuda::getCurrentCUDAStream()),
+        "residual_norm's backward");
+    return out;
+  }
+};
+
+// (total, normed), or (normed,) without a branch
+variable_list residual_norm(torch::Tensor residual, OptionalTensor branch, torch::Tensor pre_weight,
+                            OptionalTensor post_weight, OptionalTensor gate,
+                            OptionalTensor scale_tensor, double scale, double eps) {
+  if (records_gradients({residual, or_undefined(branch), pre_weight, or_undefined(post_weight),
+                         or_undefined(gate), or_undefined(scale_tensor)}))
+    return NormNode::apply(residual, branch, pre_weight, post_weight, gate, scale_tensor, scale, eps);
   const Norm n = norm_of(residual, branch, pre_weight, post_weight, gate, scale_tensor, scale, eps);
-  const fhb_norm_problem& p = n.problem;
-  TORCH_CHECK(wants.size() == 6, "wants must have 6 entries");
-  TORCH_CHECK(stats.is_cuda() && stats.is_contiguous() &&
-                  stats.scalar_type() == torch::kFloat32 && stats.numel() == 2 * p.rows,
-              "stats must be what residual_norm returned for these arguments");
-  const c10::cuda::CUDAGuard device_guard(residual.device());
-  torch::Tensor dt, dn;
-  if (grad_total) {
-    check_like(*grad_total, residual, "grad_total", "residual");
-    TORCH_CHECK(grad_total->numel() == residual.numel() && grad_total->size(-1) == p.width,
-                "grad_total must have the shape of residual");
-    dt = as_rows(*grad_total);
-  }
-  if (grad_normed) {
-    check_like(*grad_normed, pre_weight, "grad_normed", "pre_weight");
-    TORCH_CHECK(grad_normed->numel() == residual.numel() && grad_normed->size(-1) == p.width,
-                "grad_normed must have the shape of residual");
-    dn = as_rows(*grad_normed);
-  }
-  const auto like = [](bool want, const torch::Tensor& t) -> OptionalTensor {
-    if (!want) return c10::nullopt;
-    return torch::empty(t.sizes(), t.options());
-  };
-  std::vector<OptionalTensor> out{
-      like(wants[0], residual),
-      like(wants[1] && branch, branch ? *branch : residual),
-      like(wants[2], pre_weight),
-      like(wants[3] && post_weight, post_weight ? *post_weight : residual),
-      like(wants[4] && gate, gate ? *gate : residual),
-      like(wants[5] && scale_tensor, scale_tensor ? *scale_tensor : residual)};
-  const fhb_norm_grads grads{data_of(out[0]), data_of(out[1]), data_of(out[2]), data_of(out[3]),
-                             data_of(out[4]), static_cast<float*>(data_of(out[5]))};
-  auto workspace = bytes_for(fhb_residual_norm_workspace_bytes(&p), residual);
-  check_status(
-      fhb_residual_norm_backward(
-          &p, grad_total ? data_of(dt) : nullptr, grad_total ? row_stride(dt) : 0,
-          grad_normed ? data_of(dn) : nullptr, grad_normed ? row_stride(dn) : 0,
-          static_cast<const float*>(data_of(stats)), &grads, data_of(workspace),
-          static_cast<size_t>(workspace.numel()), at::cuda::getCurrentCUDAStream()),
-      "residual_norm_backward");
-  return out;
+  auto [total, normed] = norm_forward(n, residual, pre_weight, branch.has_value(), nullptr);
+  if (branch) return {total, normed};
+  return {normed};
 }
 
 // ---- AdamW over many tensors ----
@@ -407,23 +453,15 @@ void adamw_step(const std::vector<torch::Tensor>& params, const std::vector<torc
 void bind_blocks(pybind11::module& module) {
   using pybind11::arg;
   module.def("gated_feed_forward", &gated_feed_forward,
-             "Gated feed-forward block (CUDA, sm_100a): (y, saved)", arg("x"), arg("w_gate"),
-             arg("w_up"), arg("w_down"), arg("b_gate") = pybind11::none(),
+             "Gated feed-forward block (CUDA, sm_100a), differentiable once", arg("x"),
+             arg("w_gate"), arg("w_up"), arg("w_down"), arg("b_gate") = pybind11::none(),
              arg("b_up") = pybind11::none(), arg("b_down") = pybind11::none(),
-             arg("activation") = "silu", arg("want_saved") = false);
-  module.def("gated_feed_forward_backward", &gated_feed_forward_backward,
-             "Gradients of the gated feed-forward block (CUDA, sm_100a)", arg("grad_y"), arg("x"),
-             arg("w_gate"), arg("w_up"), arg("w_down"), arg("b_gate"), arg("b_up"), arg("b_down"),
-             arg("activation"), arg("saved"), arg("wants"));
+             arg("activation") = "silu");
   module.def("residual_norm", &residual_norm,
              "RMS norms before and after a block with its gate and residual scale (CUDA, "
-             "sm_100a): (total, normed, stats)",
+             "sm_100a), differentiable once: (total, normed), or (normed,) without a branch",
              arg("residual"), arg("branch"), arg("pre_weight"), arg("post_weight"), arg("gate"),
-             arg("scale_tensor"), arg("scale"), arg("eps"), arg("want_total"), arg("want_stats"));
-  module.def("residual_norm_backward", &residual_norm_backward,
-             "Gradients of residual_norm (CUDA, sm_100a)", arg("grad_total"), arg("grad_normed"),
-             arg("residual"), arg("branch"), arg("pre_weight"), arg("post_weight"), arg("gate"),
-             arg("scale_tensor"), arg("scale"), arg("eps"), arg("stats"), arg("wants"));
+             arg("scale_tensor"), arg("scale"), arg("eps"));
   module.def("adamw_step", &adamw_step, "AdamW over many tensors, 32- or 8-bit states",
              arg("params"), arg("grads"), arg("exp_avgs"), arg("exp_avg_sqs"),
              arg("exp_avg_scales"), arg("exp_avg_sq_scales"), arg("step"), arg("lr"),

@@ -878,10 +878,10 @@ Plan plan_of(const TcProduct& p, const DeviceInfo& dev) {
       const int64_t units = dev.sms / cg;
       const double mma = 2.0 * columns * (wide ? 6 : 1);
       const double block = p.sum_terms * std::max(mma, block_bytes_of(wide, cg, columns) / 64.0);
-      // parts that fill one, two, three or four rounds of the SMs
-      for (int rounds = 0; rounds <= (p.epilogue == TcEpilogue::kStore ? 4 : 0); ++rounds) {
-        const int64_t wanted = rounds == 0 ? 1 : units * rounds / tiles;
-        if (rounds > 0 && (wanted < 2 || wanted > 128)) continue;
+      // one to four parts, or as many as fill one or two rounds of the SMs
+      for (int choice = 1; choice <= (p.epilogue == TcEpilogue::kStore ? 6 : 1); ++choice) {
+        const int64_t wanted = choice <= 4 ? choice : std::min<int64_t>(units * (choice - 4) / tiles, 128);
+        if (choice > 4 && wanted <= 4) continue;
         const int part_blocks = static_cast<int>(blocks_of(k_blocks, wanted));
         const int parts = static_cast<int>(blocks_of(k_blocks, part_blocks));
         double cycles = static_cast<double>(blocks_of(tiles * parts, units)) * (2000.0 + part_blocks * block);

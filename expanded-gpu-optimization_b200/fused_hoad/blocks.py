@@ -16,27 +16,6 @@ from fused_hoad._extension import load_extension
 from fused_hoad.problem import ACTIVATIONS
 
 
-class _GatedFeedForward(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, activation, *tensors):
-        y, saved = load_extension().gated_feed_forward(*tensors, activation, True)
-        ctx.activation = activation
-        ctx.save_for_backward(saved, *tensors)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_y):
-        saved, *tensors = ctx.saved_tensors
-        wants = list(ctx.needs_input_grad[1:])
-        if not any(wants):
-            return (None,) * 8
-        grads = load_extension().gated_feed_forward_backward(
-            grad_y, *tensors, ctx.activation, saved, wants
-        )
-        return (None, *grads)
-
-
 def gated_feed_forward(
     x: Tensor,
     w_gate: Tensor,
@@ -53,46 +32,20 @@ def gated_feed_forward(
     ``[out, hidden]``, all float32 or all bfloat16; ``activation`` ``"silu"`` or ``"tanh"``.
     Rows may have any stride (a slice of a larger tensor is not copied). Sums are held in 32
     bits. In bfloat16 the gated product, and in the backward the gradients of the two
-    projections, are rounded to bfloat16 as operands of the next matrix product.
+    projections, are rounded to bfloat16 as operands of the next matrix product. Differentiable
+    once (``create_graph`` raises).
     """
-    tensors = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return _GatedFeedForward.apply(activation, *tensors)
-    return load_extension().gated_feed_forward(*tensors, activation, False)[0]
+    return load_extension().gated_feed_forward(
+        x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation
+    )
 
 
-class _ResidualNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, scale, eps, want_total, *tensors):
-        total, normed, stats = load_extension().residual_norm(
-            *tensors, scale, eps, want_total, True
-        )
-        ctx.scale, ctx.eps, ctx.want_total = scale, eps, want_total
-        ctx.save_for_backward(stats, *tensors)
-        ctx.set_materialize_grads(False)
-        return total, normed
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_total, grad_normed):
-        stats, *tensors = ctx.saved_tensors
-        wants = list(ctx.needs_input_grad[3:])
-        if not any(wants):
-            return (None,) * 9
-        grads = load_extension().residual_norm_backward(
-            grad_total if ctx.want_total else None, grad_normed, *tensors, ctx.scale, ctx.eps,
-            stats, wants
-        )
-        return (None, None, None, *grads)
-
-
-def _norm(residual, branch, pre_weight, post_weight, gate, residual_scale, eps, want_total):
-    scale_tensor = residual_scale if isinstance(residual_scale, Tensor) else None
-    scale = 1.0 if scale_tensor is not None else float(residual_scale)
-    tensors = (residual, branch, pre_weight, post_weight, gate, scale_tensor)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return _ResidualNorm.apply(scale, eps, want_total, *tensors)
-    return load_extension().residual_norm(*tensors, scale, eps, want_total, False)[:2]
+def _norm(residual, branch, pre_weight, post_weight, gate, residual_scale, eps):
+    tensor = isinstance(residual_scale, Tensor)
+    return load_extension().residual_norm(
+        residual, branch, pre_weight, post_weight, gate, residual_scale if tensor else None,
+        1.0 if tensor else float(residual_scale), eps
+    )
 
 
 def residual_norm(
@@ -116,16 +69,17 @@ def residual_norm(
     (``[batch, 1, width]``: a gate for each sample). ``residual_scale`` is a number or a float32
     tensor with one element, which then gets a gradient. ``residual`` and ``total`` may be
     float32 where everything else is bfloat16. Sums and norms are held in 32 bits, and the
-    norm is that of the unrounded total.
+    norm is that of the unrounded total. Differentiable once.
     """
     if branch is None:
         raise ValueError("residual_norm needs a branch; rms_norm is the norm alone")
-    return _norm(residual, branch, pre_weight, post_weight, gate, residual_scale, eps, True)
+    total, normed = _norm(residual, branch, pre_weight, post_weight, gate, residual_scale, eps)
+    return total, normed
 
 
 def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6) -> Tensor:
     """``x / sqrt(mean(x^2) + eps) * weight`` over the last dimension, in the weight's type."""
-    return _norm(x, None, weight, None, None, 1.0, eps, False)[1]
+    return _norm(x, None, weight, None, None, 1.0, eps)[0]
 
 
 class GatedResidualTrunk(nn.Module):

@@ -197,3 +197,32 @@ def test_messages_with_numbers():
     step = torch.zeros(1, dtype=torch.int64, device="cuda")
     with pytest.raises(RuntimeError, match="grad must have 8 values"):
         fused_hoad.load_extension().adam_step(p, p[:4], p, p, step, 1e-3, 0.9, 0.999, 1e-8)
+
+
+@pytest.mark.gpu
+def test_differentiable_once():
+    """Recording a graph of a backward is refused: it would be cut off there."""
+    x, w, d = (torch.randn(s, device="cuda", requires_grad=True) for s in ((3, 8), (16, 8), (8, 16)))
+    y = fused_hoad.gated_feed_forward(x, w, w, d)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(y.sum(), x, create_graph=True, retain_graph=True)
+    (gradient,) = torch.autograd.grad(y.sum(), x)
+    assert not gradient.requires_grad
+    scale = torch.ones(8, device="cuda", requires_grad=True)
+    total, normed = fused_hoad.residual_norm(x, x, scale)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad((total.sum() + normed.square().sum()), scale, create_graph=True)
+
+
+@pytest.mark.gpu
+def test_inputs_used_twice_and_saved_inputs_changed():
+    x, w, d = (torch.randn(s, device="cuda", requires_grad=True) for s in ((5, 8), (16, 8), (8, 16)))
+    (twice,) = torch.autograd.grad(fused_hoad.gated_feed_forward(x, w, w, d).sum(), [w])
+    v = w.detach().clone().requires_grad_()
+    parts = torch.autograd.grad(fused_hoad.gated_feed_forward(x, w, v, d).sum(), [w, v])
+    assert torch.allclose(twice, parts[0] + parts[1], rtol=1e-6, atol=1e-6)
+    y = fused_hoad.gated_feed_forward(x, w, w, d)
+    with torch.no_grad():
+        w.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
