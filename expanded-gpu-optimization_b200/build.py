@@ -42,7 +42,7 @@ NVCC_FLAGS = [
 CU_SOURCES = [
     "forward_fp32.cu", "forward_tc.cu", "backward_fp32.cu", "backward_tc.cu", "adam.cu",
     "collective.cu", "capi.cu", "noalloc.cu", "biharmonic.cu",
-    "gated_ffn.cu", "gemm_tc.cu", "residual_norm.cu", "adamw.cu", "capi_blocks.cu",
+    "gated_ffn.cu", "gated_ffn_small.cu", "gemm_tc.cu", "residual_norm.cu", "adamw.cu", "capi_blocks.cu",
 ]
 BINDING_SOURCES = ["bindings.cpp", "bindings_blocks.cpp"]
 

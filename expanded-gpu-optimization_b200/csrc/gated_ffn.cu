@@ -8,6 +8,8 @@
 // on the tensor cores (gemm_tc.cu).
 #include <algorithm>
 
+#include "common.cuh"
+#include "gated_ffn.cuh"
 #include "gemm_tc.cuh"
 
 namespace fhb {
@@ -78,6 +80,8 @@ __device__ __forceinline__ void add_rows(const S* p, int64_t stride, int64_t fir
 
 template <typename T>
 __global__ void __launch_bounds__(256) column_parts_kernel(const __grid_constant__ ColumnSources s) {
+  allow_dependents();
+  wait_for_prerequisites();
   const ColumnSource& src = s.source[blockIdx.z];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t c0 = blockIdx.x * 64ll, c[2] = {c0 + lane, c0 + lane + 32};
@@ -101,6 +105,8 @@ __global__ void __launch_bounds__(256) column_parts_kernel(const __grid_constant
 
 template <typename T>
 __global__ void __launch_bounds__(256) column_totals_kernel(const __grid_constant__ ColumnSources s) {
+  allow_dependents();
+  wait_for_prerequisites();
   const ColumnSource& src = s.source[blockIdx.y];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t c = blockIdx.x * 32ll + lane;
@@ -130,10 +136,14 @@ __global__ void __launch_bounds__(256) column_totals_kernel(const __grid_constan
 template <typename T>
 cudaError_t column_sums(const ColumnSources& s, int count, cudaStream_t stream) {
   if (count == 0) return cudaSuccess;
-  column_parts_kernel<T><<<dim3(static_cast<unsigned>((s.widest + 63) / 64),
-                                static_cast<unsigned>(s.part_count), count), 256, 0, stream>>>(s);
-  column_totals_kernel<T><<<dim3(static_cast<unsigned>((s.widest + 31) / 32), count), 256, 0, stream>>>(s);
-  return cudaGetLastError();
+  const cudaError_t e = launch_dependent(
+      column_parts_kernel<T>, dim3(static_cast<unsigned>((s.widest + 63) / 64),
+                                   static_cast<unsigned>(s.part_count), count),
+      dim3(256), 0, stream, s);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(column_totals_kernel<T>,
+                          dim3(static_cast<unsigned>((s.widest + 31) / 32), count), dim3(256), 0,
+                          stream, s);
 }
 
 // ---- the products ----
@@ -260,7 +270,7 @@ size_t ffn_workspace_bytes(const fhb_ffn_problem& p, bool backward, const Device
     const Saved s = saved_in(p, room);
     const size_t parts = gemm_tc_workspace_bytes(down_product(p, o, s, nullptr), dev);
     room.take(parts);
-    return room.used;
+    return std::max(room.used, ffn_small_bytes(p));
   }
   // the upstream gradient may need a copy: the size asked for does not depend on it
   inputs_in(p, nullptr, 0, room, o);
@@ -280,16 +290,19 @@ size_t ffn_workspace_bytes(const fhb_ffn_problem& p, bool backward, const Device
 
 cudaError_t launch_ffn_forward(const fhb_ffn_problem& p, void* y, void* saved, void* workspace,
                                const DeviceInfo& dev, cudaStream_t stream) {
+  if (saved == nullptr && p.tokens <= kFfnSmallTokens)
+    return launch_ffn_small(p, y, workspace, dev, stream);
   Room room{static_cast<char*>(workspace)}, kept{static_cast<char*>(saved)};
   Operands o;
   const Inputs x = inputs_in(p, nullptr, 0, room, o);
-  cudaError_t e = launch_pack(x.in, x.out, 5, p.dtype, stream);
+  bool packed = false;
+  cudaError_t e = launch_pack(x.in, x.out, 5, p.dtype, &packed, stream);
   if (e != cudaSuccess) return e;
   const Saved s = saved_in(p, saved != nullptr ? kept : room);
-  e = launch_gemm_tc(gate_product(p, o, s, saved != nullptr), nullptr, dev, stream);
+  e = launch_gemm_tc(gate_product(p, o, s, saved != nullptr), nullptr, packed, dev, stream);
   if (e != cudaSuccess) return e;
   const TcProduct down = down_product(p, o, s, y);
-  return launch_gemm_tc(down, room.take(gemm_tc_workspace_bytes(down, dev)), dev, stream);
+  return launch_gemm_tc(down, room.take(gemm_tc_workspace_bytes(down, dev)), true, dev, stream);
 }
 
 cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, int64_t grad_y_stride,
@@ -313,7 +326,8 @@ cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, in
   Room room{static_cast<char*>(workspace)}, kept{static_cast<char*>(const_cast<void*>(saved))};
   Operands o;
   const Inputs x = inputs_in(p, grad_y, grad_y_stride, room, o);
-  cudaError_t e = launch_pack(x.in, x.out, 5, p.dtype, stream);
+  bool packed = false;
+  cudaError_t e = launch_pack(x.in, x.out, 5, p.dtype, &packed, stream);
   if (e != cudaSuccess) return e;
   const Saved s = saved_in(p, kept);
   const Backward b = backward_of(p, o, s, out, room);
@@ -322,10 +336,10 @@ cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, in
                                 std::pair{b.want_down, &b.down}})
     if (want) parts = std::max(parts, gemm_tc_workspace_bytes(*q, dev));
   void* sums = room.take(parts);  // one product after the other
-  e = launch_gemm_tc(b.hidden, nullptr, dev, stream);
-  if (e == cudaSuccess && b.want_x) e = launch_gemm_tc(b.x, sums, dev, stream);
-  if (e == cudaSuccess && b.want_weights) e = launch_gemm_tc(b.weights, sums, dev, stream);
-  if (e == cudaSuccess && b.want_down) e = launch_gemm_tc(b.down, sums, dev, stream);
+  e = launch_gemm_tc(b.hidden, nullptr, packed, dev, stream);
+  if (e == cudaSuccess && b.want_x) e = launch_gemm_tc(b.x, sums, true, dev, stream);
+  if (e == cudaSuccess && b.want_weights) e = launch_gemm_tc(b.weights, sums, true, dev, stream);
+  if (e == cudaSuccess && b.want_down) e = launch_gemm_tc(b.down, sums, true, dev, stream);
   if (e != cudaSuccess) return e;
   ColumnSources columns{};
   int count = 0;

@@ -435,6 +435,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (Cg == 2) cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = tmem_at;
+  // launched as a dependent of the kernel before it: the set-up above runs beside that one's
+  // end, and nothing of its results, nor of what it still reads, is touched before this wait
+  allow_dependents();
+  wait_for_prerequisites();
 
   const uint32_t items = static_cast<uint32_t>(p.tiles_m) * p.tiles_n * p.parts * p.groups;
   const uint32_t first = blockIdx.x / Cg, stride = gridDim.x / Cg;
@@ -772,6 +776,8 @@ __global__ void __launch_bounds__(256)
     add_parts_kernel(const float* __restrict__ partial, int64_t part_values, int64_t stride, int parts,
                      int64_t m, int64_t n, const T* __restrict__ bias, Outputs<T> outputs,
                      int64_t out_stride) {
+  allow_dependents();
+  wait_for_prerequisites();
   const int64_t quads = stride / 4, step = part_values / 4;
   T* const out = outputs.group[blockIdx.y];
   partial += blockIdx.y * parts * part_values;
@@ -811,6 +817,7 @@ struct PackJobs {
 };
 template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJobs jobs) {
+  allow_dependents();
   const PackJob& j = jobs.job[blockIdx.y];
   const int64_t pieces = j.stride / 8;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < j.rows * pieces; i += gridDim.x * 256ll) {
@@ -940,28 +947,38 @@ size_t smem_bytes(const Plan& plan, bool wide) {
 }
 
 template <int Cg, TcEpilogue E, typename T>
-cudaError_t launch(const Maps& maps, const Args& args, const Plan& plan, cudaStream_t stream) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = Cg;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+cudaError_t launch(const Maps& maps, const Args& args, const Plan& plan, bool dependent, cudaStream_t stream) {
+  cudaLaunchAttribute attr[2];
+  int attrs = 0;
+  if (Cg == 2) {
+    attr[attrs].id = cudaLaunchAttributeClusterDimension;
+    attr[attrs].val.clusterDim.x = Cg;
+    attr[attrs].val.clusterDim.y = attr[attrs].val.clusterDim.z = 1;
+    ++attrs;
+  }
+  if (dependent) {
+    attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[attrs].val.programmaticStreamSerializationAllowed = 1;
+    ++attrs;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(plan.grid);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem_bytes(plan, sizeof(T) == 4);
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = Cg == 2 ? 1 : 0;
+  cfg.numAttrs = attrs;
   return cudaLaunchKernelEx(&cfg, gemm_tc_kernel<Cg, E, T>, maps, args);
 }
 
 template <TcEpilogue E>
-cudaError_t launch_kind(bool wide, const Maps& maps, const Args& args, const Plan& plan, cudaStream_t stream) {
+cudaError_t launch_kind(bool wide, const Maps& maps, const Args& args, const Plan& plan, bool dependent,
+                        cudaStream_t stream) {
   if (wide)
-    return plan.cg == 2 ? launch<2, E, float>(maps, args, plan, stream)
-                        : launch<1, E, float>(maps, args, plan, stream);
-  return plan.cg == 2 ? launch<2, E, bf16>(maps, args, plan, stream)
-                      : launch<1, E, bf16>(maps, args, plan, stream);
+    return plan.cg == 2 ? launch<2, E, float>(maps, args, plan, dependent, stream)
+                        : launch<1, E, float>(maps, args, plan, dependent, stream);
+  return plan.cg == 2 ? launch<2, E, bf16>(maps, args, plan, dependent, stream)
+                      : launch<1, E, bf16>(maps, args, plan, dependent, stream);
 }
 
 template <int Cg, TcEpilogue E>
@@ -978,10 +995,10 @@ cudaError_t add_parts(const TcProduct& p, const Plan& plan, const float* partial
                       cudaStream_t stream) {
   const int64_t values = p.m * plan.partial_stride;
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks_of(values / 4, 256), 8ll * dev.sms)), p.groups);
-  add_parts_kernel<T><<<grid, 256, 0, stream>>>(
-      partial, values, plan.partial_stride, plan.parts, p.m, p.n, static_cast<const T*>(p.bias[0]),
+  return launch_dependent(
+      add_parts_kernel<T>, grid, dim3(256), 0, stream, partial, values, plan.partial_stride,
+      plan.parts, p.m, p.n, static_cast<const T*>(p.bias[0]),
       Outputs<T>{{static_cast<T*>(p.out[0]), static_cast<T*>(p.out[1])}}, p.out_stride);
-  return cudaGetLastError();
 }
 
 }  // namespace
@@ -1007,8 +1024,8 @@ size_t gemm_tc_workspace_bytes(const TcProduct& p, const DeviceInfo& dev) {
   return plan.parts == 1 ? 0 : static_cast<size_t>(plan.parts) * p.groups * p.m * plan.partial_stride * 4;
 }
 
-cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, const DeviceInfo& dev,
-                           cudaStream_t stream) {
+cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, bool dependent,
+                           const DeviceInfo& dev, cudaStream_t stream) {
   const Plan plan = plan_of(p, dev);
   const bool wide = p.dtype == FHB_DTYPE_F32, gate = p.epilogue == TcEpilogue::kGate;
   // items are counted in 32 bits, with room for a last stride beyond them
@@ -1064,12 +1081,12 @@ cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, const DeviceInfo
       return cudaErrorInvalidValue;
   }
   switch (p.epilogue) {
-    case TcEpilogue::kGate: return launch_kind<TcEpilogue::kGate>(wide, maps, args, plan, stream);
-    case TcEpilogue::kGateGrad: return launch_kind<TcEpilogue::kGateGrad>(wide, maps, args, plan, stream);
+    case TcEpilogue::kGate: return launch_kind<TcEpilogue::kGate>(wide, maps, args, plan, dependent, stream);
+    case TcEpilogue::kGateGrad: return launch_kind<TcEpilogue::kGateGrad>(wide, maps, args, plan, dependent, stream);
     default: break;
   }
-  if (plan.parts == 1) return launch_kind<TcEpilogue::kStore>(wide, maps, args, plan, stream);
-  const cudaError_t e = launch_kind<TcEpilogue::kPartial>(wide, maps, args, plan, stream);
+  if (plan.parts == 1) return launch_kind<TcEpilogue::kStore>(wide, maps, args, plan, dependent, stream);
+  const cudaError_t e = launch_kind<TcEpilogue::kPartial>(wide, maps, args, plan, dependent, stream);
   if (e != cudaSuccess) return e;
   return wide ? add_parts<float>(p, plan, args.partial, dev, stream)
               : add_parts<bf16>(p, plan, args.partial, dev, stream);
@@ -1101,7 +1118,7 @@ TcMatrix tc_operand(const TcInput& in, int dtype, void* room) {
 }
 
 cudaError_t launch_pack(const TcInput* in, const TcMatrix* out, int count, int dtype,
-                        cudaStream_t stream) {
+                        bool* launched, cudaStream_t stream) {
   PackJobs jobs{};
   int used = 0;
   int64_t most = 0;
@@ -1111,6 +1128,7 @@ cudaError_t launch_pack(const TcInput* in, const TcMatrix* out, int count, int d
                         out[i].stride, out[i].plane};
     most = std::max(most, in[i].rows * (out[i].stride / 8));
   }
+  *launched = used > 0;
   if (used == 0) return cudaSuccess;
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks_of(most, 256), 2368)), used);
   if (dtype == FHB_DTYPE_F32) pack_kernel<float><<<grid, 256, 0, stream>>>(jobs);

@@ -63,8 +63,11 @@ struct TcProduct {
 
 // Workspace of a product: the FP32 partial sums of its parts of K (0 where it has one).
 size_t gemm_tc_workspace_bytes(const TcProduct& p, const DeviceInfo& dev);
-cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, const DeviceInfo& dev,
-                           cudaStream_t stream);
+// `dependent`: launched as a dependent of the kernel before it in the stream, which has to be
+// one of this file's or gated_ffn.cu's (they wait for their own predecessors, so a chain of them
+// keeps its order; the first kernel of a call is an ordinary launch).
+cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, bool dependent,
+                           const DeviceInfo& dev, cudaStream_t stream);
 
 // A caller's matrix: `rows` x `cols` elements of the block's type, rows `stride` apart.
 struct TcInput {
@@ -76,7 +79,7 @@ struct TcInput {
 size_t tc_operand_bytes(const TcInput& in, int dtype);
 TcMatrix tc_operand(const TcInput& in, int dtype, void* room);
 cudaError_t launch_pack(const TcInput* in, const TcMatrix* out, int count, int dtype,
-                        cudaStream_t stream);
+                        bool* launched, cudaStream_t stream);
 // A matrix of the block's type in operand form at `room`, to be written by a product.
 size_t tc_result_bytes(int64_t rows, int64_t cols, int dtype);
 TcMatrix tc_result(void* room, int64_t rows, int64_t cols, int dtype);
