@@ -290,7 +290,7 @@ size_t ffn_workspace_bytes(const fhb_ffn_problem& p, bool backward, const Device
 
 cudaError_t launch_ffn_forward(const fhb_ffn_problem& p, void* y, void* saved, void* workspace,
                                const DeviceInfo& dev, cudaStream_t stream) {
-  if (saved == nullptr && p.tokens <= kFfnSmallTokens)
+  if (saved == nullptr && p.tokens <= ffn_small_tokens(p.dtype))
     return launch_ffn_small(p, y, workspace, dev, stream);
   Room room{static_cast<char*>(workspace)}, kept{static_cast<char*>(saved)};
   Operands o;

@@ -24,11 +24,11 @@ constexpr int kMaxColumns = 256;                 // result columns of a tile
 constexpr int kEpilogueWarps = 16;
 constexpr int kGroup = 16;                       // columns that a thread works on together
 constexpr int kThreads = 32 * (kEpilogueWarps + 2);
-constexpr int kMaxSlots = 10;
+constexpr int kMaxSlots = 16;
 constexpr int kRingBytes = 216 * 1024;
 constexpr int kPlanes = 3;                       // of an FP32 operand
 constexpr int kMaxOperands = 5;  // of a block's products
-constexpr int kATileBytes = kRows * kKBlock * 2;  // 16 KB
+constexpr int kATileBytes = kRows * kKBlock * 2;  // 16 KB: of 128 rows, all of which an MMA reads
 
 struct Maps {
   CUtensorMap a[2], b[2];
@@ -42,7 +42,9 @@ struct Args {
   int slots, slot_blocks;     // of the ring; blocks of K in a slot
   int sum_terms;
   int a_k_major, b_k_major;
-  int a_rows;                 // rows of one A copy (fewer than 128 where m is small)
+  // rows of one A copy: fewer than 128 where m is small (the MMAs then read what follows as the
+  // other rows, whose results are not used)
+  int a_rows;
   uint32_t idesc;
   // results
   void* out[2];
@@ -415,7 +417,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t rank = Cg == 2 ? cluster_rank() : 0;
   const int b_rows = p.columns / Cg;  // rows of this CTA's B tile
   const uint32_t b_tile_bytes = static_cast<uint32_t>(b_rows) * kKBlock * 2;
-  const uint32_t block_bytes = kCopies * (kATileBytes + b_tile_bytes);  // of one block of K
+  const uint32_t a_tile_bytes = static_cast<uint32_t>(p.a_rows) * kKBlock * 2;
+  const uint32_t block_bytes = kCopies * (a_tile_bytes + b_tile_bytes);  // of one block of K
   const uint32_t slot_bytes = block_bytes * p.slot_blocks;
 
   if (threadIdx.x == 0) {
@@ -450,8 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t phase = 0;
       bool ok = true;
       int64_t issued = 0;
-      const uint32_t a_bytes = p.a_k_major ? static_cast<uint32_t>(p.a_rows) * kKBlock * 2 : kATileBytes;
-      const uint32_t bytes = Cg * kCopies * (a_bytes + b_tile_bytes);
+      const uint32_t bytes = Cg * block_bytes;
       const uint32_t first_bar = Cg == 2 ? in_cta(smem_u32(&full[0]), 0) : smem_u32(&full[0]);
       for (uint32_t index = first; ok && index < items; index += stride) {
         const Item it = item_at<Cg, kGateTile>(p, index);
@@ -475,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint32_t bar = first_bar + slot * 8;
               for (int j = 0; j < blocks; ++j) {
                 const uint32_t at = ring + slot * slot_bytes + j * block_bytes;
-                const uint32_t bt = at + kCopies * kATileBytes;
+                const uint32_t bt = at + kCopies * a_tile_bytes;
                 const int k0 = (kb + j) * kKBlock;
                 if (p.a_k_major) {
                   copy_tile<Cg>(at, am, k0, a0, 0, bar);
@@ -525,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       const uint32_t a_step = p.a_k_major ? 2 : 128, b_step = p.b_k_major ? 2 : 128;  // 16 of K
       // bytes from plane to plane and (operand across K) from one block of 64 rows to the next
-      const uint32_t a_plane = p.a_k_major ? static_cast<uint32_t>(p.a_rows) * 128 : 8192;
+      const uint32_t a_plane = p.a_k_major ? a_tile_bytes : 8192;
       const uint32_t b_plane = p.b_k_major ? b_tile_bytes : 8192;
       const uint64_t a_desc = tile_descriptor(0, kCopies * 8192), b_desc = a_desc;
       for (uint32_t index = first; ok && index < items; index += stride) {
@@ -548,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               tc::fence_after_sync();
               const uint32_t at = ring + slot * slot_bytes;
               if constexpr (kChunked) {
-                const uint32_t bt = at + kCopies * kATileBytes;
+                const uint32_t bt = at + kCopies * a_tile_bytes;
                 const uint64_t a0 = a_desc | (at >> 4), b0 = b_desc | (bt >> 4);
                 const uint64_t a1 = a0 + (a_plane >> 4), b1 = b0 + (b_plane >> 4);
                 const uint64_t a2 = a1 + (a_plane >> 4), b2 = b1 + (b_plane >> 4);
@@ -562,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 accumulate = 1;
               } else {
                 const int here = min(p.slot_blocks, blocks - kb);
-                uint64_t a0 = a_desc | (at >> 4), b0 = b_desc | ((at + kATileBytes) >> 4);
+                uint64_t a0 = a_desc | (at >> 4), b0 = b_desc | ((at + a_tile_bytes) >> 4);
                 for (int j = 0; j < here; ++j) {
                   mma_slot<Cg>(d, a0, b0, a_step, b_step, p.idesc, accumulate);
                   accumulate = 1;
@@ -856,35 +858,39 @@ int64_t blocks_of(int64_t x, int64_t size) { return (x + size - 1) / size; }
 
 // ---- the plan of a product: tile, pairing, parts of K ----
 struct Plan {
-  int cg, columns, parts, part_blocks, k_blocks, tiles_m, tiles_n, slots, slot_blocks, grid;
+  int cg, columns, a_rows, parts, part_blocks, k_blocks, tiles_m, tiles_n, slots, slot_blocks, grid;
   int64_t partial_stride;
 };
 // Bytes of the ring that one block of K takes.
-int block_bytes_of(bool wide, int cg, int columns) {
-  return (wide ? kPlanes : 1) * (kATileBytes + columns / cg * kKBlock * 2);
+int block_bytes_of(bool wide, int cg, int columns, int a_rows) {
+  return (wide ? kPlanes : 1) * (a_rows + columns / cg) * kKBlock * 2;
 }
 
 // Chooses by an estimate of the launch's cycles. A block of K costs its MMAs (4 x columns / 2
 // cycles a product of planes, the same in a pair with half the B tile each) or the copies of its
 // bytes (about 64 a cycle), whichever is longer; an item costs about 2,000 cycles more (its
 // first copies, its last results), and a second launch that adds the parts about 3,000 and its
-// bytes.
+// bytes. So a few tokens get tiles as narrow as still fill one
+// round of the SMs (48 x 2048 x 5632 bf16, first product: 14.1 us with 118 tiles of 96 columns,
+// 14.6 with 88 of 128, 19.7 with 176 of 64).
 Plan plan_of(const TcProduct& p, const DeviceInfo& dev) {
   const bool wide = p.dtype == FHB_DTYPE_F32, gate = p.epilogue == TcEpilogue::kGate;
   const int k_blocks = static_cast<int>(blocks_of(p.k, kKBlock));
   const int64_t n_columns = gate ? 2 * p.n : p.n;
+  // an operand across K comes in blocks of 64 rows
+  const int a_rows = p.a_k_major ? static_cast<int>(std::min<int64_t>(kRows, round_up(p.m, 8))) : kRows;
   Plan best{};
   double least = 0.0;
   for (int cg = 1; cg <= 2; ++cg)
-    for (int columns = 64; columns <= (wide ? kSmallColumns : kMaxColumns); columns *= 2) {
-      if (cg == 2 && columns < 128) continue;  // an operand across K comes in blocks of 64
-      if (cg == 2 && p.m <= kRows) continue;
+    for (const int columns : {64, 96, 128, 192, 256}) {
+      if (columns > (wide ? kSmallColumns : kMaxColumns) || (cg == 2 && (columns < 128 || p.m <= kRows))) continue;
+      if (!p.b_k_major && columns / cg % 64 != 0) continue;  // an operand across K comes in blocks of 64
       const int64_t tiles_m = blocks_of(p.m, kRows * cg);
       const int64_t tiles_n = blocks_of(n_columns, columns);
       const int64_t tiles = tiles_m * tiles_n * p.groups;
       const int64_t units = dev.sms / cg;
       const double mma = 2.0 * columns * (wide ? 6 : 1);
-      const double block = p.sum_terms * std::max(mma, block_bytes_of(wide, cg, columns) / 64.0);
+      const double block = p.sum_terms * std::max(mma, block_bytes_of(wide, cg, columns, a_rows) / 64.0);
       // one to four parts, or as many as fill one or two rounds of the SMs
       for (int choice = 1; choice <= (p.epilogue == TcEpilogue::kStore ? 6 : 1); ++choice) {
         const int64_t wanted = choice <= 4 ? choice : std::min<int64_t>(units * (choice - 4) / tiles, 128);
@@ -907,10 +913,17 @@ Plan plan_of(const TcProduct& p, const DeviceInfo& dev) {
       }
     }
   best.k_blocks = k_blocks;
-  // two blocks of K a slot halve the waits between MMAs, where at least three slots remain
-  const int block_bytes = block_bytes_of(wide, best.cg, best.columns);
-  best.slot_blocks = !wide && best.part_blocks > 1 && kRingBytes / (2 * block_bytes) >= 3 ? 2 : 1;
-  best.slots = std::min(kMaxSlots, kRingBytes / (best.slot_blocks * block_bytes));
+  best.a_rows = a_rows;
+  const int block_bytes = block_bytes_of(wide, best.cg, best.columns, a_rows);
+  const int room = kRingBytes - (a_rows < kRows ? kATileBytes : 0);  // an MMA reads past the last rows
+  // blocks of K a slot: two halve the waits between MMAs, where at least three slots remain; four
+  // in narrow tiles, whose time is that of reading the weights: DRAM then gives 512 bytes of a
+  // row together (48 x 2048 x 5632 bf16, 64 columns: 31, 23 and 20 us with 1, 2 and 4)
+  best.slot_blocks = 1;
+  for (const int blocks : {2, 4})
+    if (!wide && best.part_blocks >= blocks && (blocks == 2 || best.columns < 128) && room / (blocks * block_bytes) >= 3)
+      best.slot_blocks = blocks;
+  best.slots = std::min(kMaxSlots, room / (best.slot_blocks * block_bytes));
   best.partial_stride = round_up(p.n, 32);
   return best;
 }
@@ -943,7 +956,9 @@ bool tile_map(const TcMatrix& x, int box_rows, int box_planes, CUtensorMap* out)
 }
 
 size_t smem_bytes(const Plan& plan, bool wide) {
-  return static_cast<size_t>(plan.slots) * plan.slot_blocks * block_bytes_of(wide, plan.cg, plan.columns) + 1024;
+  return static_cast<size_t>(plan.slots) * plan.slot_blocks *
+             block_bytes_of(wide, plan.cg, plan.columns, plan.a_rows) +
+         (plan.a_rows < kRows ? kATileBytes : 0) + 1024;
 }
 
 template <int Cg, TcEpilogue E, typename T>
@@ -1046,7 +1061,7 @@ cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, bool dependent,
   args.sum_terms = p.sum_terms;
   args.a_k_major = p.a_k_major;
   args.b_k_major = p.b_k_major;
-  args.a_rows = static_cast<int>(std::min<int64_t>(kRows, round_up(p.m, 8)));
+  args.a_rows = plan.a_rows;
   args.idesc = (1u << 4) | (1u << 7) | (1u << 10) | (p.a_k_major ? 0u : tc::kIdescAMnMajor) |
                (p.b_k_major ? 0u : tc::kIdescBMnMajor) |
                (static_cast<uint32_t>(plan.columns) >> 3 << 17) |
