@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "blocks.cuh"
+#include "common.cuh"
 
 namespace fhb {
 namespace {
@@ -28,6 +29,61 @@ struct NormArgs {
   int width;
   const float* scale_ptr;
   float scale, eps;
+  int stages;            // rows on their way to a CTA (0: it loads them itself)
+  unsigned int* status;
+};
+
+// Rows on their way (a CTA a row, aligned rows): one thread starts the bulk copies of a row's
+// arrays into shared memory `stages` rows ahead, so that what is in flight takes no registers.
+// A stage is free again when the CTA has met in the row's sums, after everybody read it.
+constexpr int kMaxStages = 4;
+constexpr int kMaxArrays = 5;
+struct Stage {
+  uint64_t* full;        // one barrier a stage
+  unsigned char* base;
+  int stages, at;
+  uint32_t phase, bytes;  // of the arrays of one row
+  bool late;              // a wait gave up: no more waits, the status says so
+  unsigned int* status;
+
+  __device__ __forceinline__ void start(unsigned char* memory, uint64_t* barriers, int count,
+                                        uint32_t row_bytes, unsigned int* word) {
+    full = barriers;
+    base = memory;
+    stages = count;
+    at = 0;
+    phase = 0;
+    bytes = row_bytes;
+    late = false;
+    status = word;
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < stages; ++i) mbar_init(&full[i], 1);
+      fence_barrier_init();
+    }
+    __syncthreads();
+  }
+  // one thread: the arrays of a row into stage `into`
+  __device__ __forceinline__ void copy(int into, const void* const (&from)[kMaxArrays],
+                                       const uint32_t (&size)[kMaxArrays]) const {
+    mbar_arrive_expect_tx(&full[into], bytes);
+    unsigned char* to = base + into * bytes;
+#pragma unroll
+    for (int i = 0; i < kMaxArrays; ++i)
+      if (size[i] != 0) {
+        bulk_copy_g2s(to, from[i], size[i], &full[into]);
+        to += size[i];
+      }
+  }
+  __device__ __forceinline__ const unsigned char* wait() {
+    if (!late) late = !mbar_wait_bounded(&full[at], phase, status, FHB_STATUS_STAGE_TIMEOUT);
+    return base + at * bytes;
+  }
+  __device__ __forceinline__ void next() {
+    if (++at == stages) {
+      at = 0;
+      phase ^= 1;
+    }
+  }
 };
 
 // How a row lies over threads. Lanes: 8, 16, 32 (parts of a warp, 256-thread CTAs) or 0 (the
@@ -150,8 +206,8 @@ __device__ __forceinline__ void row_sum(float (&s)[K], int& round) {
 #define FHB_EACH(L) \
   _Pragma("unroll") for (int v = 0; v < L::V; ++v) _Pragma("unroll") for (int i = 0; i < kVector; ++i)
 
-template <typename L, typename TR, typename T>
-__global__ void __launch_bounds__(L::Most)
+template <typename L, typename TR, typename T, bool Staged>
+__global__ void __launch_bounds__(L::Most, L::Most <= 256 ? 4 : 1)
     norm_kernel(NormArgs a, TR* __restrict__ total, T* __restrict__ normed,
                 float* __restrict__ stats) {
   const float scale = a.scale_ptr != nullptr ? *a.scale_ptr : a.scale;
@@ -164,18 +220,48 @@ __global__ void __launch_bounds__(L::Most)
   if (one_gate) load_row<L>(static_cast<const T*>(a.gate), a.width, gate);
   int round = 0;
   const int64_t step = static_cast<int64_t>(gridDim.x) * L::slots();
+  const auto residual_at = [&](int64_t row) {
+    return static_cast<const TR*>(a.residual) + row * a.residual_stride;
+  };
+  const auto branch_at = [&](int64_t row) {
+    return static_cast<const T*>(a.branch) + row * a.branch_stride;
+  };
+  const auto gate_at = [&](int64_t row) {
+    return static_cast<const T*>(a.gate) + row / a.gate_rows * a.width;
+  };
+  extern __shared__ __align__(16) unsigned char rows_memory[];
+  __shared__ uint64_t full[kMaxStages];
+  Stage stage;
+  const uint32_t wide = a.width * sizeof(TR), narrow = a.width * sizeof(T);
+  const uint32_t size[kMaxArrays] = {wide, a.branch != nullptr ? narrow : 0,
+                                     gated && !one_gate ? narrow : 0, 0, 0};
+  const auto send = [&](int into, int64_t row) {
+    const void* const from[kMaxArrays] = {residual_at(row), branch_at(row),
+                                          gated ? gate_at(row) : nullptr, nullptr, nullptr};
+    stage.copy(into, from, size);
+  };
+  if (Staged) {
+    stage.start(rows_memory, full, a.stages, size[0] + size[1] + size[2], a.status);
+    if (threadIdx.x == 0)
+      for (int i = 0; i < a.stages && blockIdx.x + i * step < a.rows; ++i) send(i, blockIdx.x + i * step);
+  }
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * L::slots(); first < a.rows; first += step) {
     const int64_t row = first + L::slot();
     const bool real = row < a.rows;
     float t[L::V][kVector], b[L::V][kVector];
-    fill<L>(t, 0.0f);
     fill<L>(b, 0.0f);
-    if (real) {
-      load_row<L>(static_cast<const TR*>(a.residual) + row * a.residual_stride, a.width, t);
-      if (a.branch != nullptr)
-        load_row<L>(static_cast<const T*>(a.branch) + row * a.branch_stride, a.width, b);
-      if (gated && !one_gate)
-        load_row<L>(static_cast<const T*>(a.gate) + row / a.gate_rows * a.width, a.width, gate);
+    if (Staged) {
+      const unsigned char* from = stage.wait();
+      load_row<L>(reinterpret_cast<const TR*>(from), a.width, t);
+      if (size[1] != 0) load_row<L>(reinterpret_cast<const T*>(from + size[0]), a.width, b);
+      if (size[2] != 0) load_row<L>(reinterpret_cast<const T*>(from + size[0] + size[1]), a.width, gate);
+    } else {
+      fill<L>(t, 0.0f);
+      if (real) {
+        load_row<L>(residual_at(row), a.width, t);
+        if (a.branch != nullptr) load_row<L>(branch_at(row), a.width, b);
+        if (gated && !one_gate) load_row<L>(gate_at(row), a.width, gate);
+      }
     }
     float ib = 1.0f;
     if (post) {
@@ -193,6 +279,11 @@ __global__ void __launch_bounds__(L::Most)
       s[0] += t[v][i] * t[v][i];
     }
     row_sum<L>(s, round);
+    if (Staged) {
+      const int64_t ahead = row + a.stages * step;
+      if (threadIdx.x == 0 && ahead < a.rows) send(stage.at, ahead);
+      stage.next();
+    }
     const float it = 1.0f / sqrtf(s[0] * inverse + a.eps);
     if (!real) continue;
     if (total != nullptr) store_row<L>(total + row * a.width, a.width, t);
@@ -222,7 +313,7 @@ struct NormGrads {
   bool want_pre, want_post, want_gate, want_scale;
 };
 
-template <typename L, typename TR, typename T>
+template <typename L, typename TR, typename T, bool Staged>
 __global__ void __launch_bounds__(L::Most, L::Resident)
     norm_backward_kernel(NormArgs a, NormGrads g, Units units, const float* __restrict__ stats) {
   const float scale = a.scale_ptr != nullptr ? *a.scale_ptr : a.scale;
@@ -240,13 +331,45 @@ __global__ void __launch_bounds__(L::Most, L::Resident)
   int round = 0;
   const int64_t count = units.groups * units.parts;
   const int64_t step = static_cast<int64_t>(gridDim.x) * L::slots();
+  // the rows [begin, end) of a unit, none for a unit past the last
+  const auto rows_of = [&](int64_t unit, int64_t& begin, int64_t& end) {
+    const int64_t group = unit / units.parts, part = unit - group * units.parts;
+    begin = group * units.group_rows + part * units.part_rows;
+    end = unit < count ? min(begin + units.part_rows, min((group + 1) * units.group_rows, a.rows)) : begin;
+  };
+  extern __shared__ __align__(16) unsigned char rows_memory[];
+  __shared__ uint64_t full[kMaxStages];
+  Stage stage;
+  const uint32_t wide = a.width * sizeof(TR), narrow = a.width * sizeof(T);
+  const uint32_t size[kMaxArrays] = {wide, branch ? narrow : 0, g.total != nullptr ? wide : 0,
+                                     g.normed != nullptr ? narrow : 0, by_group ? narrow : 0};
+  // thread 0's place in the rows to come
+  int64_t send_unit = blockIdx.x, send_row = 0, send_end = 0;
+  const auto send = [&](int into) {
+    while (send_row >= send_end) {
+      if (send_unit >= count) return;
+      rows_of(send_unit, send_row, send_end);
+      send_unit += step;
+    }
+    const void* const from[kMaxArrays] = {
+        static_cast<const TR*>(a.residual) + send_row * a.residual_stride,
+        static_cast<const T*>(a.branch) + send_row * a.branch_stride,
+        static_cast<const TR*>(g.total) + send_row * g.total_stride,
+        static_cast<const T*>(g.normed) + send_row * g.normed_stride,
+        static_cast<const T*>(a.gate) + send_row / a.gate_rows * a.width};
+    stage.copy(into, from, size);
+    ++send_row;
+  };
+  if (Staged) {
+    stage.start(rows_memory, full, a.stages, size[0] + size[1] + size[2] + size[3] + size[4], a.status);
+    if (threadIdx.x == 0)
+      for (int i = 0; i < a.stages; ++i) send(i);
+  }
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * L::slots(); first < count; first += step) {
-    const int64_t unit = first + L::slot();
-    const int64_t group = unit / units.parts, part = unit % units.parts;
-    const int64_t group_end = min((group + 1) * units.group_rows, a.rows);
-    const int64_t begin = group * units.group_rows + part * units.part_rows;
-    const int64_t end = unit < count ? min(begin + units.part_rows, group_end) : begin;
-    if (by_group && unit < count)
+    const int64_t unit = first + L::slot(), group = unit / units.parts;
+    int64_t begin, end;
+    rows_of(unit, begin, end);
+    if (!Staged && by_group && unit < count)
       load_row<L>(static_cast<const T*>(a.gate) + group * a.width, a.width, gate);
     // the slots of a warp go through as many rows together, some of them without a row
     for (int64_t k = 0; k < units.part_rows; ++k) {
@@ -254,20 +377,35 @@ __global__ void __launch_bounds__(L::Most, L::Resident)
       const bool real = row < end;
       if (L::Lanes == 0 && !real) break;
       float r[L::V][kVector], b[L::V][kVector], dT[L::V][kVector], dn[L::V][kVector];
-      fill<L>(r, 0.0f);
+      float ib = 1.0f, it = 1.0f;
+      if (real) {
+        ib = stats[2 * row];
+        it = stats[2 * row + 1];
+      }
       fill<L>(b, 0.0f);
       fill<L>(dT, 0.0f);
       fill<L>(dn, 0.0f);
-      float ib = 1.0f, it = 1.0f;
-      if (real) {
-        load_row<L>(static_cast<const TR*>(a.residual) + row * a.residual_stride, a.width, r);
-        if (branch) load_row<L>(static_cast<const T*>(a.branch) + row * a.branch_stride, a.width, b);
-        if (g.total != nullptr)
-          load_row<L>(static_cast<const TR*>(g.total) + row * g.total_stride, a.width, dT);
-        if (g.normed != nullptr)
-          load_row<L>(static_cast<const T*>(g.normed) + row * g.normed_stride, a.width, dn);
-        ib = stats[2 * row];
-        it = stats[2 * row + 1];
+      if (Staged) {
+        const unsigned char* from = stage.wait();
+        load_row<L>(reinterpret_cast<const TR*>(from), a.width, r);
+        from += size[0];
+        if (size[1] != 0) load_row<L>(reinterpret_cast<const T*>(from), a.width, b);
+        from += size[1];
+        if (size[2] != 0) load_row<L>(reinterpret_cast<const TR*>(from), a.width, dT);
+        from += size[2];
+        if (size[3] != 0) load_row<L>(reinterpret_cast<const T*>(from), a.width, dn);
+        from += size[3];
+        if (size[4] != 0) load_row<L>(reinterpret_cast<const T*>(from), a.width, gate);
+      } else {
+        fill<L>(r, 0.0f);
+        if (real) {
+          load_row<L>(static_cast<const TR*>(a.residual) + row * a.residual_stride, a.width, r);
+          if (branch) load_row<L>(static_cast<const T*>(a.branch) + row * a.branch_stride, a.width, b);
+          if (g.total != nullptr)
+            load_row<L>(static_cast<const TR*>(g.total) + row * g.total_stride, a.width, dT);
+          if (g.normed != nullptr)
+            load_row<L>(static_cast<const T*>(g.normed) + row * g.normed_stride, a.width, dn);
+        }
       }
       float s[3] = {};
       FHB_EACH(L) {
@@ -280,6 +418,10 @@ __global__ void __launch_bounds__(L::Most, L::Resident)
         s[2] += th * cz;
       }
       row_sum<L>(s, round);
+      if (Staged) {
+        if (threadIdx.x == 0) send(stage.at);
+        stage.next();
+      }
       if (!real) continue;
       const float m1 = s[0] * inverse, m2 = (s[1] - it * m1 * s[2]) * inverse;
       FHB_EACH(L) {
@@ -312,7 +454,7 @@ __global__ void __launch_bounds__(L::Most, L::Resident)
     }
   }
   // the CTA's column sums: its slots' one after the other
-  extern __shared__ float columns[];
+  float* columns = reinterpret_cast<float*>(rows_memory);
   float* out = g.columns + static_cast<int64_t>(blockIdx.x) * 3 * a.width;
   const auto leave = [&](const float (&x)[L::V][kVector], int which) {
     if (L::Lanes == 0) {
@@ -423,7 +565,13 @@ __global__ void __launch_bounds__(256) norm_totals_kernel(Totals t) {
 NormArgs arguments(const fhb_norm_problem& p) {
   return {p.residual, p.branch, p.pre_weight, p.post_weight, p.gate, p.rows, p.residual_stride,
           p.branch_stride, p.gate != nullptr ? p.gate_rows : std::max<int64_t>(p.rows, 1),
-          static_cast<int>(p.width), p.residual_scale_ptr, p.residual_scale, p.eps};
+          static_cast<int>(p.width), p.residual_scale_ptr, p.residual_scale, p.eps, 0, nullptr};
+}
+
+// Rows a CTA can have on their way in its part of an SM's shared memory; fewer than two: none.
+int stages_of(int64_t row_bytes, int resident) {
+  const int64_t n = std::min<int64_t>(216 * 1024 / resident / row_bytes, kMaxStages);
+  return n >= 2 ? static_cast<int>(n) : 0;
 }
 
 bool wide_rows(const void* p, int64_t stride, int dtype) {
@@ -447,10 +595,11 @@ int row_threads(int64_t width) {
 int slots_of(int threads) { return threads <= 32 ? 256 / threads : 1; }
 int block_of(int threads) { return threads <= 32 ? 256 : threads; }
 
-// CTAs: enough for 1,536 threads on every SM in the forward, 1,024 in the backward (its sums
-// take registers, and every CTA leaves a row of column sums).
-int64_t ctas(int threads, int per_sm_threads, const DeviceInfo& dev) {
-  return static_cast<int64_t>(dev.sms) * std::max(1, per_sm_threads / block_of(threads));
+// CTAs an SM holds: four of up to 256 threads in the forward, two in the backward (whose sums
+// take registers, and where every CTA leaves a row of column sums).
+int resident_of(int threads, bool backward) { return block_of(threads) <= 256 ? (backward ? 2 : 4) : 1; }
+int64_t ctas(int threads, bool backward, const DeviceInfo& dev) {
+  return static_cast<int64_t>(dev.sms) * resident_of(threads, backward);
 }
 
 Units units_of(const fhb_norm_problem& p, const DeviceInfo& dev) {
@@ -459,12 +608,12 @@ Units units_of(const fhb_norm_problem& p, const DeviceInfo& dev) {
   u.group_rows = p.gate != nullptr ? std::min(p.gate_rows, std::max<int64_t>(p.rows, 1))
                                    : std::max<int64_t>(p.rows, 1);
   u.groups = std::max<int64_t>(1, (p.rows + u.group_rows - 1) / u.group_rows);
-  u.slots = ctas(threads, 1024, dev) * slots_of(threads);
+  u.slots = ctas(threads, true, dev) * slots_of(threads);
   u.parts = std::min(std::max<int64_t>(1, u.slots / u.groups), u.group_rows);
   u.part_rows = (u.group_rows + u.parts - 1) / u.parts;
   u.parts = (u.group_rows + u.part_rows - 1) / u.part_rows;
   const int64_t count = u.groups * u.parts;
-  u.grid = std::min((count + slots_of(threads) - 1) / slots_of(threads), ctas(threads, 1024, dev));
+  u.grid = std::min((count + slots_of(threads) - 1) / slots_of(threads), ctas(threads, true, dev));
   return u;
 }
 
@@ -487,6 +636,17 @@ cudaError_t with_layout(bool wide, int64_t width, Body body) {
   return wide ? with_layout<true>(width, body) : with_layout<false>(width, body);
 }
 
+// A launch with more than 48 KB of shared memory.
+template <typename Kernel, typename... Arguments>
+cudaError_t launch_staged(Kernel kernel, unsigned grid, int block, size_t smem, cudaStream_t stream,
+                          Arguments... arguments) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  kernel<<<grid, block, smem, stream>>>(arguments...);
+  return cudaGetLastError();
+}
+
 template <typename TR, typename T>
 cudaError_t forward(const fhb_norm_problem& p, void* total, void* normed, float* stats,
                     const DeviceInfo& dev, cudaStream_t stream) {
@@ -494,10 +654,22 @@ cudaError_t forward(const fhb_norm_problem& p, void* total, void* normed, float*
                     wide_rows(normed, p.width, p.dtype);
   const int threads = row_threads(p.width);
   const int64_t need = (p.rows + slots_of(threads) - 1) / slots_of(threads);
-  const unsigned grid = static_cast<unsigned>(std::min(need, ctas(threads, 1536, dev)));
+  const unsigned grid = static_cast<unsigned>(std::min(need, ctas(threads, false, dev)));
+  NormArgs args = arguments(p);
+  const int64_t row_bytes =
+      p.width * (sizeof(TR) + (p.branch != nullptr ? sizeof(T) : 0) +
+                 (p.gate != nullptr && p.gate_rows < p.rows ? sizeof(T) : 0));
+  // a single row a CTA has nothing to fetch ahead
+  if (threads > 32 && wide && need > grid) args.stages = stages_of(row_bytes, resident_of(threads, false));
+  args.status = dev.status;
   return with_layout(wide, p.width, [&](auto layout) {
-    norm_kernel<decltype(layout), TR, T><<<grid, block_of(threads), 0, stream>>>(
-        arguments(p), static_cast<TR*>(total), static_cast<T*>(normed), stats);
+    using L = decltype(layout);
+    if constexpr (L::Lanes == 0 && L::Wide)
+      if (args.stages > 0)
+        return launch_staged(norm_kernel<L, TR, T, true>, grid, block_of(threads), args.stages * row_bytes,
+                             stream, args, static_cast<TR*>(total), static_cast<T*>(normed), stats);
+    norm_kernel<L, TR, T, false><<<grid, block_of(threads), 0, stream>>>(
+        args, static_cast<TR*>(total), static_cast<T*>(normed), stats);
     return cudaGetLastError();
   });
 }
@@ -516,12 +688,25 @@ Room room_of(const fhb_norm_problem& p, const Units& u, void* base) {
 
 template <typename TR, typename T>
 cudaError_t backward(const fhb_norm_problem& p, const NormGrads& g, const Units& u, const Totals& t,
-                     const float* stats, bool wide, cudaStream_t stream) {
+                     const float* stats, bool wide, const DeviceInfo& dev,
+                     cudaStream_t stream) {
   const int threads = row_threads(p.width);
   const size_t smem = threads <= 32 ? static_cast<size_t>(slots_of(threads)) * p.width * 4 : 0;
+  NormArgs args = arguments(p);
+  const int64_t row_bytes = p.width * (sizeof(TR) + (p.branch != nullptr ? sizeof(T) : 0) +
+                                       (g.total != nullptr ? sizeof(TR) : 0) +
+                                       (g.normed != nullptr ? sizeof(T) : 0) +
+                                       (p.gate != nullptr && u.groups > 1 ? sizeof(T) : 0));
+  if (threads > 32 && wide && p.rows > u.grid) args.stages = stages_of(row_bytes, resident_of(threads, true));
+  args.status = dev.status;
   const cudaError_t e = with_layout(wide, p.width, [&](auto layout) {
-    norm_backward_kernel<decltype(layout), TR, T>
-        <<<static_cast<unsigned>(u.grid), block_of(threads), smem, stream>>>(arguments(p), g, u, stats);
+    using L = decltype(layout);
+    if constexpr (L::Lanes == 0 && L::Wide)
+      if (args.stages > 0)
+        return launch_staged(norm_backward_kernel<L, TR, T, true>, static_cast<unsigned>(u.grid),
+                             block_of(threads), args.stages * row_bytes, stream, args, g, u, stats);
+    norm_backward_kernel<L, TR, T, false>
+        <<<static_cast<unsigned>(u.grid), block_of(threads), smem, stream>>>(args, g, u, stats);
     return cudaGetLastError();
   });
   if (e != cudaSuccess || !(g.want_pre || g.want_post || g.want_gate || g.want_scale)) return e;
@@ -564,9 +749,9 @@ cudaError_t launch_residual_norm_backward(const fhb_norm_problem& p, const void*
                     wide_rows(out.residual, p.width, p.residual_dtype) &&
                     wide_rows(out.branch, p.width, p.dtype) && wide_rows(out.gate, p.width, p.dtype);
   if (p.residual_dtype == FHB_DTYPE_F32)
-    return p.dtype == FHB_DTYPE_F32 ? backward<float, float>(p, g, u, t, stats, wide, stream)
-                                    : backward<float, bf16>(p, g, u, t, stats, wide, stream);
-  return backward<bf16, bf16>(p, g, u, t, stats, wide, stream);
+    return p.dtype == FHB_DTYPE_F32 ? backward<float, float>(p, g, u, t, stats, wide, dev, stream)
+                                    : backward<float, bf16>(p, g, u, t, stats, wide, dev, stream);
+  return backward<bf16, bf16>(p, g, u, t, stats, wide, dev, stream);
 }
 
 }  // namespace fhb
