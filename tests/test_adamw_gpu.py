@@ -238,3 +238,14 @@ def test_trunk_in_bfloat16_follows_float32():
         want = model(points)
         got = model.to(torch.bfloat16)(points.to(torch.bfloat16)).float()
     assert float((got - want).norm() / want.norm()) < 0.1
+
+
+@pytest.mark.parametrize("dtype,bits", [(torch.float32, 32), (torch.bfloat16, 8)])
+def test_fit_trunk_example(dtype, bits):
+    from fused_hoad.fit_trunk import fit_trunk
+
+    model, before, after, ms = fit_trunk(points=4096, blocks=2, hidden=128, steps=150, dtype=dtype,
+                                         state_bits=bits)
+    assert after < 0.1 * before and ms > 0
+    assert next(model.parameters()).dtype == dtype
+    assert fused_hoad.read_device_status(0) == 0
