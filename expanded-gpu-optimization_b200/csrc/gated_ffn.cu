@@ -202,8 +202,8 @@ TcProduct down_product(const fhb_ffn_problem& p, const Operands& o, const Saved&
 
 struct Backward {
   TcMatrix dg, du;
-  TcProduct hidden, x, weights, down;
-  bool want_x, want_weights, want_down;
+  TcProduct hidden;
+  TcProduct rest[kTcMaxProducts];  // the projections', w_down's and x's gradients
 };
 Backward backward_of(const fhb_ffn_problem& p, const Operands& o, const Saved& s,
                      const fhb_ffn_grads& out, Room& room) {
@@ -222,28 +222,34 @@ Backward backward_of(const fhb_ffn_problem& p, const Operands& o, const Saved& s
     b.hidden.row_sums = static_cast<float*>(room.take(
         static_cast<size_t>((p.tokens + 31) / 32 * 2 * b.hidden.row_sums_stride * 4)));
   }
-  b.want_x = out.x != nullptr;
-  b.x = store_product(p, p.tokens, p.width, p.hidden, out.x);
-  b.x.a[0] = b.dg, b.x.a[1] = b.du, b.x.b[0] = o.w_gate, b.x.b[1] = o.w_up;
-  b.x.b_k_major = false;
-  b.x.sum_terms = 2;
-  b.want_weights = out.w_gate != nullptr || out.w_up != nullptr;
-  const bool both = out.w_gate != nullptr && out.w_up != nullptr;
-  b.weights = store_product(p, p.hidden, p.width, p.tokens, both || out.w_up == nullptr ? out.w_gate : out.w_up);
-  b.weights.a[0] = both || out.w_up == nullptr ? b.dg : b.du;
-  if (both) b.weights.a[1] = b.du, b.weights.out[1] = out.w_up;
-  b.weights.groups = both ? 2 : 1;
-  b.weights.b[0] = o.x;
-  b.weights.a_k_major = b.weights.b_k_major = false;
-  b.want_down = out.w_down != nullptr;
-  b.down = store_product(p, p.out_width, p.hidden, p.tokens, out.w_down);
-  b.down.a[0] = o.dy, b.down.b[0] = s.h;
-  b.down.a_k_major = b.down.b_k_major = false;
+  // the long sums over the tokens first: in one launch their items are its longest
+  TcProduct &weights = b.rest[0], &down = b.rest[1], &x = b.rest[2];
+  weights = store_product(p, p.hidden, p.width, p.tokens, out.w_gate);
+  weights.out[1] = out.w_up;
+  weights.groups = 2;
+  weights.a[0] = b.dg, weights.a[1] = b.du, weights.b[0] = o.x;
+  weights.a_k_major = weights.b_k_major = false;
+  down = store_product(p, p.out_width, p.hidden, p.tokens, out.w_down);
+  down.a[0] = o.dy, down.b[0] = s.h;
+  down.a_k_major = down.b_k_major = false;
+  x = store_product(p, p.tokens, p.width, p.hidden, out.x);
+  x.a[0] = b.dg, x.a[1] = b.du, x.b[0] = o.w_gate, x.b[1] = o.w_up;
+  x.b_k_major = false;
+  x.sum_terms = 2;
   return b;
 }
 
+// Workspace of those products: of one launch, or of three that use it one after the other.
+size_t rest_bytes(const Backward& b, const DeviceInfo& dev) {
+  if (gemm_tc_shares_launch(b.rest, kTcMaxProducts, dev))
+    return gemm_tc_workspace_bytes(b.rest, kTcMaxProducts, dev);
+  size_t most = 0;
+  for (const TcProduct& q : b.rest) most = std::max(most, gemm_tc_workspace_bytes(&q, 1, dev));
+  return most;
+}
+
 // Stands for "every gradient wanted" where sizes are asked for before the outputs exist.
-fhb_ffn_grads all_grads(const fhb_ffn_problem& p) {
+fhb_ffn_grads all_grads() {
   static char any;
   return {&any, &any, &any, &any, &any, &any, &any};
 }
@@ -268,8 +274,8 @@ size_t ffn_workspace_bytes(const fhb_ffn_problem& p, bool backward, const Device
   if (!backward) {
     inputs_in(p, nullptr, 0, room, o);
     const Saved s = saved_in(p, room);
-    const size_t parts = gemm_tc_workspace_bytes(down_product(p, o, s, nullptr), dev);
-    room.take(parts);
+    const TcProduct down = down_product(p, o, s, nullptr);
+    room.take(gemm_tc_workspace_bytes(&down, 1, dev));
     return std::max(room.used, ffn_small_bytes(p));
   }
   // the upstream gradient may need a copy: the size asked for does not depend on it
@@ -277,13 +283,8 @@ size_t ffn_workspace_bytes(const fhb_ffn_problem& p, bool backward, const Device
   room.take(tc_result_bytes(p.tokens, p.out_width, p.dtype));
   Room aside{nullptr};
   const Saved s = saved_in(p, aside);
-  const Backward b = backward_of(p, o, s, all_grads(p), room);
-  TcProduct one = b.weights;  // a single weight's gradient may be split further
-  one.groups = 1;
-  size_t parts = 0;
-  for (const TcProduct* q : {&b.x, &b.weights, static_cast<const TcProduct*>(&one), &b.down})
-    parts = std::max(parts, gemm_tc_workspace_bytes(*q, dev));
-  room.take(parts);
+  const Backward b = backward_of(p, o, s, all_grads(), room);
+  room.take(rest_bytes(b, dev));
   room.take(static_cast<size_t>(3 * column_part_count(p) * std::max(p.hidden, p.out_width) * 4));
   return room.used;
 }
@@ -299,10 +300,11 @@ cudaError_t launch_ffn_forward(const fhb_ffn_problem& p, void* y, void* saved, v
   cudaError_t e = launch_pack(x.in, x.out, 5, p.dtype, &packed, stream);
   if (e != cudaSuccess) return e;
   const Saved s = saved_in(p, saved != nullptr ? kept : room);
-  e = launch_gemm_tc(gate_product(p, o, s, saved != nullptr), nullptr, packed, dev, stream);
+  const TcProduct gate = gate_product(p, o, s, saved != nullptr);
+  e = launch_gemm_tc(&gate, 1, nullptr, packed, dev, stream);
   if (e != cudaSuccess) return e;
   const TcProduct down = down_product(p, o, s, y);
-  return launch_gemm_tc(down, room.take(gemm_tc_workspace_bytes(down, dev)), true, dev, stream);
+  return launch_gemm_tc(&down, 1, room.take(gemm_tc_workspace_bytes(&down, 1, dev)), true, dev, stream);
 }
 
 cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, int64_t grad_y_stride,
@@ -331,15 +333,14 @@ cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, in
   if (e != cudaSuccess) return e;
   const Saved s = saved_in(p, kept);
   const Backward b = backward_of(p, o, s, out, room);
-  size_t parts = 0;
-  for (const auto& [want, q] : {std::pair{b.want_x, &b.x}, std::pair{b.want_weights, &b.weights},
-                                std::pair{b.want_down, &b.down}})
-    if (want) parts = std::max(parts, gemm_tc_workspace_bytes(*q, dev));
-  void* sums = room.take(parts);  // one product after the other
-  e = launch_gemm_tc(b.hidden, nullptr, packed, dev, stream);
-  if (e == cudaSuccess && b.want_x) e = launch_gemm_tc(b.x, sums, true, dev, stream);
-  if (e == cudaSuccess && b.want_weights) e = launch_gemm_tc(b.weights, sums, true, dev, stream);
-  if (e == cudaSuccess && b.want_down) e = launch_gemm_tc(b.down, sums, true, dev, stream);
+  void* sums = room.take(rest_bytes(b, dev));
+  e = launch_gemm_tc(&b.hidden, 1, nullptr, packed, dev, stream);
+  if (gemm_tc_shares_launch(b.rest, kTcMaxProducts, dev)) {
+    if (e == cudaSuccess) e = launch_gemm_tc(b.rest, kTcMaxProducts, sums, true, dev, stream);
+  } else {
+    for (const TcProduct& q : b.rest)
+      if (e == cudaSuccess) e = launch_gemm_tc(&q, 1, sums, true, dev, stream);
+  }
   if (e != cudaSuccess) return e;
   ColumnSources columns{};
   int count = 0;

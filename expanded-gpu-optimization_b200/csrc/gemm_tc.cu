@@ -31,32 +31,40 @@ constexpr int kMaxOperands = 5;  // of a block's products
 constexpr int kATileBytes = kRows * kKBlock * 2;  // 16 KB: of 128 rows, all of which an MMA reads
 
 struct Maps {
-  CUtensorMap a[2], b[2];
+  CUtensorMap a[kTcMaxProducts][2], b[kTcMaxProducts][2];
 };
 
-struct Args {
+// One product of a launch.
+struct Job {
   int64_t m, n;               // result rows and columns (gate: n hidden features, 2 n columns)
   int tiles_m, tiles_n, groups, parts;
   int k_blocks, part_blocks;  // of K, and of each part of K
-  int columns;                // columns of a tile (both halves of a gate tile)
-  int slots, slot_blocks;     // of the ring; blocks of K in a slot
   int sum_terms;
   int a_k_major, b_k_major;
   // rows of one A copy: fewer than 128 where m is small (the MMAs then read what follows as the
   // other rows, whose results are not used)
   int a_rows;
   uint32_t idesc;
-  // results
+  uint32_t first_item;
+  // results: out + bias, or FP32 sums of each part of K
   void* out[2];
   int64_t out_stride;
   int out_wide;               // 32-byte stores are aligned
   const void* bias[2];
+  float* partial;
+  int64_t partial_stride;
+};
+struct Args {
+  Job job[kTcMaxProducts];
+  int jobs;
+  uint32_t items;
+  int columns;                // columns of a tile (both halves of a gate tile)
+  int slots, slot_blocks;     // of the ring; blocks of K in a slot
+  uint32_t slot_bytes;
   bf16* gated[2];
   int64_t gated_stride, gated_plane;
   TcFactors factors;
   int activation;
-  float* partial;
-  int64_t partial_stride;
   float* row_sums;            // [32 rows][dg, du][row_sums_stride]: their column sums, or null
   int64_t row_sums_stride;
   unsigned int* status;
@@ -364,29 +372,33 @@ __device__ __forceinline__ float sum_rows(const float (&v)[kGroup], int lane) {
   return s[0] + __shfl_xor_sync(0xffffffffu, s[0], 16);
 }
 
-// One item of work: a tile of one group's result and one part of K.
+// One item of work: a tile of one group's result of a product, and one part of K.
 struct Item {
-  int group, part, first_block, blocks;
+  int job, group, part, first_block, blocks;
   int64_t m0, n0;  // first row of the tile (of the pair), first column (gate: feature)
 };
 // (32-bit divisions: there are fewer than 2^31 items, and 64-bit ones took 3,000 cycles an item)
 template <int Cg, bool Gate>
 __device__ __forceinline__ Item item_at(const Args& p, uint32_t index) {
-  const uint32_t tiles = static_cast<uint32_t>(p.tiles_m) * static_cast<uint32_t>(p.tiles_n);
   Item it;
+  it.job = 0;
+  while (it.job + 1 < p.jobs && index >= p.job[it.job + 1].first_item) ++it.job;
+  const Job& q = p.job[it.job];
+  index -= q.first_item;
+  const uint32_t tiles = static_cast<uint32_t>(q.tiles_m) * static_cast<uint32_t>(q.tiles_n);
   const uint32_t rest = index / tiles;
   uint32_t tile = index - rest * tiles;
-  it.group = static_cast<int>(rest / p.parts);
-  it.part = static_cast<int>(rest) - it.group * p.parts;
+  it.group = static_cast<int>(rest / q.parts);
+  it.part = static_cast<int>(rest) - it.group * q.parts;
   // bands of 8 tile rows, column by column: the tiles in flight share their operands in L2
-  const uint32_t band_tiles = 8u * static_cast<uint32_t>(p.tiles_n), band = tile / band_tiles;
-  const uint32_t rows = min(8u, static_cast<uint32_t>(p.tiles_m) - 8u * band);
+  const uint32_t band_tiles = 8u * static_cast<uint32_t>(q.tiles_n), band = tile / band_tiles;
+  const uint32_t rows = min(8u, static_cast<uint32_t>(q.tiles_m) - 8u * band);
   tile -= band * band_tiles;
   const uint32_t column = tile / rows;
   it.m0 = static_cast<int64_t>(8u * band + (tile - column * rows)) * (kRows * Cg);
   it.n0 = static_cast<int64_t>(column) * (Gate ? p.columns / 2 : p.columns);
-  it.first_block = it.part * p.part_blocks;
-  it.blocks = min(p.part_blocks, p.k_blocks - it.first_block);
+  it.first_block = it.part * q.part_blocks;
+  it.blocks = min(q.part_blocks, q.k_blocks - it.first_block);
   return it;
 }
 
@@ -417,9 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t rank = Cg == 2 ? cluster_rank() : 0;
   const int b_rows = p.columns / Cg;  // rows of this CTA's B tile
   const uint32_t b_tile_bytes = static_cast<uint32_t>(b_rows) * kKBlock * 2;
-  const uint32_t a_tile_bytes = static_cast<uint32_t>(p.a_rows) * kKBlock * 2;
-  const uint32_t block_bytes = kCopies * (a_tile_bytes + b_tile_bytes);  // of one block of K
-  const uint32_t slot_bytes = block_bytes * p.slot_blocks;
+  const uint32_t slot_bytes = p.slot_bytes;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.slots; ++s) {
@@ -443,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   allow_dependents();
   wait_for_prerequisites();
 
-  const uint32_t items = static_cast<uint32_t>(p.tiles_m) * p.tiles_n * p.parts * p.groups;
+  const uint32_t items = p.items;
   const uint32_t first = blockIdx.x / Cg, stride = gridDim.x / Cg;
 
   if (warp == kEpilogueWarps) {
@@ -453,10 +463,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t phase = 0;
       bool ok = true;
       int64_t issued = 0;
-      const uint32_t bytes = Cg * block_bytes;
       const uint32_t first_bar = Cg == 2 ? in_cta(smem_u32(&full[0]), 0) : smem_u32(&full[0]);
       for (uint32_t index = first; ok && index < items; index += stride) {
         const Item it = item_at<Cg, kGateTile>(p, index);
+        const Job& q = p.job[it.job];
+        const uint32_t a_tile_bytes = static_cast<uint32_t>(q.a_rows) * kKBlock * 2;
+        const uint32_t block_bytes = kCopies * (a_tile_bytes + b_tile_bytes);  // of one block of K
+        const bool a_k_major = q.a_k_major != 0, b_k_major = q.b_k_major != 0;
         const int chunks = chunk_count<T>(it.blocks);
         const int a0 = static_cast<int>(it.m0 + rank * kRows);
         const int b0 = static_cast<int>(it.n0) + (kGateTile ? 0 : static_cast<int>(rank) * b_rows);
@@ -464,22 +477,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int low = it.first_block + (kChunked ? c * kChunkBlocks : 0);
           const int high = kChunked ? min(low + kChunkBlocks, it.first_block + it.blocks)
                                     : it.first_block + it.blocks;
-          for (int t = 0; ok && t < p.sum_terms; ++t) {
-            const CUtensorMap* am = &maps.a[p.groups == 2 ? it.group : t];
-            const CUtensorMap* bm = &maps.b[kGateTile && Cg == 2 ? static_cast<int>(rank) : t];
+          for (int t = 0; ok && t < q.sum_terms; ++t) {
+            const CUtensorMap* am = &maps.a[it.job][q.groups == 2 ? it.group : t];
+            const CUtensorMap* bm = &maps.b[it.job][kGateTile && Cg == 2 ? static_cast<int>(rank) : t];
             for (int kb = low; kb < high; kb += p.slot_blocks) {
               if (!mbar_wait_bounded(&empty[slot], phase ^ 1, p.status, FHB_STATUS_MMA_TIMEOUT)) {
                 ok = false;
                 break;
               }
               const int blocks = min(p.slot_blocks, high - kb);
-              if (rank == 0) mbar_arrive_expect_tx(&full[slot], bytes * blocks);
+              if (rank == 0) mbar_arrive_expect_tx(&full[slot], Cg * block_bytes * blocks);
               const uint32_t bar = first_bar + slot * 8;
               for (int j = 0; j < blocks; ++j) {
                 const uint32_t at = ring + slot * slot_bytes + j * block_bytes;
                 const uint32_t bt = at + kCopies * a_tile_bytes;
                 const int k0 = (kb + j) * kKBlock;
-                if (p.a_k_major) {
+                if (a_k_major) {
                   copy_tile<Cg>(at, am, k0, a0, 0, bar);
                 } else {
                   copy_tile<Cg>(at, am, a0, k0, 0, bar);
@@ -488,11 +501,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (kGateTile && Cg == 1) {
                   // half of the columns from each weight; FP32: plane by plane, so that the
                   // halves of a plane are neighbours
-                  for (int q = 0; q < kCopies; ++q) {
-                    copy_tile<Cg>(bt + q * b_tile_bytes, &maps.b[0], k0, b0, q, bar);
-                    copy_tile<Cg>(bt + q * b_tile_bytes + b_tile_bytes / 2, &maps.b[1], k0, b0, q, bar);
+                  for (int z = 0; z < kCopies; ++z) {
+                    copy_tile<Cg>(bt + z * b_tile_bytes, &maps.b[0][0], k0, b0, z, bar);
+                    copy_tile<Cg>(bt + z * b_tile_bytes + b_tile_bytes / 2, &maps.b[0][1], k0, b0, z, bar);
                   }
-                } else if (p.b_k_major) {
+                } else if (b_k_major) {
                   copy_tile<Cg>(bt, bm, k0, b0, 0, bar);
                 } else {
                   for (int i = 0; i < b_rows; i += 64)
@@ -525,13 +538,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t phase = 0;
       int64_t sums = 0;
       bool ok = true;
-      const uint32_t a_step = p.a_k_major ? 2 : 128, b_step = p.b_k_major ? 2 : 128;  // 16 of K
-      // bytes from plane to plane and (operand across K) from one block of 64 rows to the next
-      const uint32_t a_plane = p.a_k_major ? a_tile_bytes : 8192;
-      const uint32_t b_plane = p.b_k_major ? b_tile_bytes : 8192;
+      // (operand across K: bytes from one block of 64 rows to the next)
       const uint64_t a_desc = tile_descriptor(0, kCopies * 8192), b_desc = a_desc;
       for (uint32_t index = first; ok && index < items; index += stride) {
         const Item it = item_at<Cg, kGateTile>(p, index);
+        const Job& q = p.job[it.job];
+        const uint32_t a_step = q.a_k_major ? 2 : 128, b_step = q.b_k_major ? 2 : 128;  // 16 of K
+        const uint32_t a_tile_bytes = static_cast<uint32_t>(q.a_rows) * kKBlock * 2;
+        const uint32_t block_bytes = kCopies * (a_tile_bytes + b_tile_bytes);
+        // bytes from plane to plane
+        const uint32_t a_plane = q.a_k_major ? a_tile_bytes : 8192;
+        const uint32_t b_plane = q.b_k_major ? b_tile_bytes : 8192;
+        const uint32_t idesc = q.idesc;
+        const int sum_terms = q.sum_terms;
         const int chunks = chunk_count<T>(it.blocks);
         for (int c = 0; ok && c < chunks; ++c, ++sums) {
           const int low = kChunked ? c * kChunkBlocks : 0;
@@ -543,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::fence_after_sync();
           const uint32_t d = tmem + buffer * kMaxColumns;
           uint32_t accumulate = 0;
-          for (int t = 0; ok && t < p.sum_terms; ++t)
+          for (int t = 0; ok && t < sum_terms; ++t)
             for (int kb = 0; kb < blocks; kb += p.slot_blocks) {
               ok = mbar_wait_bounded(&full[slot], phase, p.status, FHB_STATUS_MMA_TIMEOUT);
               if (!ok) break;
@@ -555,18 +574,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint64_t a1 = a0 + (a_plane >> 4), b1 = b0 + (b_plane >> 4);
                 const uint64_t a2 = a1 + (a_plane >> 4), b2 = b1 + (b_plane >> 4);
                 const uint32_t small = d + kSmallColumns;
-                mma_slot<Cg>(small, a2, b0, a_step, b_step, p.idesc, accumulate);
-                mma_slot<Cg>(d, a0, b0, a_step, b_step, p.idesc, accumulate);
-                mma_slot<Cg>(small, a0, b2, a_step, b_step, p.idesc, 1);
-                mma_slot<Cg>(small, a1, b1, a_step, b_step, p.idesc, 1);
-                mma_slot<Cg>(small, a1, b0, a_step, b_step, p.idesc, 1);
-                mma_slot<Cg>(small, a0, b1, a_step, b_step, p.idesc, 1);
+                mma_slot<Cg>(small, a2, b0, a_step, b_step, idesc, accumulate);
+                mma_slot<Cg>(d, a0, b0, a_step, b_step, idesc, accumulate);
+                mma_slot<Cg>(small, a0, b2, a_step, b_step, idesc, 1);
+                mma_slot<Cg>(small, a1, b1, a_step, b_step, idesc, 1);
+                mma_slot<Cg>(small, a1, b0, a_step, b_step, idesc, 1);
+                mma_slot<Cg>(small, a0, b1, a_step, b_step, idesc, 1);
                 accumulate = 1;
               } else {
                 const int here = min(p.slot_blocks, blocks - kb);
                 uint64_t a0 = a_desc | (at >> 4), b0 = b_desc | ((at + a_tile_bytes) >> 4);
                 for (int j = 0; j < here; ++j) {
-                  mma_slot<Cg>(d, a0, b0, a_step, b_step, p.idesc, accumulate);
+                  mma_slot<Cg>(d, a0, b0, a_step, b_step, idesc, accumulate);
                   accumulate = 1;
                   a0 += block_bytes >> 4;
                   b0 += block_bytes >> 4;
@@ -591,6 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (uint32_t index = first; ok && index < items; index += stride) {
       const Item it = item_at<Cg, kGateTile>(p, index);
+      const Job& q = p.job[it.job];
       const int chunks = chunk_count<T>(it.blocks);
       const int64_t row = it.m0 + rank * kRows + quadrant * 32 + lane;
       const auto release_sums = [&](int buffer) {
@@ -640,29 +660,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         FactorWords<T> f1, f2;
         const auto prefetch = [&](int group) {
           const int64_t n0 = it.n0 + 32 * (quarter + 4 * (group / 2)) + 16 * (group % 2);
-          if (row >= p.m || n0 >= p.n) return;
+          if (row >= q.m || n0 >= q.n) return;
           const int64_t place = (row * p.factors.groups + n0 / kFactorGroup) * 2;
           load_factors<T>(p.factors, place, f1);
           load_factors<T>(p.factors, place + 1, f2);
         };
         const auto finish = [&](int group, const float (&v)[kGroup]) {
           const int64_t n0 = it.n0 + 32 * (quarter + 4 * (group / 2)) + 16 * (group % 2);
-          if (n0 >= p.n) return;
+          if (n0 >= q.n) return;
 #pragma unroll
           for (int which = 0; which < 2; ++which) {  // dg = dh f2, then du = dh f1
             float d[kGroup];
             times_factors<T>(which == 0 ? f2 : f1, v, d);
-            if (row < p.m)
+            if (row < q.m)
               store_operand<T>(p.gated[which] + row * p.gated_stride + n0, p.gated_plane, d);
             if (p.row_sums == nullptr) continue;
-            if (row >= p.m) {
+            if (row >= q.m) {
 #pragma unroll
               for (int i = 0; i < kGroup; ++i) d[i] = 0.0f;
             }
             __syncwarp();
             const float sum = sum_rows(d, lane);
             const int64_t rows = it.m0 + rank * kRows + quadrant * 32;
-            if (rows < p.m && lane < kGroup) p.row_sums[(rows / 32 * 2 + which) * p.row_sums_stride + n0 + lane] = sum;
+            if (rows < q.m && lane < kGroup) p.row_sums[(rows / 32 * 2 + which) * p.row_sums_stride + n0 + lane] = sum;
           }
         };
         const int groups = quarter < pairs ? 2 * ((pairs - quarter + 3) / 4) : 0;
@@ -701,12 +721,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         // two groups of 16 columns at a time: a gate tile's g and u, else neighbours
         const auto finish = [&](int pair, float (&v0)[kGroup], float (&v1)[kGroup]) {
-          if (row >= p.m) return;
+          if (row >= q.m) return;
           if constexpr (kGateTile) {
             const int64_t n0 = it.n0 + 16 * pair;
-            if (n0 >= p.n) return;
-            add_bias<T>(p.bias[0], n0, p.n, v0);
-            add_bias<T>(p.bias[1], n0, p.n, v1);
+            if (n0 >= q.n) return;
+            add_bias<T>(q.bias[0], n0, q.n, v0);
+            add_bias<T>(q.bias[1], n0, q.n, v1);
             float h[kGroup];
             const auto gate = [&](auto tanh) {
 #pragma unroll
@@ -731,13 +751,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 2; ++j) {
               float(&v)[kGroup] = j == 0 ? v0 : v1;
               const int64_t n0 = it.n0 + 32 * pair + 16 * j;
-              if (n0 >= p.n) break;
-              if constexpr (E == TcEpilogue::kPartial) {
-                float* out = p.partial + ((static_cast<int64_t>(it.group) * p.parts + it.part) * p.m + row) * p.partial_stride;
-                store_results<float>(out, n0, p.partial_stride, true, v);
+              if (n0 >= q.n) break;
+              if (q.partial != nullptr) {
+                float* out = q.partial + ((static_cast<int64_t>(it.group) * q.parts + it.part) * q.m + row) * q.partial_stride;
+                store_results<float>(out, n0, q.partial_stride, true, v);
               } else {
-                add_bias<T>(p.bias[0], n0, p.n, v);
-                store_results<T>(static_cast<T*>(p.out[it.group]) + row * p.out_stride, n0, p.n, p.out_wide != 0, v);
+                add_bias<T>(q.bias[0], n0, q.n, v);
+                store_results<T>(static_cast<T*>(q.out[it.group]) + row * q.out_stride, n0, q.n, q.out_wide != 0, v);
               }
             }
           }
@@ -768,42 +788,45 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kEpilogueWarps) free_tmem<Cg>(tmem);
 }
 
-// out[m][n] = the sum of the parts in order + bias[n]; one group of the product per blockIdx.y.
-template <typename T>
-struct Outputs {
-  T* group[2];
+// out[m][n] = the sum of the parts in order + bias[n]; one group of a product per blockIdx.y.
+struct Parts {
+  const float* partial;
+  int64_t part_values, stride, m, n, out_stride;
+  int parts;
+  const void* bias;
+  void* out;
+};
+struct PartsList {
+  Parts of[2 * kTcMaxProducts];
 };
 template <typename T>
-__global__ void __launch_bounds__(256)
-    add_parts_kernel(const float* __restrict__ partial, int64_t part_values, int64_t stride, int parts,
-                     int64_t m, int64_t n, const T* __restrict__ bias, Outputs<T> outputs,
-                     int64_t out_stride) {
+__global__ void __launch_bounds__(256) add_parts_kernel(const __grid_constant__ PartsList list) {
   allow_dependents();
   wait_for_prerequisites();
-  const int64_t quads = stride / 4, step = part_values / 4;
-  T* const out = outputs.group[blockIdx.y];
-  partial += blockIdx.y * parts * part_values;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < m * quads; i += gridDim.x * 256ll) {
+  const Parts& p = list.of[blockIdx.y];
+  const int64_t quads = p.stride / 4, step = p.part_values / 4;
+  const T* const bias = static_cast<const T*>(p.bias);
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < p.m * quads; i += gridDim.x * 256ll) {
     const int64_t row = i / quads, c = (i - row * quads) * 4;
-    const float4* src = reinterpret_cast<const float4*>(partial + row * stride + c);
+    const float4* src = reinterpret_cast<const float4*>(p.partial + row * p.stride + c);
     float4 s = src[0];
     int k = 1;
-    for (; k + 4 <= parts; k += 4) {  // four parts in flight
+    for (; k + 4 <= p.parts; k += 4) {  // four parts in flight
       float4 v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = src[(k + j) * step];
 #pragma unroll
       for (int j = 0; j < 4; ++j) s = make_float4(s.x + v[j].x, s.y + v[j].y, s.z + v[j].z, s.w + v[j].w);
     }
-    for (; k < parts; ++k) {
+    for (; k < p.parts; ++k) {
       const float4 v = src[k * step];
       s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
     }
     const float v[4] = {s.x, s.y, s.z, s.w};
+    T* const out = static_cast<T*>(p.out) + row * p.out_stride + c;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (c + j < n)
-        out[row * out_stride + c + j] = from_float<T>(v[j] + (bias != nullptr ? to_float(bias[c + j]) : 0.0f));
+      if (c + j < p.n) out[j] = from_float<T>(v[j] + (bias != nullptr ? to_float(bias[c + j]) : 0.0f));
   }
 }
 
@@ -856,10 +879,17 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJ
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 int64_t blocks_of(int64_t x, int64_t size) { return (x + size - 1) / size; }
 
-// ---- the plan of a product: tile, pairing, parts of K ----
-struct Plan {
-  int cg, columns, a_rows, parts, part_blocks, k_blocks, tiles_m, tiles_n, slots, slot_blocks, grid;
+// ---- the plan of a launch: tile, pairing, each product's parts of K ----
+struct JobPlan {
+  int a_rows, parts, part_blocks, k_blocks, tiles_m, tiles_n;
   int64_t partial_stride;
+};
+struct Plan {
+  int cg, columns, slots, slot_blocks, slot_bytes, grid;
+  bool cut_rows;  // some A tile has fewer than 128 rows
+  int64_t items;
+  double cycles;  // the estimate
+  JobPlan job[kTcMaxProducts];
 };
 // Bytes of the ring that one block of K takes.
 int block_bytes_of(bool wide, int cg, int columns, int a_rows) {
@@ -870,61 +900,91 @@ int block_bytes_of(bool wide, int cg, int columns, int a_rows) {
 // cycles a product of planes, the same in a pair with half the B tile each) or the copies of its
 // bytes (about 64 a cycle), whichever is longer; an item costs about 2,000 cycles more (its
 // first copies, its last results), and a second launch that adds the parts about 3,000 and its
-// bytes. So a few tokens get tiles as narrow as still fill one
-// round of the SMs (48 x 2048 x 5632 bf16, first product: 14.1 us with 118 tiles of 96 columns,
-// 14.6 with 88 of 128, 19.7 with 176 of 64).
-Plan plan_of(const TcProduct& p, const DeviceInfo& dev) {
-  const bool wide = p.dtype == FHB_DTYPE_F32, gate = p.epilogue == TcEpilogue::kGate;
-  const int k_blocks = static_cast<int>(blocks_of(p.k, kKBlock));
-  const int64_t n_columns = gate ? 2 * p.n : p.n;
-  // an operand across K comes in blocks of 64 rows
-  const int a_rows = p.a_k_major ? static_cast<int>(std::min<int64_t>(kRows, round_up(p.m, 8))) : kRows;
+// bytes. So a few tokens get tiles as narrow as still fill one round of the SMs (48 x 2048 x 5632
+// bf16, first product: 14.1 us with 118 tiles of 96 columns, 14.6 with 88 of 128, 19.7 with 176
+// of 64), and products that share a launch are cut so that no item is long against the launch.
+Plan plan_of(const TcProduct* products, int count, const DeviceInfo& dev) {
+  const bool wide = products[0].dtype == FHB_DTYPE_F32, gate = products[0].epilogue == TcEpilogue::kGate;
+  const bool parted = products[0].epilogue == TcEpilogue::kStore;
   Plan best{};
   double least = 0.0;
   for (int cg = 1; cg <= 2; ++cg)
     for (const int columns : {64, 96, 128, 192, 256}) {
-      if (columns > (wide ? kSmallColumns : kMaxColumns) || (cg == 2 && (columns < 128 || p.m <= kRows))) continue;
-      if (!p.b_k_major && columns / cg % 64 != 0) continue;  // an operand across K comes in blocks of 64
-      const int64_t tiles_m = blocks_of(p.m, kRows * cg);
-      const int64_t tiles_n = blocks_of(n_columns, columns);
-      const int64_t tiles = tiles_m * tiles_n * p.groups;
+      bool fits = columns <= (wide ? kSmallColumns : kMaxColumns) && (cg == 1 || columns >= 128);
+      for (int i = 0; i < count; ++i) {
+        // an operand across K comes in blocks of 64
+        if (!products[i].b_k_major && columns / cg % 64 != 0) fits = false;
+        if (cg == 2 && products[i].m <= kRows) fits = false;
+      }
+      if (!fits) continue;
       const int64_t units = dev.sms / cg;
-      const double mma = 2.0 * columns * (wide ? 6 : 1);
-      const double block = p.sum_terms * std::max(mma, block_bytes_of(wide, cg, columns, a_rows) / 64.0);
-      // one to four parts, or as many as fill one or two rounds of the SMs
-      for (int choice = 1; choice <= (p.epilogue == TcEpilogue::kStore ? 6 : 1); ++choice) {
-        const int64_t wanted = choice <= 4 ? choice : std::min<int64_t>(units * (choice - 4) / tiles, 128);
-        if (choice > 4 && wanted <= 4) continue;
-        const int part_blocks = static_cast<int>(blocks_of(k_blocks, wanted));
-        const int parts = static_cast<int>(blocks_of(k_blocks, part_blocks));
-        double cycles = static_cast<double>(blocks_of(tiles * parts, units)) * (2000.0 + part_blocks * block);
-        if (parts > 1)
-          cycles += 3000.0 + 8.0 * static_cast<double>(p.m) * n_columns * p.groups * parts / (64.0 * dev.sms);
+      Plan plan{};
+      plan.cg = cg;
+      plan.columns = columns;
+      double block[kTcMaxProducts], whole = 0.0;
+      int64_t tiles[kTcMaxProducts];
+      for (int i = 0; i < count; ++i) {
+        const TcProduct& p = products[i];
+        JobPlan& j = plan.job[i];
+        j.a_rows = p.a_k_major ? static_cast<int>(std::min<int64_t>(kRows, round_up(p.m, 8))) : kRows;
+        j.k_blocks = static_cast<int>(blocks_of(p.k, kKBlock));
+        j.tiles_m = static_cast<int>(blocks_of(p.m, kRows * cg));
+        j.tiles_n = static_cast<int>(blocks_of(gate ? 2 * p.n : p.n, columns));
+        j.partial_stride = round_up(p.n, 32);
+        tiles[i] = static_cast<int64_t>(j.tiles_m) * j.tiles_n * p.groups;
+        block[i] = p.sum_terms * std::max(2.0 * columns * (wide ? 6 : 1),
+                                          block_bytes_of(wide, cg, columns, j.a_rows) / 64.0);
+        whole += static_cast<double>(tiles[i]) * (2000.0 + j.k_blocks * block[i]) / static_cast<double>(units);
+      }
+      for (int choice = 1; choice <= (parted ? 6 : 1); ++choice) {
+        double cycles = 0.0, longest = 0.0, added = 0.0;
+        plan.items = 0;
+        for (int i = 0; i < count; ++i) {
+          const TcProduct& p = products[i];
+          JobPlan& j = plan.job[i];
+          int64_t wanted;
+          if (count == 1)  // one to four parts, or as many as fill one or two rounds of the SMs
+            wanted = choice <= 4 ? choice : units * (choice - 4) / tiles[0];
+          else  // items of at most the whole, a half, ... a fifth of it; or no parts
+            wanted = choice == 6 ? 1 : static_cast<int64_t>(j.k_blocks * block[i] * choice / whole) + 1;
+          wanted = std::min<int64_t>(std::max<int64_t>(wanted, 1), 128);
+          j.part_blocks = static_cast<int>(blocks_of(j.k_blocks, wanted));
+          j.parts = static_cast<int>(blocks_of(j.k_blocks, j.part_blocks));
+          const double item = 2000.0 + j.part_blocks * block[i];
+          const int64_t items = tiles[i] * j.parts;
+          plan.items += items;
+          cycles += count == 1 ? static_cast<double>(blocks_of(items, units)) * item
+                               : static_cast<double>(items) * item / static_cast<double>(units);
+          longest = std::max(longest, item);
+          if (j.parts > 1)
+            added += 8.0 * static_cast<double>(p.m) * j.partial_stride * p.groups * j.parts / (64.0 * dev.sms);
+        }
+        if (count > 1) cycles += 0.5 * longest;
+        if (added > 0.0) cycles += 3000.0 + added;
         if (least == 0.0 || cycles < least) {
           least = cycles;
-          best.cg = cg;
-          best.columns = columns;
-          best.parts = parts;
-          best.part_blocks = part_blocks;
-          best.tiles_m = static_cast<int>(tiles_m);
-          best.tiles_n = static_cast<int>(tiles_n);
-          best.grid = static_cast<int>(std::min<int64_t>(tiles * parts, units)) * cg;
+          best = plan;
+          best.cycles = cycles;
         }
       }
     }
-  best.k_blocks = k_blocks;
-  best.a_rows = a_rows;
-  const int block_bytes = block_bytes_of(wide, best.cg, best.columns, a_rows);
-  const int room = kRingBytes - (a_rows < kRows ? kATileBytes : 0);  // an MMA reads past the last rows
+  int block_bytes = 0, part_blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    const JobPlan& j = best.job[i];
+    block_bytes = std::max(block_bytes, block_bytes_of(wide, best.cg, best.columns, j.a_rows));
+    part_blocks = std::max(part_blocks, j.part_blocks);
+    best.cut_rows = best.cut_rows || j.a_rows < kRows;
+  }
+  const int room = kRingBytes - (best.cut_rows ? kATileBytes : 0);  // an MMA reads past the last rows
   // blocks of K a slot: two halve the waits between MMAs, where at least three slots remain; four
   // in narrow tiles, whose time is that of reading the weights: DRAM then gives 512 bytes of a
   // row together (48 x 2048 x 5632 bf16, 64 columns: 31, 23 and 20 us with 1, 2 and 4)
   best.slot_blocks = 1;
   for (const int blocks : {2, 4})
-    if (!wide && best.part_blocks >= blocks && (blocks == 2 || best.columns < 128) && room / (blocks * block_bytes) >= 3)
+    if (!wide && part_blocks >= blocks && (blocks == 2 || best.columns < 128) && room / (blocks * block_bytes) >= 3)
       best.slot_blocks = blocks;
-  best.slots = std::min(kMaxSlots, room / (best.slot_blocks * block_bytes));
-  best.partial_stride = round_up(p.n, 32);
+  best.slot_bytes = best.slot_blocks * block_bytes;
+  best.slots = std::min(kMaxSlots, room / best.slot_bytes);
   return best;
 }
 
@@ -955,10 +1015,8 @@ bool tile_map(const TcMatrix& x, int box_rows, int box_planes, CUtensorMap* out)
   return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && encode();
 }
 
-size_t smem_bytes(const Plan& plan, bool wide) {
-  return static_cast<size_t>(plan.slots) * plan.slot_blocks *
-             block_bytes_of(wide, plan.cg, plan.columns, plan.a_rows) +
-         (plan.a_rows < kRows ? kATileBytes : 0) + 1024;
+size_t smem_bytes(const Plan& plan) {
+  return static_cast<size_t>(plan.slots) * plan.slot_bytes + (plan.cut_rows ? kATileBytes : 0) + 1024;
 }
 
 template <int Cg, TcEpilogue E, typename T>
@@ -979,7 +1037,7 @@ cudaError_t launch(const Maps& maps, const Args& args, const Plan& plan, bool de
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(plan.grid);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem_bytes(plan, sizeof(T) == 4);
+  cfg.dynamicSmemBytes = smem_bytes(plan);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = attrs;
@@ -1005,17 +1063,6 @@ cudaError_t prepare_kind() {
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes + 1024);
 }
 
-template <typename T>
-cudaError_t add_parts(const TcProduct& p, const Plan& plan, const float* partial, const DeviceInfo& dev,
-                      cudaStream_t stream) {
-  const int64_t values = p.m * plan.partial_stride;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks_of(values / 4, 256), 8ll * dev.sms)), p.groups);
-  return launch_dependent(
-      add_parts_kernel<T>, grid, dim3(256), 0, stream, partial, values, plan.partial_stride,
-      plan.parts, p.m, p.n, static_cast<const T*>(p.bias[0]),
-      Outputs<T>{{static_cast<T*>(p.out[0]), static_cast<T*>(p.out[1])}}, p.out_stride);
-}
-
 }  // namespace
 
 cudaError_t prepare_gemm_tc() {
@@ -1027,84 +1074,116 @@ cudaError_t prepare_gemm_tc() {
   if (found != cudaDriverEntryPointSuccess || entry == nullptr) return cudaErrorSymbolNotFound;
   g_encode = reinterpret_cast<EncodeTiled>(entry);
   for (auto prepare : {prepare_kind<1, TcEpilogue::kStore>, prepare_kind<2, TcEpilogue::kStore>,
-                       prepare_kind<1, TcEpilogue::kPartial>, prepare_kind<2, TcEpilogue::kPartial>,
                        prepare_kind<1, TcEpilogue::kGate>, prepare_kind<2, TcEpilogue::kGate>,
                        prepare_kind<1, TcEpilogue::kGateGrad>, prepare_kind<2, TcEpilogue::kGateGrad>})
     if ((e = prepare()) != cudaSuccess) return e;
   return cudaSuccess;
 }
 
-size_t gemm_tc_workspace_bytes(const TcProduct& p, const DeviceInfo& dev) {
-  const Plan plan = plan_of(p, dev);
-  return plan.parts == 1 ? 0 : static_cast<size_t>(plan.parts) * p.groups * p.m * plan.partial_stride * 4;
+bool gemm_tc_shares_launch(const TcProduct* products, int count, const DeviceInfo& dev) {
+  return plan_of(products, count, dev).cycles < 60000.0;  // about 35 us
 }
 
-cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, bool dependent,
+size_t gemm_tc_workspace_bytes(const TcProduct* products, int count, const DeviceInfo& dev) {
+  const Plan plan = plan_of(products, count, dev);
+  size_t bytes = 0;
+  for (int i = 0; i < count; ++i)
+    if (plan.job[i].parts > 1)
+      bytes += static_cast<size_t>(plan.job[i].parts) * products[i].groups * products[i].m *
+               plan.job[i].partial_stride * 4;
+  return bytes;
+}
+
+cudaError_t launch_gemm_tc(const TcProduct* products, int count, void* workspace, bool dependent,
                            const DeviceInfo& dev, cudaStream_t stream) {
-  const Plan plan = plan_of(p, dev);
+  Plan plan = plan_of(products, count, dev);
+  const TcProduct& p = products[0];
   const bool wide = p.dtype == FHB_DTYPE_F32, gate = p.epilogue == TcEpilogue::kGate;
+  const int planes = wide ? kPlanes : 1;
   // items are counted in 32 bits, with room for a last stride beyond them
-  if (static_cast<int64_t>(plan.tiles_m) * plan.tiles_n > 0x70000000 / (plan.parts * p.groups))
-    return cudaErrorInvalidValue;
+  if (plan.items > 0x70000000) return cudaErrorInvalidValue;
   Args args{};
-  args.m = p.m;
-  args.n = p.n;
-  args.tiles_m = plan.tiles_m;
-  args.tiles_n = plan.tiles_n;
-  args.groups = p.groups;
-  args.parts = plan.parts;
-  args.k_blocks = plan.k_blocks;
-  args.part_blocks = plan.part_blocks;
+  Maps maps{};
+  PartsList parts{};
+  int parted = 0;
+  int64_t most = 0;
+  float* partial = static_cast<float*>(workspace);
   args.columns = plan.columns;
   args.slots = plan.slots;
   args.slot_blocks = plan.slot_blocks;
-  args.sum_terms = p.sum_terms;
-  args.a_k_major = p.a_k_major;
-  args.b_k_major = p.b_k_major;
-  args.a_rows = plan.a_rows;
-  args.idesc = (1u << 4) | (1u << 7) | (1u << 10) | (p.a_k_major ? 0u : tc::kIdescAMnMajor) |
-               (p.b_k_major ? 0u : tc::kIdescBMnMajor) |
-               (static_cast<uint32_t>(plan.columns) >> 3 << 17) |
-               (static_cast<uint32_t>(kRows * plan.cg) >> 4 << 24);  // bf16 in, FP32 sums
-  for (int i = 0; i < 2; ++i) {
-    args.out[i] = p.out[i];
-    args.bias[i] = p.bias[i];
-    args.gated[i] = const_cast<bf16*>(p.gated[i].p);
+  args.slot_bytes = static_cast<uint32_t>(plan.slot_bytes);
+  uint32_t items = 0;
+  for (int i = 0; i < count; ++i) {
+    TcProduct x = products[i];
+    const JobPlan& j = plan.job[i];
+    // results that nobody wants: the plan is that of all of them, so that the others' sums are
+    // made from the same parts either way
+    if (p.epilogue == TcEpilogue::kStore) {
+      if (x.groups == 2 && x.out[0] == nullptr) x.out[0] = x.out[1], x.a[0] = x.a[1], x.out[1] = nullptr;
+      if (x.groups == 2 && x.out[1] == nullptr) x.groups = 1;
+      if (x.out[0] == nullptr) continue;
+    }
+    const int at = args.jobs++;
+    Job& q = args.job[at];
+    q.m = x.m;
+    q.n = x.n;
+    q.tiles_m = j.tiles_m;
+    q.tiles_n = j.tiles_n;
+    q.groups = x.groups;
+    q.parts = j.parts;
+    q.k_blocks = j.k_blocks;
+    q.part_blocks = j.part_blocks;
+    q.sum_terms = x.sum_terms;
+    q.a_k_major = x.a_k_major;
+    q.b_k_major = x.b_k_major;
+    q.a_rows = j.a_rows;
+    q.idesc = (1u << 4) | (1u << 7) | (1u << 10) | (x.a_k_major ? 0u : tc::kIdescAMnMajor) |
+              (x.b_k_major ? 0u : tc::kIdescBMnMajor) | (static_cast<uint32_t>(plan.columns) >> 3 << 17) |
+              (static_cast<uint32_t>(kRows * plan.cg) >> 4 << 24);  // bf16 in, FP32 sums
+    q.first_item = items;
+    items += static_cast<uint32_t>(j.tiles_m) * j.tiles_n * x.groups * j.parts;
+    q.out_stride = x.out_stride;
+    const int64_t out_bytes = x.out_stride * static_cast<int64_t>(dtype_bytes(x.dtype));
+    q.out_wide = out_bytes % 32 == 0 && reinterpret_cast<uintptr_t>(x.out[0]) % 32 == 0 &&
+                 reinterpret_cast<uintptr_t>(x.out[1]) % 32 == 0;
+    q.partial_stride = j.partial_stride;
+    const int64_t values = x.m * j.partial_stride;
+    for (int g = 0; g < 2; ++g) {
+      q.out[g] = x.out[g];
+      q.bias[g] = x.bias[g];
+      if (j.parts == 1 || g >= x.groups) continue;
+      if (g == 0) q.partial = partial;
+      parts.of[parted++] = {partial, values, j.partial_stride, x.m, x.n, x.out_stride, j.parts, x.bias[0], x.out[g]};
+      partial += j.parts * values;
+      most = std::max(most, values);
+    }
+    const int a_box = x.a_k_major ? j.a_rows : kKBlock;
+    const int b_box = !x.b_k_major ? kKBlock : gate ? plan.columns / 2 : plan.columns / plan.cg;
+    for (int t = 0; t < 2; ++t)
+      if (!tile_map(x.a[x.a[t].p != nullptr ? t : 0], a_box, planes, &maps.a[at][t]) ||
+          !tile_map(x.b[x.b[t].p != nullptr ? t : 0], b_box, gate && plan.cg == 1 ? 1 : planes, &maps.b[at][t]))
+        return cudaErrorInvalidValue;
   }
-  args.out_stride = p.out_stride;
-  const int64_t out_bytes = p.out_stride * static_cast<int64_t>(dtype_bytes(p.dtype));
-  args.out_wide = out_bytes % 32 == 0 && reinterpret_cast<uintptr_t>(p.out[0]) % 32 == 0 &&
-                  reinterpret_cast<uintptr_t>(p.out[1]) % 32 == 0;
+  if (items == 0) return cudaSuccess;
+  args.items = items;
+  plan.grid = static_cast<int>(std::min<int64_t>(items, dev.sms / plan.cg)) * plan.cg;
+  for (int i = 0; i < 2; ++i) args.gated[i] = const_cast<bf16*>(p.gated[i].p);
   args.gated_stride = p.gated[0].stride;
   args.gated_plane = p.gated[0].plane;
   args.factors = p.factors;
   args.activation = p.activation;
-  args.partial = static_cast<float*>(workspace);
-  args.partial_stride = plan.partial_stride;
   args.row_sums = p.row_sums;
   args.row_sums_stride = p.row_sums_stride;
   args.status = dev.status;
-
-  Maps maps{};
-  const int b_rows = plan.columns / plan.cg;
-  const int planes = wide ? kPlanes : 1;
-  const int a_box = p.a_k_major ? args.a_rows : kKBlock;
-  const int b_box = !p.b_k_major ? kKBlock : gate ? plan.columns / 2 : b_rows;
-  for (int i = 0; i < 2; ++i) {
-    if (!tile_map(p.a[p.a[i].p != nullptr ? i : 0], a_box, planes, &maps.a[i]) ||
-        !tile_map(p.b[p.b[i].p != nullptr ? i : 0], b_box, gate && plan.cg == 1 ? 1 : planes, &maps.b[i]))
-      return cudaErrorInvalidValue;
-  }
   switch (p.epilogue) {
     case TcEpilogue::kGate: return launch_kind<TcEpilogue::kGate>(wide, maps, args, plan, dependent, stream);
     case TcEpilogue::kGateGrad: return launch_kind<TcEpilogue::kGateGrad>(wide, maps, args, plan, dependent, stream);
     default: break;
   }
-  if (plan.parts == 1) return launch_kind<TcEpilogue::kStore>(wide, maps, args, plan, dependent, stream);
-  const cudaError_t e = launch_kind<TcEpilogue::kPartial>(wide, maps, args, plan, dependent, stream);
-  if (e != cudaSuccess) return e;
-  return wide ? add_parts<float>(p, plan, args.partial, dev, stream)
-              : add_parts<bf16>(p, plan, args.partial, dev, stream);
+  const cudaError_t e = launch_kind<TcEpilogue::kStore>(wide, maps, args, plan, dependent, stream);
+  if (e != cudaSuccess || parted == 0) return e;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks_of(most / 4, 256), 8ll * dev.sms)), parted);
+  return launch_dependent(wide ? add_parts_kernel<float> : add_parts_kernel<bf16>, grid, dim3(256), 0, stream, parts);
 }
 
 namespace {

@@ -21,8 +21,8 @@ struct TcMatrix {
 
 // What a product does with its sums.
 enum class TcEpilogue {
-  kStore,     // out[m][n] = sum + bias[n], in the output type
-  kPartial,   // FP32 sums of one part of K into the workspace (added up by a second kernel)
+  kStore,     // out[m][n] = sum + bias[n], in the output type (or FP32 sums of one part of K into
+              // the workspace, added up by a second kernel)
   kGate,      // two products g, u side by side: h = act(g) u, and what the backward needs
   kGateGrad,  // the gradients of g and u from that of h
 };
@@ -61,12 +61,20 @@ struct TcProduct {
   int64_t row_sums_stride = 0;
 };
 
-// Workspace of a product: the FP32 partial sums of its parts of K (0 where it has one).
-size_t gemm_tc_workspace_bytes(const TcProduct& p, const DeviceInfo& dev);
+// Products of one launch: their tiles share its rounds of the SMs. More than one: all kStore; one
+// whose outputs are null is left out of the launch, though not of its plan.
+constexpr int kTcMaxProducts = 3;
+// Whether products go into one launch: short ones do (training passes, us: 1,000 x 201 x 533 fp32
+// 87 apart and 67 together, 1,024 x 512 x 2048 bf16 76 and 64); for long ones it makes no
+// difference (4,096 x 1024 x 4096) or loses a little, as tiles that drift apart share less in L2
+// (16,384 x 2048 x 5632: 2,780 and 2,817).
+bool gemm_tc_shares_launch(const TcProduct* products, int count, const DeviceInfo& dev);
+// Workspace of a launch: the FP32 partial sums of the parts of K (0 where there is one of each).
+size_t gemm_tc_workspace_bytes(const TcProduct* products, int count, const DeviceInfo& dev);
 // `dependent`: launched as a dependent of the kernel before it in the stream, which has to be
 // one of this file's or gated_ffn.cu's (they wait for their own predecessors, so a chain of them
 // keeps its order; the first kernel of a call is an ordinary launch).
-cudaError_t launch_gemm_tc(const TcProduct& p, void* workspace, bool dependent,
+cudaError_t launch_gemm_tc(const TcProduct* products, int count, void* workspace, bool dependent,
                            const DeviceInfo& dev, cudaStream_t stream);
 
 // A caller's matrix: `rows` x `cols` elements of the block's type, rows `stride` apart.
