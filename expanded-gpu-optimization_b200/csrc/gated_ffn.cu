@@ -239,15 +239,6 @@ Backward backward_of(const fhb_ffn_problem& p, const Operands& o, const Saved& s
   return b;
 }
 
-// Workspace of those products: of one launch, or of three that use it one after the other.
-size_t rest_bytes(const Backward& b, const DeviceInfo& dev) {
-  if (gemm_tc_shares_launch(b.rest, kTcMaxProducts, dev))
-    return gemm_tc_workspace_bytes(b.rest, kTcMaxProducts, dev);
-  size_t most = 0;
-  for (const TcProduct& q : b.rest) most = std::max(most, gemm_tc_workspace_bytes(&q, 1, dev));
-  return most;
-}
-
 // Stands for "every gradient wanted" where sizes are asked for before the outputs exist.
 fhb_ffn_grads all_grads() {
   static char any;
@@ -257,6 +248,10 @@ fhb_ffn_grads all_grads() {
 int64_t column_part_count(const fhb_ffn_problem& p) {
   const int64_t rows = part_rows_of(p.tokens);
   return (p.tokens + rows - 1) / rows;
+}
+
+size_t column_bytes(const fhb_ffn_problem& p) {
+  return static_cast<size_t>(3 * column_part_count(p) * std::max(p.hidden, p.out_width) * 4);
 }
 
 }  // namespace
@@ -284,8 +279,8 @@ size_t ffn_workspace_bytes(const fhb_ffn_problem& p, bool backward, const Device
   Room aside{nullptr};
   const Saved s = saved_in(p, aside);
   const Backward b = backward_of(p, o, s, all_grads(), room);
-  room.take(rest_bytes(b, dev));
-  room.take(static_cast<size_t>(3 * column_part_count(p) * std::max(p.hidden, p.out_width) * 4));
+  room.take(column_bytes(p));
+  room.take(gemm_tc_workspace_bytes(b.rest, kTcMaxProducts, dev));
   return room.used;
 }
 
@@ -304,7 +299,7 @@ cudaError_t launch_ffn_forward(const fhb_ffn_problem& p, void* y, void* saved, v
   e = launch_gemm_tc(&gate, 1, nullptr, packed, dev, stream);
   if (e != cudaSuccess) return e;
   const TcProduct down = down_product(p, o, s, y);
-  return launch_gemm_tc(&down, 1, room.take(gemm_tc_workspace_bytes(&down, 1, dev)), true, dev, stream);
+  return launch_gemm_tc(&down, 1, room.take(0), true, dev, stream);
 }
 
 cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, int64_t grad_y_stride,
@@ -333,14 +328,10 @@ cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, in
   if (e != cudaSuccess) return e;
   const Saved s = saved_in(p, kept);
   const Backward b = backward_of(p, o, s, out, room);
-  void* sums = room.take(rest_bytes(b, dev));
+  float* column_parts = static_cast<float*>(room.take(column_bytes(p)));
+  void* sums = room.take(0);  // the rest
   e = launch_gemm_tc(&b.hidden, 1, nullptr, packed, dev, stream);
-  if (gemm_tc_shares_launch(b.rest, kTcMaxProducts, dev)) {
-    if (e == cudaSuccess) e = launch_gemm_tc(b.rest, kTcMaxProducts, sums, true, dev, stream);
-  } else {
-    for (const TcProduct& q : b.rest)
-      if (e == cudaSuccess) e = launch_gemm_tc(&q, 1, sums, true, dev, stream);
-  }
+  if (e == cudaSuccess) e = launch_gemm_tc(b.rest, kTcMaxProducts, sums, true, dev, stream);
   if (e != cudaSuccess) return e;
   ColumnSources columns{};
   int count = 0;
@@ -354,7 +345,7 @@ cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, in
   columns.part_rows = part_rows_of(p.tokens);
   columns.part_count = column_part_count(p);
   columns.widest = std::max(p.hidden, p.out_width);
-  columns.parts = static_cast<float*>(room.take(0));
+  columns.parts = column_parts;
   return p.dtype == FHB_DTYPE_F32 ? column_sums<float>(columns, count, stream)
                                   : column_sums<bf16>(columns, count, stream);
 }

@@ -1080,12 +1080,12 @@ cudaError_t prepare_gemm_tc() {
   return cudaSuccess;
 }
 
-bool gemm_tc_shares_launch(const TcProduct* products, int count, const DeviceInfo& dev) {
-  return plan_of(products, count, dev).cycles < 60000.0;  // about 35 us
-}
+namespace {
 
-size_t gemm_tc_workspace_bytes(const TcProduct* products, int count, const DeviceInfo& dev) {
-  const Plan plan = plan_of(products, count, dev);
+// Short products go into one launch (see gemm_tc.cuh).
+bool shares_launch(const Plan& plan) { return plan.cycles < 60000.0; }  // about 35 us
+
+size_t parts_bytes(const TcProduct* products, int count, const Plan& plan) {
   size_t bytes = 0;
   for (int i = 0; i < count; ++i)
     if (plan.job[i].parts > 1)
@@ -1094,9 +1094,8 @@ size_t gemm_tc_workspace_bytes(const TcProduct* products, int count, const Devic
   return bytes;
 }
 
-cudaError_t launch_gemm_tc(const TcProduct* products, int count, void* workspace, bool dependent,
-                           const DeviceInfo& dev, cudaStream_t stream) {
-  Plan plan = plan_of(products, count, dev);
+cudaError_t launch_planned(const TcProduct* products, int count, Plan plan, void* workspace,
+                           bool dependent, const DeviceInfo& dev, cudaStream_t stream) {
   const TcProduct& p = products[0];
   const bool wide = p.dtype == FHB_DTYPE_F32, gate = p.epilogue == TcEpilogue::kGate;
   const int planes = wide ? kPlanes : 1;
@@ -1159,10 +1158,11 @@ cudaError_t launch_gemm_tc(const TcProduct* products, int count, void* workspace
     }
     const int a_box = x.a_k_major ? j.a_rows : kKBlock;
     const int b_box = !x.b_k_major ? kKBlock : gate ? plan.columns / 2 : plan.columns / plan.cg;
-    for (int t = 0; t < 2; ++t)
-      if (!tile_map(x.a[x.a[t].p != nullptr ? t : 0], a_box, planes, &maps.a[at][t]) ||
-          !tile_map(x.b[x.b[t].p != nullptr ? t : 0], b_box, gate && plan.cg == 1 ? 1 : planes, &maps.b[at][t]))
+    for (int t = 0; t < 2; ++t) {
+      if (x.a[t].p != nullptr && !tile_map(x.a[t], a_box, planes, &maps.a[at][t])) return cudaErrorInvalidValue;
+      if (x.b[t].p != nullptr && !tile_map(x.b[t], b_box, gate && plan.cg == 1 ? 1 : planes, &maps.b[at][t]))
         return cudaErrorInvalidValue;
+    }
   }
   if (items == 0) return cudaSuccess;
   args.items = items;
@@ -1184,6 +1184,29 @@ cudaError_t launch_gemm_tc(const TcProduct* products, int count, void* workspace
   if (e != cudaSuccess || parted == 0) return e;
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks_of(most / 4, 256), 8ll * dev.sms)), parted);
   return launch_dependent(wide ? add_parts_kernel<float> : add_parts_kernel<bf16>, grid, dim3(256), 0, stream, parts);
+}
+
+}  // namespace
+
+size_t gemm_tc_workspace_bytes(const TcProduct* products, int count, const DeviceInfo& dev) {
+  const Plan plan = plan_of(products, count, dev);
+  if (count == 1 || shares_launch(plan)) return parts_bytes(products, count, plan);
+  size_t most = 0;
+  for (int i = 0; i < count; ++i) most = std::max(most, gemm_tc_workspace_bytes(products + i, 1, dev));
+  return most;
+}
+
+cudaError_t launch_gemm_tc(const TcProduct* products, int count, void* workspace, bool dependent,
+                           const DeviceInfo& dev, cudaStream_t stream) {
+  const Plan plan = plan_of(products, count, dev);
+  if (count == 1 || shares_launch(plan))
+    return launch_planned(products, count, plan, workspace, dependent, dev, stream);
+  for (int i = 0; i < count; ++i) {
+    const cudaError_t e = launch_planned(products + i, 1, plan_of(products + i, 1, dev), workspace,
+                                         dependent || i > 0, dev, stream);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 namespace {

@@ -61,15 +61,14 @@ struct TcProduct {
   int64_t row_sums_stride = 0;
 };
 
-// Products of one launch: their tiles share its rounds of the SMs. More than one: all kStore; one
-// whose outputs are null is left out of the launch, though not of its plan.
+// Products of one call, none of which needs another's result: kGate and kGateGrad alone, up to
+// three of kStore. One whose outputs are null is left out, though not of the plan. Short ones go
+// into one launch, where their tiles share its rounds of the SMs (training passes, us: 1,000 x 201
+// x 533 fp32 87 apart and 67 together, 1,024 x 512 x 2048 bf16 76 and 64); for long ones it makes
+// no difference (4,096 x 1024 x 4096) or loses a little, as tiles that drift apart share less in
+// L2 (16,384 x 2048 x 5632: 2,780 and 2,817).
 constexpr int kTcMaxProducts = 3;
-// Whether products go into one launch: short ones do (training passes, us: 1,000 x 201 x 533 fp32
-// 87 apart and 67 together, 1,024 x 512 x 2048 bf16 76 and 64); for long ones it makes no
-// difference (4,096 x 1024 x 4096) or loses a little, as tiles that drift apart share less in L2
-// (16,384 x 2048 x 5632: 2,780 and 2,817).
-bool gemm_tc_shares_launch(const TcProduct* products, int count, const DeviceInfo& dev);
-// Workspace of a launch: the FP32 partial sums of the parts of K (0 where there is one of each).
+// Workspace of a call: the FP32 partial sums of the parts of K (0 where there is one of each).
 size_t gemm_tc_workspace_bytes(const TcProduct* products, int count, const DeviceInfo& dev);
 // `dependent`: launched as a dependent of the kernel before it in the stream, which has to be
 // one of this file's or gated_ffn.cu's (they wait for their own predecessors, so a chain of them
