@@ -250,7 +250,10 @@ __device__ __forceinline__ void update_block(const fhb_adamw_tensor& t, int64_t 
     fma2o(d0, d1, v[i], v[i + 1], inverse_root, inverse_root, k.eps, k.eps);
     mul2o(w0, w1, p[i], p[i + 1], k.decay, k.decay);
     // a denominator of 0 (eps 0): 0 / 0 and x / 0 as IEEE has them
-    fma2o(p[i], p[i + 1], __fdividef(m[i], d0), __fdividef(m[i + 1], d1), -step_size, -step_size, w0, w1);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d0));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d1));
+    mul2o(d0, d1, d0, d1, m[i], m[i + 1]);
+    fma2o(p[i], p[i + 1], d0, d1, -step_size, -step_size, w0, w1);
   }
   store8(static_cast<T*>(t.param) + at, full, left, p);
   if (!Eight) return;

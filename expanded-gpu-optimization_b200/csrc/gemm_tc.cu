@@ -788,6 +788,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kEpilogueWarps) free_tmem<Cg>(tmem);
 }
 
+// i / d of non-negative numbers, in 32 bits where they fit.
+__device__ __forceinline__ int64_t quotient(int64_t i, int64_t d) {
+  return (i | d) >> 32 == 0 ? static_cast<uint32_t>(i) / static_cast<uint32_t>(d) : i / d;
+}
+
 // out[m][n] = the sum of the parts in order + bias[n]; one group of a product per blockIdx.y.
 struct Parts {
   const float* partial;
@@ -807,7 +812,7 @@ __global__ void __launch_bounds__(256) add_parts_kernel(const __grid_constant__ 
   const int64_t quads = p.stride / 4, step = p.part_values / 4;
   const T* const bias = static_cast<const T*>(p.bias);
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < p.m * quads; i += gridDim.x * 256ll) {
-    const int64_t row = i / quads, c = (i - row * quads) * 4;
+    const int64_t row = quotient(i, quads), c = (i - row * quads) * 4;
     const float4* src = reinterpret_cast<const float4*>(p.partial + row * p.stride + c);
     float4 s = src[0];
     int k = 1;
@@ -846,7 +851,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJ
   const PackJob& j = jobs.job[blockIdx.y];
   const int64_t pieces = j.stride / 8;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < j.rows * pieces; i += gridDim.x * 256ll) {
-    const int64_t row = i / pieces, c = (i % pieces) * 8;
+    const int64_t row = quotient(i, pieces), c = (i - row * pieces) * 8;
     const T* src = static_cast<const T*>(j.in) + row * j.in_stride + c;
     float v[8];
     if (sizeof(T) == 4 && c + 8 <= j.cols && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {

@@ -231,6 +231,9 @@ __global__ void __launch_bounds__(L::Most, L::Most <= 256 ? 4 : 1)
   const bool one_gate = gated && a.gate_rows >= a.rows;
   float wpre[L::V][L::Vec], wpost[L::V][L::Vec], gate[L::V][L::Vec];
   load_row<L>(static_cast<const T*>(a.pre_weight), a.width, wpre);
+  // what is not there is 1: no value's arithmetic branches
+  fill<L>(wpost, 1.0f);
+  fill<L>(gate, 1.0f);
   if (post) load_row<L>(static_cast<const T*>(a.post_weight), a.width, wpost);
   if (one_gate) load_row<L>(static_cast<const T*>(a.gate), a.width, gate);
   int round = 0;
@@ -287,10 +290,7 @@ __global__ void __launch_bounds__(L::Most, L::Most <= 256 ? 4 : 1)
     }
     float s[1] = {};
     FHB_EACH(L) {
-      float z = b[v][i];
-      if (post) z = z * ib * wpost[v][i];
-      if (gated) z *= gate[v][i];
-      t[v][i] = scale * t[v][i] + z;
+      t[v][i] = scale * t[v][i] + b[v][i] * ib * wpost[v][i] * gate[v][i];
       s[0] += t[v][i] * t[v][i];
     }
     row_sum<L>(s, round);
@@ -337,6 +337,9 @@ __global__ void __launch_bounds__(L::Most, L::Resident)
   const bool by_group = gated && units.groups > 1;
   float wpre[L::V][L::Vec], wpost[L::V][L::Vec], gate[L::V][L::Vec];
   load_row<L>(static_cast<const T*>(a.pre_weight), a.width, wpre);
+  // what is not there is 1: no value's arithmetic branches
+  fill<L>(wpost, 1.0f);
+  fill<L>(gate, 1.0f);
   if (post) load_row<L>(static_cast<const T*>(a.post_weight), a.width, wpost);
   if (gated) load_row<L>(static_cast<const T*>(a.gate), a.width, gate);
   float spre[L::V][L::Vec], spost[L::V][L::Vec], sgate[L::V][L::Vec], sscale = 0.0f;
@@ -425,9 +428,7 @@ __global__ void __launch_bounds__(L::Most, L::Resident)
       }
       float s[3] = {};
       FHB_EACH(L) {
-        float cz = b[v][i];
-        if (post) cz = cz * ib * wpost[v][i];
-        if (gated) cz *= gate[v][i];
+        const float cz = b[v][i] * ib * wpost[v][i] * gate[v][i];
         const float th = (scale * r[v][i] + cz) * it, q = dn[v][i] * wpre[v][i];
         s[0] += q * th;
         s[1] += (dT[v][i] + it * q) * cz;
@@ -439,19 +440,18 @@ __global__ void __launch_bounds__(L::Most, L::Resident)
         stage.next();
       }
       if (!real) continue;
-      const float m1 = s[0] * inverse, m2 = (s[1] - it * m1 * s[2]) * inverse;
+      const float m1 = s[0] * inverse, m2 = post ? (s[1] - it * m1 * s[2]) * inverse : 0.0f;
       FHB_EACH(L) {
-        const float bh = b[v][i] * ib, z = post ? bh * wpost[v][i] : b[v][i];
-        const float cz = gated ? gate[v][i] * z : z;
+        const float bh = b[v][i] * ib, z = bh * wpost[v][i], cz = z * gate[v][i];
         const float th = (scale * r[v][i] + cz) * it, q = dn[v][i] * wpre[v][i];
         const float dt = dT[v][i] + it * (q - th * m1);
-        const float dz = gated ? dt * gate[v][i] : dt;
+        const float dz = dt * gate[v][i];
         spre[v][i] += dn[v][i] * th;
         spost[v][i] += dz * bh;
         sgate[v][i] += dt * z;
         sscale += dt * r[v][i];
         r[v][i] = scale * dt;
-        b[v][i] = post ? ib * (dz * wpost[v][i] - bh * m2) : dz;
+        b[v][i] = ib * (dz * wpost[v][i] - bh * m2);
       }
       if (g.residual != nullptr) store_row<L>(static_cast<TR*>(g.residual) + row * a.width, a.width, r);
       if (g.branch != nullptr) store_row<L>(static_cast<T*>(g.branch) + row * a.width, a.width, b);
