@@ -30,8 +30,11 @@ constexpr int kPlanes = 3;                       // of an FP32 operand
 constexpr int kMaxOperands = 5;  // of a block's products
 constexpr int kATileBytes = kRows * kKBlock * 2;  // 16 KB: of 128 rows, all of which an MMA reads
 
+// Of a launch of Jobs products. A launch of one has its own kernels: constants at places that are
+// known when they are compiled (looked up by product, they cost large products 8%, small ones more).
+template <int Jobs>
 struct Maps {
-  CUtensorMap a[kTcMaxProducts][2], b[kTcMaxProducts][2];
+  CUtensorMap a[Jobs][2], b[Jobs][2];
 };
 
 // One product of a launch.
@@ -54,8 +57,7 @@ struct Job {
   float* partial;
   int64_t partial_stride;
 };
-struct Args {
-  Job job[kTcMaxProducts];
+struct Common {
   int jobs;
   uint32_t items;
   int columns;                // columns of a tile (both halves of a gate tile)
@@ -68,6 +70,10 @@ struct Args {
   float* row_sums;            // [32 rows][dg, du][row_sums_stride]: their column sums, or null
   int64_t row_sums_stride;
   unsigned int* status;
+};
+template <int Jobs>
+struct Args : Common {
+  Job job[Jobs];
 };
 
 // ---- PTX pieces that the other kernels' header does not have ----
@@ -372,19 +378,25 @@ __device__ __forceinline__ float sum_rows(const float (&v)[kGroup], int lane) {
   return s[0] + __shfl_xor_sync(0xffffffffu, s[0], 16);
 }
 
+template <int Jobs>
+__device__ __forceinline__ const Job& job_of(const Args<Jobs>& p, int job) {
+  return p.job[Jobs == 1 ? 0 : job];
+}
+
 // One item of work: a tile of one group's result of a product, and one part of K.
 struct Item {
   int job, group, part, first_block, blocks;
   int64_t m0, n0;  // first row of the tile (of the pair), first column (gate: feature)
 };
 // (32-bit divisions: there are fewer than 2^31 items, and 64-bit ones took 3,000 cycles an item)
-template <int Cg, bool Gate>
-__device__ __forceinline__ Item item_at(const Args& p, uint32_t index) {
+template <int Cg, bool Gate, int Jobs>
+__device__ __forceinline__ Item item_at(const Args<Jobs>& p, uint32_t index) {
   Item it;
   it.job = 0;
-  while (it.job + 1 < p.jobs && index >= p.job[it.job + 1].first_item) ++it.job;
-  const Job& q = p.job[it.job];
-  index -= q.first_item;
+  if constexpr (Jobs > 1)
+    while (it.job + 1 < p.jobs && index >= p.job[it.job + 1].first_item) ++it.job;
+  const Job& q = job_of(p, it.job);
+  if constexpr (Jobs > 1) index -= q.first_item;
   const uint32_t tiles = static_cast<uint32_t>(q.tiles_m) * static_cast<uint32_t>(q.tiles_n);
   const uint32_t rest = index / tiles;
   uint32_t tile = index - rest * tiles;
@@ -415,9 +427,9 @@ __device__ __forceinline__ int chunk_count(int blocks) {
   return sizeof(T) == 4 ? (blocks + kChunkBlocks - 1) / kChunkBlocks : 1;
 }
 
-template <int Cg, TcEpilogue E, typename T>
+template <int Cg, TcEpilogue E, typename T, int Jobs>
 __global__ void __launch_bounds__(kThreads, 1)
-    gemm_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
+    gemm_tc_kernel(const __grid_constant__ Maps<Jobs> maps, const __grid_constant__ Args<Jobs> p) {
   constexpr bool kGateTile = E == TcEpilogue::kGate;
   constexpr bool kChunked = sizeof(T) == 4;
   constexpr int kCopies = kChunked ? kPlanes : 1;  // planes that come with one copy
@@ -465,8 +477,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int64_t issued = 0;
       const uint32_t first_bar = Cg == 2 ? in_cta(smem_u32(&full[0]), 0) : smem_u32(&full[0]);
       for (uint32_t index = first; ok && index < items; index += stride) {
-        const Item it = item_at<Cg, kGateTile>(p, index);
-        const Job& q = p.job[it.job];
+        const Item it = item_at<Cg, kGateTile, Jobs>(p, index);
+        const Job& q = job_of(p, it.job);
         const uint32_t a_tile_bytes = static_cast<uint32_t>(q.a_rows) * kKBlock * 2;
         const uint32_t block_bytes = kCopies * (a_tile_bytes + b_tile_bytes);  // of one block of K
         const bool a_k_major = q.a_k_major != 0, b_k_major = q.b_k_major != 0;
@@ -478,8 +490,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int high = kChunked ? min(low + kChunkBlocks, it.first_block + it.blocks)
                                     : it.first_block + it.blocks;
           for (int t = 0; ok && t < q.sum_terms; ++t) {
-            const CUtensorMap* am = &maps.a[it.job][q.groups == 2 ? it.group : t];
-            const CUtensorMap* bm = &maps.b[it.job][kGateTile && Cg == 2 ? static_cast<int>(rank) : t];
+            const CUtensorMap* am = &maps.a[Jobs == 1 ? 0 : it.job][q.groups == 2 ? it.group : t];
+            const CUtensorMap* bm = &maps.b[Jobs == 1 ? 0 : it.job][kGateTile && Cg == 2 ? static_cast<int>(rank) : t];
             for (int kb = low; kb < high; kb += p.slot_blocks) {
               if (!mbar_wait_bounded(&empty[slot], phase ^ 1, p.status, FHB_STATUS_MMA_TIMEOUT)) {
                 ok = false;
@@ -541,8 +553,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // (operand across K: bytes from one block of 64 rows to the next)
       const uint64_t a_desc = tile_descriptor(0, kCopies * 8192), b_desc = a_desc;
       for (uint32_t index = first; ok && index < items; index += stride) {
-        const Item it = item_at<Cg, kGateTile>(p, index);
-        const Job& q = p.job[it.job];
+        const Item it = item_at<Cg, kGateTile, Jobs>(p, index);
+        const Job& q = job_of(p, it.job);
         const uint32_t a_step = q.a_k_major ? 2 : 128, b_step = q.b_k_major ? 2 : 128;  // 16 of K
         const uint32_t a_tile_bytes = static_cast<uint32_t>(q.a_rows) * kKBlock * 2;
         const uint32_t block_bytes = kCopies * (a_tile_bytes + b_tile_bytes);
@@ -609,8 +621,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int64_t sums = 0;
     bool ok = true;
     for (uint32_t index = first; ok && index < items; index += stride) {
-      const Item it = item_at<Cg, kGateTile>(p, index);
-      const Job& q = p.job[it.job];
+      const Item it = item_at<Cg, kGateTile, Jobs>(p, index);
+      const Job& q = job_of(p, it.job);
       const int chunks = chunk_count<T>(it.blocks);
       const int64_t row = it.m0 + rank * kRows + quadrant * 32 + lane;
       const auto release_sums = [&](int buffer) {
@@ -1024,8 +1036,9 @@ size_t smem_bytes(const Plan& plan) {
   return static_cast<size_t>(plan.slots) * plan.slot_bytes + (plan.cut_rows ? kATileBytes : 0) + 1024;
 }
 
-template <int Cg, TcEpilogue E, typename T>
-cudaError_t launch(const Maps& maps, const Args& args, const Plan& plan, bool dependent, cudaStream_t stream) {
+template <int Cg, TcEpilogue E, typename T, int Jobs>
+cudaError_t launch(const Maps<Jobs>& maps, const Args<Jobs>& args, const Plan& plan, bool dependent,
+                   cudaStream_t stream) {
   cudaLaunchAttribute attr[2];
   int attrs = 0;
   if (Cg == 2) {
@@ -1046,12 +1059,12 @@ cudaError_t launch(const Maps& maps, const Args& args, const Plan& plan, bool de
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = attrs;
-  return cudaLaunchKernelEx(&cfg, gemm_tc_kernel<Cg, E, T>, maps, args);
+  return cudaLaunchKernelEx(&cfg, gemm_tc_kernel<Cg, E, T, Jobs>, maps, args);
 }
 
-template <TcEpilogue E>
-cudaError_t launch_kind(bool wide, const Maps& maps, const Args& args, const Plan& plan, bool dependent,
-                        cudaStream_t stream) {
+template <TcEpilogue E, int Jobs>
+cudaError_t launch_kind(bool wide, const Maps<Jobs>& maps, const Args<Jobs>& args, const Plan& plan,
+                        bool dependent, cudaStream_t stream) {
   if (wide)
     return plan.cg == 2 ? launch<2, E, float>(maps, args, plan, dependent, stream)
                         : launch<1, E, float>(maps, args, plan, dependent, stream);
@@ -1059,13 +1072,17 @@ cudaError_t launch_kind(bool wide, const Maps& maps, const Args& args, const Pla
                       : launch<1, E, bf16>(maps, args, plan, dependent, stream);
 }
 
-template <int Cg, TcEpilogue E>
+template <TcEpilogue E, int Jobs>
 cudaError_t prepare_kind() {
-  const cudaError_t e = cudaFuncSetAttribute(gemm_tc_kernel<Cg, E, float>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes + 1024);
-  return e != cudaSuccess ? e
-                          : cudaFuncSetAttribute(gemm_tc_kernel<Cg, E, bf16>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes + 1024);
+  const void* const kernels[] = {reinterpret_cast<const void*>(gemm_tc_kernel<1, E, float, Jobs>),
+                                 reinterpret_cast<const void*>(gemm_tc_kernel<2, E, float, Jobs>),
+                                 reinterpret_cast<const void*>(gemm_tc_kernel<1, E, bf16, Jobs>),
+                                 reinterpret_cast<const void*>(gemm_tc_kernel<2, E, bf16, Jobs>)};
+  for (const void* kernel : kernels) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes + 1024);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace
@@ -1078,9 +1095,8 @@ cudaError_t prepare_gemm_tc() {
   if (e != cudaSuccess) return e;
   if (found != cudaDriverEntryPointSuccess || entry == nullptr) return cudaErrorSymbolNotFound;
   g_encode = reinterpret_cast<EncodeTiled>(entry);
-  for (auto prepare : {prepare_kind<1, TcEpilogue::kStore>, prepare_kind<2, TcEpilogue::kStore>,
-                       prepare_kind<1, TcEpilogue::kGate>, prepare_kind<2, TcEpilogue::kGate>,
-                       prepare_kind<1, TcEpilogue::kGateGrad>, prepare_kind<2, TcEpilogue::kGateGrad>})
+  for (auto prepare : {prepare_kind<TcEpilogue::kStore, 1>, prepare_kind<TcEpilogue::kStore, kTcMaxProducts>,
+                       prepare_kind<TcEpilogue::kGate, 1>, prepare_kind<TcEpilogue::kGateGrad, 1>})
     if ((e = prepare()) != cudaSuccess) return e;
   return cudaSuccess;
 }
@@ -1106,8 +1122,8 @@ cudaError_t launch_planned(const TcProduct* products, int count, Plan plan, void
   const int planes = wide ? kPlanes : 1;
   // items are counted in 32 bits, with room for a last stride beyond them
   if (plan.items > 0x70000000) return cudaErrorInvalidValue;
-  Args args{};
-  Maps maps{};
+  Args<kTcMaxProducts> args{};
+  Maps<kTcMaxProducts> maps{};
   PartsList parts{};
   int parted = 0;
   int64_t most = 0;
@@ -1180,12 +1196,20 @@ cudaError_t launch_planned(const TcProduct* products, int count, Plan plan, void
   args.row_sums = p.row_sums;
   args.row_sums_stride = p.row_sums_stride;
   args.status = dev.status;
-  switch (p.epilogue) {
-    case TcEpilogue::kGate: return launch_kind<TcEpilogue::kGate>(wide, maps, args, plan, dependent, stream);
-    case TcEpilogue::kGateGrad: return launch_kind<TcEpilogue::kGateGrad>(wide, maps, args, plan, dependent, stream);
-    default: break;
+  cudaError_t e;
+  if (args.jobs == 1) {
+    Args<1> one{};
+    static_cast<Common&>(one) = args;
+    one.job[0] = args.job[0];
+    Maps<1> of_one;
+    for (int t = 0; t < 2; ++t) of_one.a[0][t] = maps.a[0][t], of_one.b[0][t] = maps.b[0][t];
+    if (gate) return launch_kind<TcEpilogue::kGate>(wide, of_one, one, plan, dependent, stream);
+    if (p.epilogue == TcEpilogue::kGateGrad)
+      return launch_kind<TcEpilogue::kGateGrad>(wide, of_one, one, plan, dependent, stream);
+    e = launch_kind<TcEpilogue::kStore>(wide, of_one, one, plan, dependent, stream);
+  } else {
+    e = launch_kind<TcEpilogue::kStore>(wide, maps, args, plan, dependent, stream);
   }
-  const cudaError_t e = launch_kind<TcEpilogue::kStore>(wide, maps, args, plan, dependent, stream);
   if (e != cudaSuccess || parted == 0) return e;
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks_of(most / 4, 256), 8ll * dev.sms)), parted);
   return launch_dependent(wide ? add_parts_kernel<float> : add_parts_kernel<bf16>, grid, dim3(256), 0, stream, parts);
