@@ -310,7 +310,9 @@ int fhb_train_step(const float* coords, int64_t n, int64_t n_total, const float*
  * with x [tokens][width], w_gate, w_up [hidden][width], w_down [out_width][hidden], biases
  * [hidden], [hidden], [out_width] (each may be NULL), act tanh or silu (FHB_ACTIVATION_*).
  * All tensors have type `dtype`. h is rounded to `dtype` between the two products (as are the
- * gradients of g and u in the backward): they are operands of a product of that type.
+ * gradients of g and u in the backward): they are operands of a product of that type. A NaN or
+ * infinity among the inputs reaches the rows and columns it would reach, as NaN where FP32
+ * products of infinities by pieces (an infinity times a piece that is zero) make it one.
  */
 typedef struct fhb_ffn_problem {
   int64_t tokens, width, hidden, out_width;
