@@ -23,7 +23,7 @@ namespace {
 constexpr int kBlock = FHB_ADAMW_BLOCK;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kResident = 4, kResidentEight = 3;  // CTAs an SM holds
+constexpr int kResident = 3, kResidentEight = 3;  // CTAs an SM holds
 // Tensors of one launch: its arguments hold 4 KB cheaply and 32 KB at most.
 constexpr int kFewTensors = 40, kManyTensors = 400;
 // The step counter's upper bits count the CTAs that are done (0 between launches).
