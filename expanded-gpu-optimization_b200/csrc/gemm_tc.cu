@@ -214,13 +214,44 @@ __device__ __forceinline__ void split_f32(float x, float& a, float& b, float& c)
   c = (x - a) - b;
 }
 
+// Where a lane's row lies among its neighbours': rows of lanes 2i and 2i + 1 are written together.
+struct RowPair {
+  bool odd, even_row, odd_row;  // this lane's place; which of the two rows exist
+};
+// 64 bytes of each lane's row at `p` (rows `stride` bytes apart from lane to lane), in two pieces:
+// the lanes of a pair exchange one, so that an access has 64 bytes of a row (5.8 TB/s where 32
+// bytes a row reach 4.3). For whole warps.
+__device__ __forceinline__ void store64(void* p, int64_t stride, const RowPair& rows,
+                                        const uint32_t (&first)[8], const uint32_t (&second)[8]) {
+  uint32_t got[8], w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) got[i] = __shfl_xor_sync(0xffffffffu, rows.odd ? first[i] : second[i], 1);
+  char* const at = static_cast<char*>(p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = rows.odd ? got[i] : first[i];
+  if (rows.even_row) store32(rows.odd ? at - stride + 32 : at, w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = rows.odd ? second[i] : got[i];
+  if (rows.odd_row) store32(rows.odd ? at + 32 : at + stride, w);
+}
+// 16 FP32 values of each lane's row.
+__device__ __forceinline__ void store64(float* p, int64_t stride, const RowPair& rows, const float (&v)[kGroup]) {
+  uint32_t a[8], b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = __float_as_uint(v[i]), b[i] = __float_as_uint(v[8 + i]);
+  store64(static_cast<void*>(p), stride * 4, rows, a, b);
+}
+__device__ __forceinline__ void pack_group(const float (&v)[kGroup], uint32_t (&w)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+}
+
 // 16 values of a row in operand form (bf16, or three planes), 32-byte aligned.
 template <typename T>
 __device__ __forceinline__ void store_operand(bf16* p, int64_t plane, const float (&v)[kGroup]) {
   uint32_t w[8];
   if (sizeof(T) == 2) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+    pack_group(v, w);
     store32(p, w);
   } else {
     uint32_t w1[8], w2[8];
@@ -304,29 +335,33 @@ __device__ __forceinline__ float group_unscale(uint32_t e) {
   return __uint_as_float((e - 14u) << 23);
 }
 
-// 16 factors of one kind into their place (see TcFactors).
+// The factors of a group of 16, both kinds, into their places (see TcFactors). For whole warps.
+__device__ __forceinline__ uint32_t pack_factors(const float (&v)[kGroup], uint32_t (&w)[8]) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kGroup; ++i) top = fmaxf(top, fabsf(v[i]));
+  uint32_t e;
+  const float scale = group_scale(top, e);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const __half2 h = __floats2half2_rn(v[2 * i] * scale, v[2 * i + 1] * scale);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return e;
+}
 template <typename T>
-__device__ __forceinline__ void store_factors(const TcFactors& f, int64_t place, const float (&v)[kGroup]) {
-  uint32_t w[16];
-  if (sizeof(T) == 2) {
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kGroup; ++i) top = fmaxf(top, fabsf(v[i]));
-    uint32_t e;
-    const float scale = group_scale(top, e);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const __half2 h = __floats2half2_rn(v[2 * i] * scale, v[2 * i + 1] * scale);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    store32(static_cast<__half*>(f.values) + place * kFactorGroup, w);
-    f.exponents[place] = static_cast<unsigned char>(e);
+__device__ __forceinline__ void store_factors(const TcFactors& f, int64_t place, bool own, const RowPair& rows,
+                                              const float (&f1)[kGroup], const float (&f2)[kGroup]) {
+  const int64_t row_values = f.groups * 2 * kFactorGroup;  // from one token to the next
+  if constexpr (sizeof(T) == 2) {
+    uint32_t a[8], b[8];
+    const uint32_t e1 = pack_factors(f1, a), e2 = pack_factors(f2, b);
+    store64(static_cast<__half*>(f.values) + place * kFactorGroup, row_values * 2, rows, a, b);
+    if (own) *reinterpret_cast<uint16_t*>(f.exponents + place) = static_cast<uint16_t>(e1 | e2 << 8);
   } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i]);
     float* p = static_cast<float*>(f.values) + place * kFactorGroup;
-    store32(p, w);
-    store32(p + 8, w + 8);
+    store64(p, row_values, rows, f1);
+    store64(p + kFactorGroup, row_values, rows, f2);
   }
 }
 // The factors of one kind of a group, as they lie in memory.
@@ -359,23 +394,24 @@ __device__ __forceinline__ void times_factors(const FactorWords<T>& x, const flo
   }
 }
 
-// Column sums over the warp's 32 rows (one row a lane): lanes i and i + 16 get column i's, by
-// halving the columns and doubling the rows, in a fixed order.
+// Column sums over the 16 lanes of a lane's parity: lane l gets column l / 2's, by halving the
+// columns and doubling the rows, in a fixed order.
 __device__ __forceinline__ float sum_rows(const float (&v)[kGroup], int lane) {
   float s[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float keep = lane & 8 ? v[i + 8] : v[i], give = lane & 8 ? v[i] : v[i + 8];
-    s[i] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
+    const float keep = lane & 16 ? v[i + 8] : v[i], give = lane & 16 ? v[i] : v[i + 8];
+    s[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
   }
 #pragma unroll
   for (int half = 4; half >= 1; half /= 2)
 #pragma unroll
     for (int i = 0; i < half; ++i) {
-      const float keep = lane & half ? s[i + half] : s[i], give = lane & half ? s[i] : s[i + half];
-      s[i] = keep + __shfl_xor_sync(0xffffffffu, give, half);
+      const bool upper = lane & (2 * half);
+      const float keep = upper ? s[i + half] : s[i], give = upper ? s[i] : s[i + half];
+      s[i] = keep + __shfl_xor_sync(0xffffffffu, give, 2 * half);
     }
-  return s[0] + __shfl_xor_sync(0xffffffffu, s[0], 16);
+  return s[0];
 }
 
 template <int Jobs>
@@ -617,6 +653,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---- results: each warp has 32 rows; four warps share the columns ----
     const int quadrant = warp % 4, quarter = warp / 4, pairs = p.columns / 32;
+    // a warp's pairs of 16 columns are neighbours
+    const int each = (pairs + 3) / 4, first_pair = quarter * each, end_pair = min(pairs, first_pair + each);
     const uint32_t release = Cg == 2 ? in_cta(smem_u32(&sum_empty[0]), 0) : smem_u32(&sum_empty[0]);
     int64_t sums = 0;
     bool ok = true;
@@ -625,6 +663,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Job& q = job_of(p, it.job);
       const int chunks = chunk_count<T>(it.blocks);
       const int64_t row = it.m0 + rank * kRows + quadrant * 32 + lane;
+      const bool odd = (lane & 1) != 0, own = row < q.m;
+      const RowPair rows{odd, row - odd < q.m, row + !odd < q.m};
       const auto release_sums = [&](int buffer) {
         tc::fence_before_sync();
         __syncwarp();
@@ -667,73 +707,86 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
 
       if constexpr (E == TcEpilogue::kGateGrad) {
-        // group by group of 16 columns; a group's factors are on their way while the sums (for
-        // the first) or the group before are worked on
+        // Two groups of 16 columns at a time. The lanes of a pair exchange one, so that a lane has
+        // one group of both rows and an access 64 bytes of a row (FP32, 65,536 x 64 -> 256: 117 ->
+        // 104 us). A row's factors are on their way while the sums or the row before are worked on;
+        // both rows' at once spill registers (16,384 x 2,048 -> 5,632, bf16: 374 us against 356).
         FactorWords<T> f1, f2;
-        const auto prefetch = [&](int group) {
-          const int64_t n0 = it.n0 + 32 * (quarter + 4 * (group / 2)) + 16 * (group % 2);
-          if (row >= q.m || n0 >= q.n) return;
-          const int64_t place = (row * p.factors.groups + n0 / kFactorGroup) * 2;
+        const auto prefetch = [&](int pair, int which_row) {
+          const int64_t n0 = it.n0 + 32 * pair + 16 * odd, at_row = row - odd + which_row;
+          if (at_row >= q.m || n0 >= q.n) return;
+          const int64_t place = (at_row * p.factors.groups + n0 / kFactorGroup) * 2;
           load_factors<T>(p.factors, place, f1);
           load_factors<T>(p.factors, place + 1, f2);
         };
-        const auto finish = [&](int group, const float (&v)[kGroup]) {
-          const int64_t n0 = it.n0 + 32 * (quarter + 4 * (group / 2)) + 16 * (group % 2);
-          if (n0 >= q.n) return;
+        const auto finish = [&](int pair, float (&v0)[kGroup], float (&v1)[kGroup]) {
+          if (it.n0 + 32 * pair >= q.n) return;
+          __syncwarp();
 #pragma unroll
-          for (int which = 0; which < 2; ++which) {  // dg = dh f2, then du = dh f1
-            float d[kGroup];
-            times_factors<T>(which == 0 ? f2 : f1, v, d);
-            if (row < q.m)
-              store_operand<T>(p.gated[which] + row * p.gated_stride + n0, p.gated_plane, d);
-            if (p.row_sums == nullptr) continue;
-            if (row >= q.m) {
+          for (int i = 0; i < kGroup; ++i) {
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? v0[i] : v1[i], 1);
+            v0[i] = odd ? got : v0[i];
+            v1[i] = odd ? v1[i] : got;
+          }
+          const int64_t n0 = it.n0 + 32 * pair + 16 * odd, first_row = it.m0 + rank * kRows + quadrant * 32;
+          float sum[2];
 #pragma unroll
-              for (int i = 0; i < kGroup; ++i) d[i] = 0.0f;
+          for (int r = 0; r < 2; ++r) {
+            const int64_t at_row = row - odd + r;
+            const bool live = at_row < q.m && n0 < q.n;
+            if (r == 1) prefetch(pair, 1);
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {  // dg = dh f2, then du = dh f1
+              float d[kGroup];
+              times_factors<T>(which == 0 ? f2 : f1, r == 0 ? v0 : v1, d);
+              if (live) store_operand<T>(p.gated[which] + at_row * p.gated_stride + n0, p.gated_plane, d);
+              if (p.row_sums == nullptr) continue;
+              if (!live) {
+#pragma unroll
+                for (int i = 0; i < kGroup; ++i) d[i] = 0.0f;
+              }
+              __syncwarp();
+              const float s = sum_rows(d, lane);
+              sum[which] = r == 0 ? s : sum[which] + s;
+              if (r == 1 && first_row < q.m && n0 < q.n)
+                p.row_sums[(first_row / 32 * 2 + which) * p.row_sums_stride + n0 + lane / 2] = sum[which];
             }
-            __syncwarp();
-            const float sum = sum_rows(d, lane);
-            const int64_t rows = it.m0 + rank * kRows + quadrant * 32;
-            if (rows < q.m && lane < kGroup) p.row_sums[(rows / 32 * 2 + which) * p.row_sums_stride + n0 + lane] = sum;
           }
         };
-        const int groups = quarter < pairs ? 2 * ((pairs - quarter + 3) / 4) : 0;
-        if (groups > 0) prefetch(0);
+        if (first_pair < end_pair) prefetch(first_pair, 0);
         if constexpr (kChunked) {
-          float v0[kGroup], v1[kGroup];  // at most 128 columns: two groups a warp
+          float v0[kGroup], v1[kGroup];  // at most 128 columns: a pair a warp
           for (int c = 0; c < chunks; ++c, ++sums) {
             const int buffer = static_cast<int>(sums & 1);
             if (!wait_sums(buffer)) break;
-            if (groups > 0) {
-              const uint32_t from = tmem + buffer * kMaxColumns + lanes + 32 * quarter;
+            if (first_pair < end_pair) {
+              const uint32_t from = tmem + buffer * kMaxColumns + lanes + 32 * first_pair;
               add_columns(from, c == 0, v0);
               add_columns(from + 16, c == 0, v1);
             }
             release_sums(buffer);
           }
-          if (ok && groups > 0) {
-            finish(0, v0);
-            prefetch(1);
-            finish(1, v1);
-          }
+          if (ok && first_pair < end_pair) finish(first_pair, v0, v1);
         } else {
           const int buffer = static_cast<int>(sums & 1);
           if (!wait_sums(buffer)) break;
           ++sums;
           const uint32_t from = tmem + buffer * kMaxColumns + lanes;
-          for (int group = 0; group < groups; ++group) {
-            float v[kGroup];
-            add_columns(from + 32 * (quarter + 4 * (group / 2)) + 16 * (group % 2), true, v);
-            if (group + 1 == groups) release_sums(buffer);
-            finish(group, v);
-            if (group + 1 < groups) prefetch(group + 1);
+          for (int pair = first_pair; pair < end_pair; ++pair) {
+            float v0[kGroup], v1[kGroup];
+            add_columns(from + 32 * pair, true, v0);
+            add_columns(from + 32 * pair + 16, true, v1);
+            if (pair + 1 == end_pair) release_sums(buffer);
+            finish(pair, v0, v1);
+            if (pair + 1 < end_pair) prefetch(pair + 1, 0);
           }
-          if (groups == 0) release_sums(buffer);
+          if (first_pair >= end_pair) release_sums(buffer);
         }
       } else {
         // two groups of 16 columns at a time: a gate tile's g and u, else neighbours
+        uint32_t held[8];  // bf16: h of the first of two neighbours, stored with the second's
+        bool holds = false;
         const auto finish = [&](int pair, float (&v0)[kGroup], float (&v1)[kGroup]) {
-          if (row >= q.m) return;
           if constexpr (kGateTile) {
             const int64_t n0 = it.n0 + 16 * pair;
             if (n0 >= q.n) return;
@@ -752,25 +805,56 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             if (p.activation == FHB_ACTIVATION_TANH) gate(std::true_type{});
             else gate(std::false_type{});
-            store_operand<T>(p.gated[0] + row * p.gated_stride + n0, p.gated_plane, h);
+            __syncwarp();
+            bf16* const at = p.gated[0] + row * p.gated_stride + n0;
+            if constexpr (sizeof(T) == 2) {
+              if (holds) {
+                uint32_t w[8];
+                pack_group(h, w);
+                store64(at - kGroup, p.gated_stride * 2, rows, held, w);
+                holds = false;
+              } else if (pair + 1 < end_pair && n0 + kGroup < q.n) {
+                pack_group(h, held);
+                holds = true;
+              } else if (own) {
+                store_operand<T>(at, p.gated_plane, h);
+              }
+            } else if (own) {
+              store_operand<T>(at, p.gated_plane, h);
+            }
             if (p.factors.values != nullptr) {
               const int64_t place = (row * p.factors.groups + n0 / kFactorGroup) * 2;
-              store_factors<T>(p.factors, place, v0);
-              store_factors<T>(p.factors, place + 1, v1);
+              __syncwarp();
+              store_factors<T>(p.factors, place, own, rows, v0, v1);
             }
           } else {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float(&v)[kGroup] = j == 0 ? v0 : v1;
-              const int64_t n0 = it.n0 + 32 * pair + 16 * j;
-              if (n0 >= q.n) break;
-              if (q.partial != nullptr) {
-                float* out = q.partial + ((static_cast<int64_t>(it.group) * q.parts + it.part) * q.m + row) * q.partial_stride;
-                store_results<float>(out, n0, q.partial_stride, true, v);
+            const int64_t n0 = it.n0 + 32 * pair;
+            if (n0 >= q.n) return;
+            __syncwarp();
+            if (q.partial != nullptr) {
+              float* out = q.partial +
+                           ((static_cast<int64_t>(it.group) * q.parts + it.part) * q.m + row) * q.partial_stride + n0;
+              store64(out, q.partial_stride, rows, v0);
+              store64(out + kGroup, q.partial_stride, rows, v1);
+              return;
+            }
+            add_bias<T>(q.bias[0], n0, q.n, v0);
+            if (n0 + kGroup < q.n) add_bias<T>(q.bias[0], n0 + kGroup, q.n, v1);
+            T* const out = static_cast<T*>(q.out[it.group]) + row * q.out_stride;
+            if (q.out_wide && n0 + 2 * kGroup <= q.n) {
+              __syncwarp();
+              if constexpr (sizeof(T) == 2) {
+                uint32_t a[8], b[8];
+                pack_group(v0, a);
+                pack_group(v1, b);
+                store64(out + n0, q.out_stride * 2, rows, a, b);
               } else {
-                add_bias<T>(q.bias[0], n0, q.n, v);
-                store_results<T>(static_cast<T*>(q.out[it.group]) + row * q.out_stride, n0, q.n, q.out_wide != 0, v);
+                store64(out + n0, q.out_stride, rows, v0);
+                store64(out + n0 + kGroup, q.out_stride, rows, v1);
               }
+            } else if (own) {
+              store_results<T>(out, n0, q.n, q.out_wide != 0, v0);
+              store_results<T>(out, n0 + kGroup, q.n, q.out_wide != 0, v1);
             }
           }
         };
@@ -780,16 +864,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!wait_sums(buffer)) break;
           const uint32_t from = tmem + buffer * kMaxColumns + lanes;
           // FP32 blocks have at most 128 columns: a pair a warp, kept over the chunks
-          for (int pair = quarter; pair < pairs; pair += 4) {
+          for (int pair = first_pair; pair < end_pair; ++pair) {
             const uint32_t c0 = from + (kGateTile ? 16 * pair : 32 * pair);
             const uint32_t c1 = kGateTile ? from + p.columns / 2 + 16 * pair : c0 + 16;
             add_columns(c0, !kChunked || c == 0, acc0);
             add_columns(c1, !kChunked || c == 0, acc1);
-            if (pair + 4 >= pairs) release_sums(buffer);
+            if (pair + 1 == end_pair) release_sums(buffer);
             if (!kChunked || c + 1 == chunks) finish(pair, acc0, acc1);
           }
           // a tile of 64 columns leaves half of the warps idle
-          if (quarter >= pairs) release_sums(buffer);
+          if (first_pair >= end_pair) release_sums(buffer);
         }
       }
     }
