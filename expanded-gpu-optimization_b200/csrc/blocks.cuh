@@ -29,10 +29,12 @@ __device__ __forceinline__ bf16 from_float<bf16>(float x) {
   return __float2bfloat16_rn(x);
 }
 
-// The block's activation a and its derivative at g, on the special-function unit (ex2, rcp: a
-// few ulp). silu: a = g s, a' = s (1 + g (1 - s)), s = 1 / (1 + e^-g). tanh: with r = 1 / (1 +
-// e^2g), a = 1 - 2 r and a' = 4 r (1 - r), which has no cancellation where tanh saturates;
-// below 1/4, where 1 - 2 r loses digits, the Taylor series (next term below 2^-26 of a).
+// The block's activation a and its derivative at g, on the special-function unit (ex2, rcp).
+// silu: a = g s, a' = s (1 + g (1 - s)), s = 1 / (1 + e^-g). tanh: with r = 1 / (1 + e^2|g|) <= 1/2,
+// |a| = 1 - 2 r and a' = 4 r (1 - r), which cancel nowhere on either side (with e^2g, r would go to 1
+// for negative g, and 1 - r lose all its digits by g = -9); below 1/4, where 1 - 2 r loses digits, the
+// Taylor series (next term below 2^-26 of a). An exponential e^x is off by about 1.5 |x| 2^-24, the
+// rounding of its exponent, and a few ulp: so are the tails of a and a'.
 __device__ __forceinline__ float reciprocal_of_one_plus_exp2(float x) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
@@ -42,13 +44,13 @@ __device__ __forceinline__ float reciprocal_of_one_plus_exp2(float x) {
 template <bool Tanh>
 __device__ __forceinline__ void block_activation(float g, float& a, float& slope) {
   if (Tanh) {
-    const float r = reciprocal_of_one_plus_exp2(g * 2.8853900817779268f);  // 2 / ln 2
+    const float r = reciprocal_of_one_plus_exp2(fabsf(g) * 2.8853900817779268f);  // 2 / ln 2
     const float q = g * g;
     float t = fmaf(q, 62.0f / 2835.0f, -17.0f / 315.0f);
     t = fmaf(q, t, 2.0f / 15.0f);
     t = fmaf(q, t, -1.0f / 3.0f);
     t = fmaf(g * q, t, g);
-    a = fabsf(g) < 0.25f ? t : fmaf(-2.0f, r, 1.0f);
+    a = fabsf(g) < 0.25f ? t : copysignf(fmaf(-2.0f, r, 1.0f), g);
     slope = 4.0f * r * (1.0f - r);
   } else {
     const float s = reciprocal_of_one_plus_exp2(g * -1.4426950408889634f);  // 1 / ln 2

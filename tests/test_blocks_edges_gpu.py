@@ -1,0 +1,52 @@
+"""Corners of the gated residual trunk's operators."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import fused_hoad
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16]
+
+
+# ---- the activation's derivative where it saturates ----
+
+
+def slope_tolerance(g: float, dtype: torch.dtype) -> float:
+    """e^{2|g|} is a power of 2 whose exponent 2|g| / ln 2 is rounded (2|g| 2^-24 of the result)
+    times a rounded constant (half of that again); the power, the reciprocal and the products add
+    less than 16 * 2^-24. bfloat16: the operand's and the result's rounding and one more."""
+    return (3 * abs(g) + 16) * 2.0**-24 if dtype == torch.float32 else 3 * 2.0**-9
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_slope_of_saturated_units(dtype):
+    """tanh' is even and keeps its digits on both sides: each row and each feature to its own."""
+    values = [s * k for k in range(4, 13) for s in (1.0, -1.0)]
+    exact = {g: float(torch.cosh(torch.tensor(g, dtype=torch.float64)) ** -2) for g in values}
+
+    def make(*shape, fill):
+        return torch.full(shape, fill, device="cuda", dtype=dtype, requires_grad=True)
+
+    # rows: g = x, u = 1, dh = 1, so dx is the sum of 16 equal slopes
+    x = torch.tensor(values, device="cuda").view(-1, 1).to(dtype).requires_grad_()
+    wg, wu, wd, bu = make(16, 1, fill=1.0), make(16, 1, fill=0.0), make(1, 16, fill=1.0), make(16, fill=1.0)
+    y = fused_hoad.gated_feed_forward(x, wg, wu, wd, None, bu, activation="tanh")
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    for g, got in zip(values, dx.view(-1).tolist()):
+        assert abs(got - 16 * exact[g]) <= slope_tolerance(g, dtype) * 16 * exact[g], (g, got)
+    # features: 16 of each g, as biases, one token
+    bg = torch.tensor(values, device="cuda").repeat_interleave(16).to(dtype).requires_grad_()
+    hidden = bg.numel()
+    one = make(1, 1, fill=1.0)
+    wg, wu, wd, bu = make(hidden, 1, fill=0.0), make(hidden, 1, fill=0.0), make(1, hidden, fill=1.0), \
+        make(hidden, fill=1.0)
+    y = fused_hoad.gated_feed_forward(one, wg, wu, wd, bg, bu, activation="tanh")
+    for grad in torch.autograd.grad(y, [wg, bg], torch.ones_like(y)):
+        by_value = grad.view(-1, 16)
+        for g, got in zip(values, by_value.double().tolist()):
+            for v in got:
+                assert abs(v - exact[g]) <= slope_tolerance(g, dtype) * exact[g], (g, v)
+        assert torch.equal(by_value[0::2], by_value[1::2])
