@@ -358,8 +358,12 @@ class NormNode : public torch::autograd::Function<NormNode> {
       check_like(grad_normed, pre_weight, "grad_normed", "pre_weight");
       dn = as_rows(grad_normed);
     }
+    // without rows there may still be groups, each with a gate whose gradient is zero
     for (int i = 0, edge = 0; i < 6; ++i)
-      if (t[i + 1].defined() && ctx->needs_input_grad(edge++)) out[i] = torch::empty(t[i + 1].sizes(), t[i + 1].options());
+      if (t[i + 1].defined() && ctx->needs_input_grad(edge++))
+        out[i] = p.rows > 0 ? torch::empty(t[i + 1].sizes(), t[i + 1].options())
+                            : torch::zeros(t[i + 1].sizes(), t[i + 1].options());
+    if (p.rows == 0) return out;
     const auto place = [&](int i) { return out[i].defined() ? data_of(out[i]) : nullptr; };
     const fhb_norm_grads grads{place(0), place(1), place(2), place(3), place(4),
                                static_cast<float*>(place(5))};

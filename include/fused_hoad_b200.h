@@ -378,7 +378,8 @@ int fhb_residual_norm(const fhb_norm_problem* problem, void* total, void* normed
                       fhb_stream_t stream);
 size_t fhb_residual_norm_workspace_bytes(const fhb_norm_problem* problem);
 /* grad_total and grad_normed (row strides given; each may be NULL: zeros) to the gradients, in
- * a fixed order of sums (bitwise reproducible). rows == 0 zeroes the weights' gradients. */
+ * a fixed order of sums (bitwise reproducible). rows == 0 zeroes the weights' and the scale's
+ * gradients and one row of the gate's: the caller zeroes more, since groups have no rows then. */
 int fhb_residual_norm_backward(const fhb_norm_problem* problem, const void* grad_total,
                                int64_t grad_total_stride, const void* grad_normed,
                                int64_t grad_normed_stride, const float* stats,

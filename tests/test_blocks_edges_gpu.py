@@ -50,3 +50,23 @@ def test_slope_of_saturated_units(dtype):
             for v in got:
                 assert abs(v - exact[g]) <= slope_tolerance(g, dtype) * exact[g], (g, v)
         assert torch.equal(by_value[0::2], by_value[1::2])
+
+
+# ---- batches without rows ----
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,gate_shape", [((2, 0, 48), (2, 1, 48)), ((3, 5, 0, 40), (3, 5, 1, 40)),
+                                              ((0, 4, 48), (1, 1, 48)), ((4, 0, 48), (48,))])
+def test_gate_gradient_of_no_rows(shape, gate_shape, dtype):
+    """Every group's gate has a gradient of zero, whatever was in its memory before."""
+    width = shape[-1]
+    residual, branch = (torch.zeros(shape, device="cuda", dtype=dtype, requires_grad=True) for _ in range(2))
+    weight, gate = (torch.ones(s, device="cuda", dtype=dtype, requires_grad=True) for s in ((width,), gate_shape))
+    scale = torch.ones(1, device="cuda", requires_grad=True)
+    outs = fused_hoad.residual_norm(residual, branch, weight, weight, gate, scale)
+    used = [torch.full((n,), 7.0, device="cuda") for n in (64, 128, 256, 512, 1024) for _ in range(20)]
+    del used  # the gradients' memory comes from here
+    grads = torch.autograd.grad([o.sum() for o in outs], [weight, gate, scale, residual])
+    for g, t in zip(grads, (weight, gate, scale, residual)):
+        assert g.shape == t.shape and not g.any()
