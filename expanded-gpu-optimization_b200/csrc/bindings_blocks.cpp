@@ -450,6 +450,19 @@ void adamw_step(const std::vector<torch::Tensor>& params, const std::vector<torc
                               step.data_ptr<int64_t>(), lr, beta1, beta2, eps, weight_decay,
                               at::cuda::getCurrentCUDAStream()),
                "adamw_step");
+  // in place, as autograd sees it: a backward that saved one of these before the step raises
+  const auto written = [](const std::vector<torch::Tensor>& tensors) {
+    for (const torch::Tensor& t : tensors)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  };
+  written(params);
+  written(exp_avgs);
+  written(exp_avg_sqs);
+  if (eight) {
+    written(*exp_avg_scales);
+    written(*exp_avg_sq_scales);
+  }
+  written({step});
 }
 
 }  // namespace

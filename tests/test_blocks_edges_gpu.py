@@ -70,3 +70,40 @@ def test_gate_gradient_of_no_rows(shape, gate_shape, dtype):
     grads = torch.autograd.grad([o.sum() for o in outs], [weight, gate, scale, residual])
     for g, t in zip(grads, (weight, gate, scale, residual)):
         assert g.shape == t.shape and not g.any()
+
+
+# ---- parameters that change between a forward and its backward ----
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_step_before_a_backward_is_noticed(bits):
+    x, w, d = (torch.randn(s, device="cuda", requires_grad=True) for s in ((5, 8), (16, 8), (8, 16)))
+    weight = torch.ones(8, device="cuda", requires_grad=True)
+    optimizer = fused_hoad.AdamW([w, d, weight], state_bits=bits)
+
+    def loss():
+        return fused_hoad.residual_norm(x, fused_hoad.gated_feed_forward(x, w, w, d), weight)[1].sum()
+
+    loss().backward()
+    late = loss()
+    versions = [t._version for t in (w, d, weight)]
+    optimizer.step()
+    assert all(t._version > v for t, v in zip((w, d, weight), versions))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        late.backward()
+
+
+def test_adamw_step_raises_versions_of_all_it_writes():
+    p, g = torch.randn(300, device="cuda"), torch.randn(300, device="cuda")
+    codes = [torch.zeros(300, device="cuda", dtype=torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.zeros(2, device="cuda") for _ in range(2)]
+    step = torch.zeros(1, dtype=torch.int64, device="cuda")
+    written = [p, *codes, *scales, step]
+    before, of_grad = [t._version for t in written], g._version
+    fused_hoad.adamw_step([p], [g], [codes[0]], [codes[1]], step, exp_avg_scales=[scales[0]],
+                          exp_avg_sq_scales=[scales[1]])
+    assert all(t._version == v + 1 for t, v in zip(written, before)) and g._version == of_grad
+    with torch.inference_mode():  # inference tensors have no version
+        q, m, v = (torch.zeros(8, device="cuda") for _ in range(3))
+        fused_hoad.adamw_step([q], [torch.ones(8, device="cuda")], [m], [v], step)
+        assert q.any()
