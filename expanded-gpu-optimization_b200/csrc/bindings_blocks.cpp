@@ -4,6 +4,7 @@
 // Gradients are autograd nodes in C++: autograd's threads need no Python for them (a node in
 // Python costs about 70 us a backward pass).
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime.h>
 #include <torch/extension.h>
@@ -100,6 +101,14 @@ void check_differentiated_once(const char* op) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op,
               " is differentiable once: its backward does not support create_graph");
 }
+// Forward-mode derivatives are not computed: a result without its tangent would read as a zero
+// derivative, so an input that carries one is refused.
+void check_no_tangents(const char* op, const variable_list& tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const torch::Tensor& t : tensors)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), op,
+                " does not support forward-mode derivatives");
+}
 
 // ---- gated feed-forward block ----
 
@@ -192,6 +201,7 @@ class FfnNode : public torch::autograd::Function<FfnNode> {
 
   static variable_list backward(AutogradContext* ctx, variable_list upstream) {
     check_differentiated_once("gated_feed_forward");
+    check_no_tangents("gated_feed_forward's backward", upstream);
     const variable_list t = ctx->get_saved_variables();
     const torch::Tensor &saved = t[0], &x = t[1], &grad_y = upstream[0];
     const Ffn f = ffn_of(x, t[2], t[3], t[4], given(t[5]), given(t[6]), given(t[7]),
@@ -217,8 +227,10 @@ class FfnNode : public torch::autograd::Function<FfnNode> {
 torch::Tensor gated_feed_forward(torch::Tensor x, torch::Tensor w_gate, torch::Tensor w_up,
                                  torch::Tensor w_down, OptionalTensor b_gate, OptionalTensor b_up,
                                  OptionalTensor b_down, const std::string& activation) {
-  if (records_gradients({x, w_gate, w_up, w_down, or_undefined(b_gate), or_undefined(b_up),
-                         or_undefined(b_down)}))
+  const variable_list tensors{x, w_gate, w_up, w_down, or_undefined(b_gate), or_undefined(b_up),
+                              or_undefined(b_down)};
+  check_no_tangents("gated_feed_forward", tensors);
+  if (records_gradients(tensors))
     return FfnNode::apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation);
   return ffn_forward(ffn_of(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation), x, nullptr);
 }
@@ -340,6 +352,7 @@ class NormNode : public torch::autograd::Function<NormNode> {
 
   static variable_list backward(AutogradContext* ctx, variable_list upstream) {
     check_differentiated_once("residual_norm");
+    check_no_tangents("residual_norm's backward", upstream);
     const variable_list t = ctx->get_saved_variables();
     const torch::Tensor &stats = t[0], &residual = t[1], &branch = t[2], &pre_weight = t[3];
     const Norm n = norm_of(residual, given(branch), pre_weight, given(t[4]), given(t[5]), given(t[6]),
@@ -383,8 +396,10 @@ class NormNode : public torch::autograd::Function<NormNode> {
 variable_list residual_norm(torch::Tensor residual, OptionalTensor branch, torch::Tensor pre_weight,
                             OptionalTensor post_weight, OptionalTensor gate,
                             OptionalTensor scale_tensor, double scale, double eps) {
-  if (records_gradients({residual, or_undefined(branch), pre_weight, or_undefined(post_weight),
-                         or_undefined(gate), or_undefined(scale_tensor)}))
+  const variable_list tensors{residual, or_undefined(branch), pre_weight, or_undefined(post_weight),
+                              or_undefined(gate), or_undefined(scale_tensor)};
+  check_no_tangents("residual_norm", tensors);
+  if (records_gradients(tensors))
     return NormNode::apply(residual, branch, pre_weight, post_weight, gate, scale_tensor, scale, eps);
   const Norm n = norm_of(residual, branch, pre_weight, post_weight, gate, scale_tensor, scale, eps);
   auto [total, normed] = norm_forward(n, residual, pre_weight, branch.has_value(), nullptr);

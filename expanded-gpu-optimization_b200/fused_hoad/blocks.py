@@ -33,7 +33,7 @@ def gated_feed_forward(
     Rows may have any stride (a slice of a larger tensor is not copied). Sums are held in 32
     bits. In bfloat16 the gated product, and in the backward the gradients of the two
     projections, are rounded to bfloat16 as operands of the next matrix product. Differentiable
-    once (``create_graph`` raises).
+    once, in reverse (``create_graph`` and forward-mode tangents raise).
     """
     return load_extension().gated_feed_forward(
         x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation
@@ -69,7 +69,7 @@ def residual_norm(
     (``[batch, 1, width]``: a gate for each sample). ``residual_scale`` is a number or a float32
     tensor with one element, which then gets a gradient. ``residual`` and ``total`` may be
     float32 where everything else is bfloat16. Sums and norms are held in 32 bits, and the
-    norm is that of the unrounded total. Differentiable once.
+    norm is that of the unrounded total. Differentiable once, in reverse.
     """
     if branch is None:
         raise ValueError("residual_norm needs a branch; rms_norm is the norm alone")

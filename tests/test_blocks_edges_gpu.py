@@ -107,3 +107,32 @@ def test_adamw_step_raises_versions_of_all_it_writes():
         q, m, v = (torch.zeros(8, device="cuda") for _ in range(3))
         fused_hoad.adamw_step([q], [torch.ones(8, device="cuda")], [m], [v], step)
         assert q.any()
+
+
+# ---- forward-mode derivatives ----
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as forward
+
+    x, w, d = (torch.randn(s, device="cuda") for s in ((5, 8), (16, 8), (8, 16)))
+    c = torch.ones(8, device="cuda")
+    ffn_of = fused_hoad.gated_feed_forward
+    want, normed = ffn_of(x, w, w, d), fused_hoad.rms_norm(x, c)
+    with forward.dual_level():
+        dual_x, dual_d, dual_c = (forward.make_dual(t, torch.ones_like(t)) for t in (x, d, c))
+        for call in (lambda: ffn_of(dual_x, w, w, d), lambda: ffn_of(x, w, w, dual_d),
+                     lambda: ffn_of(x, w, w, d, None, None, dual_c),
+                     lambda: fused_hoad.residual_norm(x, dual_x, c),
+                     lambda: fused_hoad.residual_norm(x, x, c, gate=dual_c),
+                     lambda: fused_hoad.rms_norm(dual_x, c), lambda: fused_hoad.rms_norm(x, dual_c)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        # the gradient of a backward would lose its tangent just so
+        leaf = x.clone().requires_grad_()
+        for y in (ffn_of(leaf, w, w, d), fused_hoad.rms_norm(leaf, c)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, forward.make_dual(torch.ones_like(y), torch.ones_like(y)))
+        assert torch.equal(ffn_of(x, w, w, d), want)  # no tangents here
+        with torch.inference_mode():
+            assert torch.equal(fused_hoad.rms_norm(x, c), normed)
