@@ -340,6 +340,11 @@ __device__ __forceinline__ uint32_t pack_factors(const float (&v)[kGroup], uint3
   float top = 0.0f;
 #pragma unroll
   for (int i = 0; i < kGroup; ++i) top = fmaxf(top, fabsf(v[i]));
+  if (!(top < INFINITY)) {  // an infinity stays one at any scale: the others set it
+    top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) top = fmaxf(top, fabsf(v[i]) < INFINITY ? fabsf(v[i]) : 0.0f);
+  }
   uint32_t e;
   const float scale = group_scale(top, e);
 #pragma unroll

@@ -30,7 +30,7 @@ enum class TcEpilogue {
 // What the forward keeps of the activation for the backward, for 16 consecutive hidden features
 // of one token: f1 = act(g) and f2 = u act'(g), so that du = dh f1 and dg = dh f2.
 // bf16 block: f16 values times one power of 2 for each of the two groups of 16 (an exponent
-// byte each), so the range is FP32's and the rounding 2^-12 of the group's largest value --
+// byte each), so the range is FP32's and the rounding 2^-12 of the group's largest finite value --
 // 16 times below the bf16 rounding of dg and du that follows. FP32 block: FP32 values.
 constexpr int kFactorGroup = 16;
 struct TcFactors {

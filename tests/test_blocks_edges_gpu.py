@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import fused_hoad
+from trunk_reference import assert_near, ffn_gradients, tolerance
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16]
@@ -136,3 +137,33 @@ def test_forward_mode_is_refused():
         assert torch.equal(ffn_of(x, w, w, d), want)  # no tangents here
         with torch.inference_mode():
             assert torch.equal(fused_hoad.rms_norm(x, c), normed)
+
+
+# ---- factors next to an infinity ----
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("activation", ["silu", "tanh"])
+def test_an_infinite_unit_keeps_to_its_column(activation, dtype):
+    """A feature whose g or u is infinite: the other features' gradients are what they were."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    tokens, width, hidden, bad = 40, 32, 48, 21
+    x, wg, wu = ((torch.randn(s, generator=g, device="cuda") * 0.5).to(dtype)
+                 for s in ((tokens, width), (hidden, width), (hidden, width)))
+    wd = torch.randn(width, hidden, generator=g, device="cuda").to(dtype)
+    bg, bu = (torch.randn(hidden, generator=g, device="cuda").to(dtype) for _ in range(2))
+    grad = torch.randn(tokens, width, generator=g, device="cuda").to(dtype)
+    keep = [k for k in range(hidden) if k != bad]
+    for which in (bg, bu):
+        old = which[bad].clone()
+        which[bad] = float("inf")
+        leaves = [t.detach().requires_grad_() for t in (x, wg, wu, wd, bg, bu)]
+        y = fused_hoad.gated_feed_forward(*leaves, activation=activation)
+        got = torch.autograd.grad(y, leaves[1:], grad)
+        which[bad] = old
+        wide = [t.double() for t in (x, wg, wu, wd, bg, bu)]
+        want = ffn_gradients(grad.double(), *wide, None, activation)
+        for name, a, b in zip(("w_gate", "w_up", "w_down", "b_gate", "b_up"), got, want[1:]):
+            a, b = (a[:, keep], b[:, keep]) if name == "w_down" else (a[keep], b[keep])
+            size = torch.full_like(b, float(b.square().mean().sqrt()))
+            assert_near(a, b, tolerance(dtype, tokens), f"d_{name}", size)
