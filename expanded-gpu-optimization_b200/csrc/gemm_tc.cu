@@ -200,18 +200,25 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return r;
 }
 
-// x as a sum of three bf16 (FP32's 24 significant bits in pieces of 8): each piece is the
-// remainder cut after 8 significant bits, so every difference is exact, the sum is x, and no
-// piece overflows. An infinity or a NaN is all in the first.
-__device__ __forceinline__ void split_f32(float x, float& a, float& b, float& c) {
-  a = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
-  if (!(fabsf(x) < INFINITY)) {
-    a = x;
-    b = c = 0.0f;
-    return;
+// x and y as sums of three bf16 each, w[i] holding the i-th pieces of both: each piece is the
+// remainder rounded to 8 significant bits, so every difference is exact, the second piece is at most
+// 2^-8 of x and the third 2^-17, with either sign. Their sum is x (from 2^-110 up; below it, x to the
+// 2^-133 at which bf16 ends). What would round up to infinity is cut instead; an infinity is all in
+// the first piece.
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&w)[3]) {
+  constexpr float kRoundsUp = 0x1.FFp127f;
+  const auto low = [](uint32_t v) { return __uint_as_float(v << 16); };
+  const auto high = [](uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); };
+  w[0] = pack_bf16(x, y);
+  float rest_x = x - low(w[0]), rest_y = y - high(w[0]);
+  if (!(fabsf(x) < kRoundsUp && fabsf(y) < kRoundsUp)) {
+    const bool real_x = fabsf(x) < INFINITY, real_y = fabsf(y) < INFINITY;
+    w[0] = pack_bf16(real_x ? high(__float_as_uint(x)) : x, real_y ? high(__float_as_uint(y)) : y);
+    rest_x = real_x ? x - low(w[0]) : 0.0f;
+    rest_y = real_y ? y - high(w[0]) : 0.0f;
   }
-  b = __uint_as_float(__float_as_uint(x - a) & 0xFFFF0000u);
-  c = (x - a) - b;
+  w[1] = pack_bf16(rest_x, rest_y);
+  w[2] = pack_bf16(rest_x - low(w[1]), rest_y - high(w[1]));
 }
 
 // Where a lane's row lies among its neighbours': rows of lanes 2i and 2i + 1 are written together.
@@ -257,12 +264,11 @@ __device__ __forceinline__ void store_operand(bf16* p, int64_t plane, const floa
     uint32_t w1[8], w2[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float a[2], b[2], c[2];
-      split_f32(v[2 * i], a[0], b[0], c[0]);
-      split_f32(v[2 * i + 1], a[1], b[1], c[1]);
-      w[i] = pack_bf16(a[0], a[1]);
-      w1[i] = pack_bf16(b[0], b[1]);
-      w2[i] = pack_bf16(c[0], c[1]);
+      uint32_t pieces[3];
+      split_pair(v[2 * i], v[2 * i + 1], pieces);
+      w[i] = pieces[0];
+      w1[i] = pieces[1];
+      w2[i] = pieces[2];
     }
     store32(p, w);
     store32(p + plane, w1);
@@ -456,11 +462,11 @@ __device__ __forceinline__ Item item_at(const Args<Jobs>& p, uint32_t index) {
 }
 
 // FP32 blocks. A slot holds the three planes of 64 of K of both operands, for six of their nine
-// products (the others are below 2^-24 of the whole): the large one has an accumulator of its
-// own and the five small ones share another, kSmallColumns on. The tensor core cuts each sum to
-// FP32 instead of rounding it, an error that grows with the number of additions and has a sign:
-// the small products do not add to it that way, and K is summed in chunks of kChunkBlocks slots
-// per term, the chunks in registers, rounded.
+// products (the others come to at most 2^-24 of a product, of either sign): the large one has an
+// accumulator of its own and the five small ones share another, kSmallColumns on. The tensor core
+// cuts each sum to FP32 instead of rounding it, an error that grows with the number of additions and
+// has a sign: the small products do not add to it that way, and K is summed in chunks of
+// kChunkBlocks slots per term, the chunks in registers, rounded.
 constexpr int kChunkBlocks = 2;
 constexpr int kSmallColumns = 128;
 template <typename T>
@@ -969,11 +975,10 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJ
       if (sizeof(T) == 2) {
         w[0][k] = pack_bf16(v[2 * k], v[2 * k + 1]);
       } else {
-        float x[3], y[3];
-        split_f32(v[2 * k], x[0], x[1], x[2]);
-        split_f32(v[2 * k + 1], y[0], y[1], y[2]);
+        uint32_t pieces[3];
+        split_pair(v[2 * k], v[2 * k + 1], pieces);
 #pragma unroll
-        for (int q = 0; q < 3; ++q) w[q][k] = pack_bf16(x[q], y[q]);
+        for (int q = 0; q < 3; ++q) w[q][k] = pieces[q];
       }
     }
 #pragma unroll

@@ -12,7 +12,7 @@ namespace fhb {
 
 // A bf16 matrix in memory, rows x columns, rows `stride` elements apart (a multiple of 8, base
 // 16-byte aligned: what a TMA tile copy needs). An FP32 matrix is three such planes whose sum
-// it is (split_f32 in gemm_tc.cu), `plane` elements apart.
+// it is (split_pair in gemm_tc.cu), `plane` elements apart.
 struct TcMatrix {
   const bf16* p = nullptr;
   int64_t rows = 0, cols = 0, stride = 0, plane = 0;

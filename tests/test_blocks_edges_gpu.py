@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import fused_hoad
-from trunk_reference import assert_near, ffn_gradients, tolerance
+from trunk_reference import assert_near, ffn, ffn_gradients, tolerance
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16]
@@ -167,3 +167,40 @@ def test_an_infinite_unit_keeps_to_its_column(activation, dtype):
             a, b = (a[:, keep], b[:, keep]) if name == "w_down" else (a[keep], b[keep])
             size = torch.full_like(b, float(b.square().mean().sqrt()))
             assert_near(a, b, tolerance(dtype, tokens), f"d_{name}", size)
+
+
+# ---- FP32 operands whose low bits are all set ----
+
+
+@pytest.mark.parametrize("value", [1 + 2**-7 - 2**-23, 1 + 2**-8 - 2**-23, 2 - 2**-23,
+                                   -(1 + 2**-7 + 2**-15 - 2**-23)])
+@pytest.mark.parametrize("activation", ["silu", "tanh"])
+def test_operands_with_all_low_bits_set(activation, value):
+    """One product a result: what is left out of the products of pieces is not averaged away."""
+    tensors = [torch.full(s, value, device="cuda") for s in ((130, 1), (1, 1), (1, 1), (1, 1))]
+    grad = torch.full((130, 1), abs(value), device="cuda")
+    tol = tolerance(torch.float32, 1)
+    wide = [t.double() for t in tensors]
+    with torch.no_grad():
+        y = fused_hoad.gated_feed_forward(*tensors, activation=activation)
+    assert_near(y, ffn(*wide, activation=activation), tol, "y")
+    leaves = [t.requires_grad_() for t in tensors]
+    y = fused_hoad.gated_feed_forward(*leaves, activation=activation)
+    got = torch.autograd.grad(y, leaves, grad)
+    want = ffn_gradients(grad.double(), *wide, None, None, None, activation)
+    # the sums over the tokens add 130 equal values: their own rounding
+    for name, a, b, terms in zip(("x", "w_gate", "w_up", "w_down"), got, want, (2, 130, 130, 130)):
+        assert_near(a, b, tolerance(torch.float32, terms), "d_" + name)
+
+
+def test_operands_at_the_ends_of_the_range():
+    """The largest numbers do not round up to infinity in their pieces."""
+    largest, least = torch.finfo(torch.float32).max, 2.0**-126
+    x = torch.tensor([[largest], [-largest], [largest / 3], [2.0**127], [1.0]], device="cuda").repeat(30, 1)
+    wg = torch.tensor([[least]], device="cuda")
+    wu, wd = torch.tensor([[0.0]], device="cuda"), torch.tensor([[1.0]], device="cuda")
+    bu = torch.tensor([1.0], device="cuda")
+    with torch.no_grad():
+        y = fused_hoad.gated_feed_forward(x, wg, wu, wd, None, bu, activation="tanh")
+    want = ffn(x.double(), wg.double(), wu.double(), wd.double(), None, bu.double(), activation="tanh")
+    assert_near(y, want, tolerance(torch.float32, 1), "y")
