@@ -67,14 +67,19 @@ int check_ffn(const fhb_ffn_problem* p) {
                   check_vector(p->b_down, p->dtype, false));
 }
 
-int check_norm(const fhb_norm_problem* p) {
+int check_norm_sizes(const fhb_norm_problem* p) {
   if (p == nullptr || !valid_dtype(p->dtype) || !valid_dtype(p->residual_dtype) ||
       (p->residual_dtype == FHB_DTYPE_BF16 && p->dtype == FHB_DTYPE_F32) || p->rows < 0 ||
       p->width < 1 || !(p->eps >= 0.0f) ||
       (p->branch == nullptr && p->rows > 0 && (p->gate != nullptr || p->post_weight != nullptr)) ||
       (p->gate != nullptr && p->gate_rows < 1))
     return FHB_ERR_INVALID_ARGUMENT;
-  if (p->rows > kMaxRows || p->width > kMaxNormWidth) return FHB_ERR_TOO_LARGE;
+  return p->rows > kMaxRows || p->width > kMaxNormWidth ? FHB_ERR_TOO_LARGE : FHB_OK;
+}
+
+int check_norm(const fhb_norm_problem* p) {
+  const int code = check_norm_sizes(p);
+  if (code != FHB_OK) return code;
   return first_of(
       check_matrix(p->residual, p->rows, p->width, p->residual_stride, p->residual_dtype),
       p->branch == nullptr ? FHB_OK
@@ -158,9 +163,7 @@ int fhb_residual_norm(const fhb_norm_problem* problem, void* total, void* normed
 
 size_t fhb_residual_norm_workspace_bytes(const fhb_norm_problem* problem) {
   const fhb::DeviceInfo* dev = nullptr;
-  if (problem == nullptr || problem->rows < 0 || problem->width < 1 || problem->rows > kMaxRows ||
-      problem->width > kMaxNormWidth || fhb::current_device_info(&dev) != FHB_OK)
-    return 0;
+  if (check_norm_sizes(problem) != FHB_OK || fhb::current_device_info(&dev) != FHB_OK) return 0;
   return fhb::residual_norm_workspace_bytes(*problem, *dev);
 }
 

@@ -2,10 +2,13 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 import fused_hoad
+from fused_hoad import _native
 from trunk_reference import assert_near, ffn, ffn_gradients, tolerance
 
 pytestmark = pytest.mark.gpu
@@ -204,3 +207,21 @@ def test_operands_at_the_ends_of_the_range():
         y = fused_hoad.gated_feed_forward(x, wg, wu, wd, None, bu, activation="tanh")
     want = ffn(x.double(), wg.double(), wu.double(), wd.double(), None, bu.double(), activation="tanh")
     assert_near(y, want, tolerance(torch.float32, 1), "y")
+
+
+# ---- sizes asked for by a C caller ----
+
+
+@pytest.mark.parametrize("change", [dict(gate_rows=0), dict(gate_rows=-1), dict(gate_rows=-(2**62)),
+                                    dict(rows=-1), dict(width=0), dict(dtype=7), dict(eps=-1.0)])
+def test_workspace_size_of_a_refused_norm(change):
+    """0, as the calls' own refusal; a host process that asks is not ended by it."""
+    fields = dict(rows=4, width=8, residual_dtype=0, dtype=0, residual=4096, branch=4096,
+                  pre_weight=4096, gate=4096, residual_stride=8, branch_stride=8, gate_rows=2,
+                  residual_scale=1.0, eps=1e-6)  # addresses that are not read
+
+    def size(**changed):
+        problem = _native.NormProblem(**{**fields, **changed})
+        return _native.library().fhb_residual_norm_workspace_bytes(ctypes.byref(problem))
+
+    assert size() > 0 and size(**change) == 0
