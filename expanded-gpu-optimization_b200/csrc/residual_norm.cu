@@ -17,6 +17,7 @@
 // backward 120 us (604 MB, 5.0 TB/s: ten registers a value leave an SM two rows at a time, and
 // the sums' barriers show) and 5 us for the column sums.
 #include <algorithm>
+#include <atomic>
 
 #include "blocks.cuh"
 #include "common.cuh"
@@ -585,8 +586,9 @@ NormArgs arguments(const fhb_norm_problem& p) {
 }
 
 // Rows a CTA can have on their way in its part of an SM's shared memory; fewer than two: none.
+constexpr int kStagedBytes = 216 * 1024;  // of an SM
 int stages_of(int64_t row_bytes, int resident) {
-  const int64_t n = std::min<int64_t>(216 * 1024 / resident / row_bytes, kMaxStages);
+  const int64_t n = std::min<int64_t>(kStagedBytes / resident / row_bytes, kMaxStages);
   return n >= 2 ? static_cast<int>(n) : 0;
 }
 
@@ -668,15 +670,25 @@ cudaError_t with_layout(bool wide, int64_t width, Body body) {
   return wide ? with_layout<true, Backward>(width, body) : with_layout<false, Backward>(width, body);
 }
 
-// A launch with more than 48 KB of shared memory.
-template <typename Kernel, typename... Arguments>
-cudaError_t launch_staged(Kernel kernel, unsigned grid, int block, size_t smem, cudaStream_t stream,
-                          Arguments... arguments) {
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(smem));
+// The most shared memory that a launch of a staged kernel asks for, set with its first call on a
+// device: the limit is the kernel's, not the launch's, and host threads with rows of different bytes
+// share it. (All of these kernels at once would take 18 ms to load.)
+template <bool Backward, typename L, typename TR, typename T>
+cudaError_t allow_staged() {
+  static std::atomic<uint64_t> allowed{0};  // a bit a device
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
-  kernel<<<grid, block, smem, stream>>>(arguments...);
-  return cudaGetLastError();
+  const uint64_t bit = uint64_t{1} << (device % 64);
+  if ((allowed.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
+  if constexpr (Backward)
+    e = cudaFuncSetAttribute(norm_backward_kernel<L, TR, T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kStagedBytes / L::Resident);
+  else
+    e = cudaFuncSetAttribute(norm_kernel<L, TR, T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kStagedBytes / (L::Most <= 256 ? 4 : 1));
+  if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 template <typename TR, typename T>
@@ -697,9 +709,13 @@ cudaError_t forward(const fhb_norm_problem& p, void* total, void* normed, float*
   return with_layout<false>(wide, p.width, [&](auto layout) {
     using L = decltype(layout);
     if constexpr (L::Lanes == 0 && L::Wide)
-      if (args.stages > 0)
-        return launch_staged(norm_kernel<L, TR, T, true>, grid, block_of(threads), args.stages * row_bytes,
-                             stream, args, static_cast<TR*>(total), static_cast<T*>(normed), stats);
+      if (args.stages > 0) {
+        const cudaError_t e = allow_staged<false, L, TR, T>();
+        if (e != cudaSuccess) return e;
+        norm_kernel<L, TR, T, true><<<grid, block_of(threads), args.stages * row_bytes, stream>>>(
+            args, static_cast<TR*>(total), static_cast<T*>(normed), stats);
+        return cudaGetLastError();
+      }
     norm_kernel<L, TR, T, false><<<grid, block_of(threads), 0, stream>>>(
         args, static_cast<TR*>(total), static_cast<T*>(normed), stats);
     return cudaGetLastError();
@@ -735,9 +751,13 @@ cudaError_t backward(const fhb_norm_problem& p, const NormGrads& g, const Units&
   const cudaError_t e = with_layout<true>(wide, p.width, [&](auto layout) {
     using L = decltype(layout);
     if constexpr (L::Lanes == 0 && L::Wide)
-      if (args.stages > 0)
-        return launch_staged(norm_backward_kernel<L, TR, T, true>, static_cast<unsigned>(u.grid),
-                             block_of(threads), args.stages * row_bytes, stream, args, g, u, stats);
+      if (args.stages > 0) {
+        const cudaError_t allowed = allow_staged<true, L, TR, T>();
+        if (allowed != cudaSuccess) return allowed;
+        norm_backward_kernel<L, TR, T, true>
+            <<<static_cast<unsigned>(u.grid), block_of(threads), args.stages * row_bytes, stream>>>(args, g, u, stats);
+        return cudaGetLastError();
+      }
     norm_backward_kernel<L, TR, T, false>
         <<<static_cast<unsigned>(u.grid), block_of(threads), smem, stream>>>(args, g, u, stats);
     return cudaGetLastError();

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -225,3 +226,45 @@ def test_workspace_size_of_a_refused_norm(change):
         return _native.library().fhb_residual_norm_workspace_bytes(ctypes.byref(problem))
 
     assert size() > 0 and size(**change) == 0
+
+
+# ---- two host threads ----
+
+
+def norm_call(width, rows=200):
+    """A call of the C ABI on tensors and a stream of its own."""
+    stream = torch.cuda.Stream()
+    x, b, total, normed = (torch.randn(rows, width, device="cuda") for _ in range(4))
+    weight = torch.ones(width, device="cuda")
+    torch.cuda.synchronize()
+    problem = _native.NormProblem(
+        rows=rows, width=width, residual_dtype=0, dtype=0, residual=x.data_ptr(), branch=b.data_ptr(),
+        pre_weight=weight.data_ptr(), residual_stride=width, branch_stride=width, gate_rows=rows,
+        residual_scale=1.0, eps=1e-6)
+    keep = (stream, x, b, total, normed, weight)
+
+    def call():
+        return _native.library().fhb_residual_norm(
+            ctypes.byref(problem), keep[3].data_ptr(), keep[4].data_ptr(), None, stream.cuda_stream)
+
+    return call
+
+
+def test_two_threads_with_rows_of_different_bytes():
+    """Both calls use one kernel, with 160 and 192 KB of shared memory."""
+    failed = []
+
+    def work(call):
+        for _ in range(4000):
+            code = call()
+            if code != 0:
+                failed.append(code)
+
+    threads = [threading.Thread(target=work, args=(norm_call(w),)) for w in (5120, 8192, 5120, 8192)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, (len(failed), failed[:3])
+    assert fused_hoad.read_device_status(0) == 0
