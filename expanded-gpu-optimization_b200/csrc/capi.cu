@@ -48,7 +48,6 @@ int prepare_locked(int device) {
     if ((e = cudaGetSymbolAddress(reinterpret_cast<void**>(&info.status), g_status_word)) != cudaSuccess ||
         (e = fhb::prepare_forward_fp32()) != cudaSuccess ||
         (e = fhb::prepare_forward_tc()) != cudaSuccess ||
-        (e = fhb::prepare_gemm_tc()) != cudaSuccess ||
         (e = fhb::prepare_backward_fp32()) != cudaSuccess ||
         (e = fhb::prepare_backward_tc()) != cudaSuccess ||
         (e = fhb::prepare_biharmonic()) != cudaSuccess) {

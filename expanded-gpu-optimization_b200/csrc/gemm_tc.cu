@@ -10,6 +10,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -1104,7 +1105,18 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiled g_encode = nullptr;
+// The driver's encoder, looked up with the first product: null where the driver has none.
+EncodeTiled encoder() {
+  static const EncodeTiled found = [] {
+    void* entry = nullptr;
+    cudaDriverEntryPointQueryResult result;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000,
+                                                           cudaEnableDefault, &result);
+    return e == cudaSuccess && result == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeTiled>(entry)
+                                                                     : nullptr;
+  }();
+  return found;
+}
 
 // Tiles of 64 columns (128 bytes, swizzled) by `box_rows` rows of `box_planes` planes.
 bool tile_map(const TcMatrix& x, int box_rows, int box_planes, CUtensorMap* out) {
@@ -1114,8 +1126,10 @@ bool tile_map(const TcMatrix& x, int box_rows, int box_planes, CUtensorMap* out)
                                  static_cast<cuuint64_t>(x.planes > 1 ? x.plane : x.stride) * 2};
   const cuuint32_t box[3] = {kKBlock, static_cast<cuuint32_t>(box_rows),
                              static_cast<cuuint32_t>(box_planes)}, step[3] = {1, 1, 1};
+  const EncodeTiled encode_tiled = encoder();
+  if (encode_tiled == nullptr) return false;
   const auto encode = [&] {
-    return g_encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<bf16*>(x.p), size, strides,
+    return encode_tiled(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<bf16*>(x.p), size, strides,
                     box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   };
@@ -1130,9 +1144,27 @@ size_t smem_bytes(const Plan& plan) {
   return static_cast<size_t>(plan.slots) * plan.slot_bytes + (plan.cut_rows ? kATileBytes : 0) + 1024;
 }
 
+// Lets a kernel have the ring's shared memory, with its first launch on a device: callers of the
+// library's other operators do not wait for these kernels to load.
+template <int Cg, TcEpilogue E, typename T, int Jobs>
+cudaError_t allow_ring() {
+  static std::atomic<uint64_t> allowed{0};  // a bit a device
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = uint64_t{1} << (device % 64);
+  if ((allowed.load(std::memory_order_acquire) & bit) != 0) return cudaSuccess;
+  e = cudaFuncSetAttribute(gemm_tc_kernel<Cg, E, T, Jobs>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           kRingBytes + 1024);
+  if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 template <int Cg, TcEpilogue E, typename T, int Jobs>
 cudaError_t launch(const Maps<Jobs>& maps, const Args<Jobs>& args, const Plan& plan, bool dependent,
                    cudaStream_t stream) {
+  const cudaError_t e = allow_ring<Cg, E, T, Jobs>();
+  if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];
   int attrs = 0;
   if (Cg == 2) {
@@ -1165,37 +1197,6 @@ cudaError_t launch_kind(bool wide, const Maps<Jobs>& maps, const Args<Jobs>& arg
   return plan.cg == 2 ? launch<2, E, bf16>(maps, args, plan, dependent, stream)
                       : launch<1, E, bf16>(maps, args, plan, dependent, stream);
 }
-
-template <TcEpilogue E, int Jobs>
-cudaError_t prepare_kind() {
-  const void* const kernels[] = {reinterpret_cast<const void*>(gemm_tc_kernel<1, E, float, Jobs>),
-                                 reinterpret_cast<const void*>(gemm_tc_kernel<2, E, float, Jobs>),
-                                 reinterpret_cast<const void*>(gemm_tc_kernel<1, E, bf16, Jobs>),
-                                 reinterpret_cast<const void*>(gemm_tc_kernel<2, E, bf16, Jobs>)};
-  for (const void* kernel : kernels) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes + 1024);
-    if (e != cudaSuccess) return e;
-  }
-  return cudaSuccess;
-}
-
-}  // namespace
-
-cudaError_t prepare_gemm_tc() {
-  void* entry = nullptr;
-  cudaDriverEntryPointQueryResult found;
-  cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000,
-                                                   cudaEnableDefault, &found);
-  if (e != cudaSuccess) return e;
-  if (found != cudaDriverEntryPointSuccess || entry == nullptr) return cudaErrorSymbolNotFound;
-  g_encode = reinterpret_cast<EncodeTiled>(entry);
-  for (auto prepare : {prepare_kind<TcEpilogue::kStore, 1>, prepare_kind<TcEpilogue::kStore, kTcMaxProducts>,
-                       prepare_kind<TcEpilogue::kGate, 1>, prepare_kind<TcEpilogue::kGateGrad, 1>})
-    if ((e = prepare()) != cudaSuccess) return e;
-  return cudaSuccess;
-}
-
-namespace {
 
 // Short products go into one launch (see gemm_tc.cuh).
 bool shares_launch(const Plan& plan) { return plan.cycles < 60000.0; }  // about 35 us

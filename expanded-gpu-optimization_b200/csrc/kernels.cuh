@@ -154,9 +154,6 @@ cudaError_t launch_forward_tc(const float* coords, const float* params, float* u
                               int64_t n, bool f16, int activation, const DeviceInfo& dev,
                               cudaStream_t stream);
 
-// ---- gemm_tc.cu (gemm_tc.cuh) ----
-cudaError_t prepare_gemm_tc();
-
 // ---- biharmonic.cu ----
 cudaError_t prepare_biharmonic();
 // (u, Laplacian, biharmonic) of the tanh MLP, FP32 CUDA cores.

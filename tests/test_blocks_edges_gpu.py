@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import ctypes
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -268,3 +270,44 @@ def test_two_threads_with_rows_of_different_bytes():
     torch.cuda.synchronize()
     assert not failed, (len(failed), failed[:3])
     assert fused_hoad.read_device_status(0) == 0
+
+
+FIRST_CALLS = """
+import ctypes, sys, threading
+sys.path[:0] = {path!r}
+import torch
+from fused_hoad import _native
+
+def call(results, k):
+    torch.cuda.set_device(0)
+    stream = torch.cuda.Stream()
+    t = [torch.full(s, 0.5, device="cuda") for s in ((64, 32), (16, 32), (16, 32), (32, 16), (64, 32))]
+    p = _native.FfnProblem(tokens=64, width=32, hidden=16, out_width=32, dtype=0, activation=1,
+                           x=t[0].data_ptr(), w_gate=t[1].data_ptr(), w_up=t[2].data_ptr(),
+                           w_down=t[3].data_ptr(), x_stride=32, w_gate_stride=32, w_up_stride=32,
+                           w_down_stride=16)
+    torch.cuda.synchronize()
+    barrier.wait(60)
+    lib = _native.library()
+    size = lib.fhb_ffn_workspace_bytes(ctypes.byref(p), 0)
+    room = torch.empty(size, device="cuda", dtype=torch.uint8)
+    code = lib.fhb_ffn_forward(ctypes.byref(p), t[4].data_ptr(), None, room.data_ptr(), size,
+                               stream.cuda_stream)
+    torch.cuda.synchronize()
+    g = 32 * 0.25
+    want = 16 * 0.5 * g * g / (1 + 2.718281828459045 ** -g)
+    results[k] = (code, bool(torch.allclose(t[4], torch.full_like(t[4], want), rtol=1e-5)))
+
+barrier, results = threading.Barrier(4), [None] * 4
+threads = [threading.Thread(target=call, args=(results, k)) for k in range(4)]
+for t in threads: t.start()
+for t in threads: t.join()
+assert results == [(0, True)] * 4, results
+"""
+
+
+def test_first_calls_of_several_threads():
+    """What a product sets up with its first call, in a process of its own."""
+    script = FIRST_CALLS.format(path=[p for p in sys.path if p])
+    run = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
