@@ -72,6 +72,8 @@ cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, in
 // ---- residual_norm.cu ----
 cudaError_t launch_residual_norm(const fhb_norm_problem& p, void* total, void* normed,
                                  float* stats, const DeviceInfo& dev, cudaStream_t stream);
+cudaError_t launch_staged_wait_selftest(const float* rows, float* out, const DeviceInfo& dev,
+                                        cudaStream_t stream);
 size_t residual_norm_workspace_bytes(const fhb_norm_problem& p, const DeviceInfo& dev);
 cudaError_t launch_residual_norm_backward(const fhb_norm_problem& p, const void* grad_total,
                                           int64_t grad_total_stride, const void* grad_normed,

@@ -203,6 +203,15 @@ int fhb_residual_norm_backward(const fhb_norm_problem* problem, const void* grad
       workspace, *dev, stream));
 }
 
+int fhb_debug_staged_wait_selftest(const float* rows, float* out, fhb_stream_t stream) {
+  if (rows == nullptr || out == nullptr) return FHB_ERR_INVALID_ARGUMENT;
+  if (!aligned(rows, 16) || !aligned(out, 4)) return FHB_ERR_MISALIGNED;
+  const fhb::DeviceInfo* dev = nullptr;
+  const int code = fhb::current_device_info(&dev);
+  if (code != FHB_OK) return code;
+  return fhb::record_cuda_error(fhb::launch_staged_wait_selftest(rows, out, *dev, stream));
+}
+
 int fhb_adamw_step(const fhb_adamw_tensor* tensors, int64_t n_tensors, int state_bits,
                    int64_t* step, double lr, double beta1, double beta2, double eps,
                    double weight_decay, fhb_stream_t stream) {

@@ -38,7 +38,9 @@ struct NormArgs {
 
 // Rows on their way (a CTA a row, aligned rows): one thread starts the bulk copies of a row's
 // arrays into shared memory `stages` rows ahead, so that what is in flight takes no registers.
-// A stage is free again when the CTA has met in the row's sums, after everybody read it.
+// A stage is free again when the CTA has met in the row's sums, after everybody read it. Where a wait
+// gives up (the status says so), that thread waits no more; thread 0 starts no more copies either and
+// at the end waits for those on their way, since the memory is another CTA's when this one is gone.
 constexpr int kMaxStages = 4;
 constexpr int kMaxArrays = 5;
 struct Stage {
@@ -46,7 +48,7 @@ struct Stage {
   unsigned char* base;
   int stages, at;
   uint32_t phase, bytes;  // of the arrays of one row
-  bool late;              // a wait gave up: no more waits, the status says so
+  bool late;              // a wait gave up
   unsigned int* status;
 
   __device__ __forceinline__ void start(unsigned char* memory, uint64_t* barriers, int count,
@@ -67,7 +69,8 @@ struct Stage {
   }
   // one thread: the arrays of a row into stage `into`
   __device__ __forceinline__ void copy(int into, const void* const (&from)[kMaxArrays],
-                                       const uint32_t (&size)[kMaxArrays]) const {
+                                       const uint32_t (&size)[kMaxArrays]) {
+    if (late) return;
     mbar_arrive_expect_tx(&full[into], bytes);
     unsigned char* to = base + into * bytes;
 #pragma unroll
@@ -80,6 +83,12 @@ struct Stage {
   __device__ __forceinline__ const unsigned char* wait() {
     if (!late) late = !mbar_wait_bounded(&full[at], phase, status, FHB_STATUS_STAGE_TIMEOUT);
     return base + at * bytes;
+  }
+  // after the last row: whatever is still on its way has landed, or had as long again
+  __device__ __forceinline__ void finish() const {
+    if (threadIdx.x != 0 || !late) return;
+    for (int i = 0; i < stages; ++i)
+      mbar_wait_bounded(&full[i], mbar_try_wait(&full[i], 0) ? 1 : 0, status, FHB_STATUS_STAGE_TIMEOUT);
   }
   __device__ __forceinline__ void next() {
     if (++at == stages) {
@@ -310,6 +319,7 @@ __global__ void __launch_bounds__(L::Most, L::Most <= 256 ? 4 : 1)
       stats[2 * row + 1] = it;
     }
   }
+  if (Staged) stage.finish();
 }
 
 // ---- backward ----
@@ -470,6 +480,7 @@ __global__ void __launch_bounds__(L::Most, L::Resident)
       fill<L>(sgate, 0.0f);
     }
   }
+  if (Staged) stage.finish();
   // the CTA's column sums: its slots' one after the other
   float* columns = reinterpret_cast<float*>(rows_memory);
   float* out = g.columns + static_cast<int64_t>(blockIdx.x) * 3 * a.width;
@@ -575,6 +586,40 @@ __global__ void __launch_bounds__(256) norm_totals_kernel(Totals t) {
     s = 0.0f;
     for (int k = 0; k < 8; ++k) s += by_group[k][lane];
     out[c] = from_float<T>(s);
+  }
+}
+
+// Test hook: three rows of 1 KB on their way, of which the first is said to be longer than it is, so
+// that the wait for it gives up. out: whether it did; which of the three have landed by then, as bits;
+// whether a row started after it lands.
+__global__ void staged_wait_selftest_kernel(const float* rows, float* out, unsigned int* status) {
+  constexpr int kRowBytes = 1024, kCount = 3;
+  __shared__ __align__(16) unsigned char memory[kCount * kRowBytes];
+  __shared__ uint64_t full[kMaxStages];
+  const uint32_t size[kMaxArrays] = {kRowBytes, 0, 0, 0, 0};
+  Stage stage;
+  stage.start(memory, full, kCount, kRowBytes, status);
+  const auto send = [&](int into) {
+    const void* const from[kMaxArrays] = {rows + into * (kRowBytes / 4), nullptr, nullptr, nullptr, nullptr};
+    stage.copy(into, from, size);
+  };
+  if (threadIdx.x == 0)
+    for (int i = 0; i < kCount; ++i) {
+      stage.bytes = kRowBytes + (i == 0 ? 16 : 0);
+      send(i);
+    }
+  stage.bytes = kRowBytes;
+  stage.wait();
+  stage.finish();
+  if (threadIdx.x == 0) {
+    int landed = 0;
+    for (int i = 0; i < kCount; ++i) landed |= (mbar_try_wait(&full[i], 0) ? 1 : 0) << i;
+    out[0] = stage.late ? 1.0f : 0.0f;
+    out[1] = static_cast<float>(landed);
+    send(1);
+    bool more = false;
+    for (int i = 0; i < 10; ++i) more = more || mbar_try_wait_for(&full[1], 1, kSuspendHintNs);
+    out[2] = more ? 1.0f : 0.0f;
   }
 }
 
@@ -777,6 +822,12 @@ cudaError_t launch_residual_norm(const fhb_norm_problem& p, void* total, void* n
     return p.dtype == FHB_DTYPE_F32 ? forward<float, float>(p, total, normed, stats, dev, stream)
                                     : forward<float, bf16>(p, total, normed, stats, dev, stream);
   return forward<bf16, bf16>(p, total, normed, stats, dev, stream);
+}
+
+cudaError_t launch_staged_wait_selftest(const float* rows, float* out, const DeviceInfo& dev,
+                                        cudaStream_t stream) {
+  staged_wait_selftest_kernel<<<1, 64, 0, stream>>>(rows, out, dev.status);
+  return cudaGetLastError();
 }
 
 size_t residual_norm_workspace_bytes(const fhb_norm_problem& p, const DeviceInfo& dev) {

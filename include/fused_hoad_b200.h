@@ -40,7 +40,7 @@ typedef struct CUstream_st* fhb_stream_t;
 #define FHB_ERR_TOO_LARGE 6        /* size beyond what the entry point supports */
 
 /* Bits of the per-device status word a kernel sets when a bounded wait gives up. */
-#define FHB_STATUS_STAGE_TIMEOUT 0x1u /* parameter staging copy never completed */
+#define FHB_STATUS_STAGE_TIMEOUT 0x1u /* a copy into shared memory never completed */
 #define FHB_STATUS_MMA_TIMEOUT 0x2u   /* tensor-core pipeline wait gave up */
 #define FHB_STATUS_PEER_TIMEOUT 0x4u  /* an exchange wait for a peer rank gave up */
 #define FHB_STATUS_SELFTEST 0x80u     /* set by fhb_debug_bounded_wait_selftest */
@@ -423,6 +423,15 @@ int fhb_read_device_status(int device, unsigned int* status_out);
  * FHB_STATUS_SELFTEST in the device status word and the kernel returns normally.
  */
 int fhb_debug_bounded_wait_selftest(uint64_t limit_ns, fhb_stream_t stream);
+
+/*
+ * Test hook for the norms' rows on their way: one CTA starts the copies of three rows of 1 KB (`rows`,
+ * 768 floats, 16-byte aligned), the first with a barrier that never completes. Its wait gives up after
+ * its limit (a second), the others' copies are waited for, FHB_STATUS_STAGE_TIMEOUT is set and the
+ * kernel returns. out (3 floats): 1 if the wait gave up; the rows that have landed, as bits; 1 if a row
+ * that is started after it lands.
+ */
+int fhb_debug_staged_wait_selftest(const float* rows, float* out, fhb_stream_t stream);
 
 /*
  * Test hook for the tensor-core kernel's tanh: out[i] = tanh_fast(x[i]) when fast != 0

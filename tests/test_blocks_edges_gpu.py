@@ -311,3 +311,25 @@ def test_first_calls_of_several_threads():
     script = FIRST_CALLS.format(path=[p for p in sys.path if p])
     run = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stderr[-2000:]
+
+
+# ---- waits that give up ----
+
+
+def test_a_row_that_never_lands():
+    """The wait gives up and says so, the copies on their way are waited for, no more are started,
+    and the context stays usable."""
+    library = _native.library()
+    assert fused_hoad.read_device_status(0) == 0
+    rows, out = torch.zeros(768, device="cuda"), torch.full((3,), -1.0, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    assert library.fhb_debug_staged_wait_selftest(rows.data_ptr(), None, stream) == 1
+    assert library.fhb_debug_staged_wait_selftest(rows.data_ptr() + 4, out.data_ptr(), stream) == 2
+    assert library.fhb_debug_staged_wait_selftest(rows.data_ptr(), out.data_ptr(), stream) == 0
+    torch.cuda.synchronize()
+    assert out.tolist() == [1.0, float(0b110), 0.0]
+    assert fused_hoad.read_device_status(0) == 1  # FHB_STATUS_STAGE_TIMEOUT
+    x = torch.randn(700, 2048, device="cuda")
+    y = fused_hoad.rms_norm(x, torch.ones(2048, device="cuda"), 0.0)
+    assert torch.allclose(y.square().mean(1), torch.ones(700, device="cuda"), rtol=1e-4)
+    assert fused_hoad.read_device_status(0) == 0
