@@ -581,9 +581,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      // the last copies have landed before this CTA's memory is given up (as far as they can be
-      // seen from here: the pair's barriers are in CTA 0, which waits for them in its MMAs)
-      if (!ok && rank == 0)
+      // the last copies have landed before this CTA's memory is given up, also where a wait gave up
+      // (a pair's barriers are in CTA 0, and its CTAs leave together)
+      if (rank == 0)
         for (int s = 0; s < p.slots && issued > 0; ++s, --issued) {
           slot = slot == 0 ? p.slots - 1 : slot - 1;
           if (slot == p.slots - 1) phase ^= 1;
@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int slot = 0;
       uint32_t phase = 0;
       int64_t sums = 0;
-      bool ok = true;
+      bool ok = true, begun = false;
       // (operand across K: bytes from one block of 64 rows to the next)
       const uint64_t a_desc = tile_descriptor(0, kCopies * 8192), b_desc = a_desc;
       for (uint32_t index = first; ok && index < items; index += stride) {
@@ -652,6 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
               }
               commit<Cg>(&empty[slot]);
+              begun = true;
               if (++slot == p.slots) {
                 slot = 0;
                 phase ^= 1;
@@ -659,6 +660,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           if (ok) commit<Cg>(&sum_full[buffer]);
         }
+      }
+      // the last MMAs are done before their accumulators and operands are given up, likewise
+      if (begun) {
+        slot = slot == 0 ? p.slots - 1 : slot - 1;
+        if (slot == p.slots - 1) phase ^= 1;
+        mbar_wait_bounded(&empty[slot], phase, p.status, FHB_STATUS_MMA_TIMEOUT);
       }
     }
     __syncwarp();

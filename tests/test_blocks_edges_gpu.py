@@ -333,3 +333,23 @@ def test_a_row_that_never_lands():
     y = fused_hoad.rms_norm(x, torch.ones(2048, device="cuda"), 0.0)
     assert torch.allclose(y.square().mean(1), torch.ones(700, device="cuda"), rtol=1e-4)
     assert fused_hoad.read_device_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_products_wait_for_their_last_copies_and_sums(dtype):
+    """Every product ends by waiting for the copies and sums of its last ring slots: a wait on a
+    phase that never comes would set the status word and take a second. One CTA a tile and pairs,
+    fewer blocks of K than slots and many times more, parts of K, several products a launch."""
+    assert fused_hoad.read_device_status(0) == 0
+    for tokens, width, hidden in [(9, 8, 8), (100, 64, 64), (130, 72, 40), (300, 1000, 24), (520, 64, 1030),
+                                  (2000, 512, 512), (4100, 520, 1100), (33, 4000, 64), (20000, 64, 256)]:
+        leaves = [torch.randn(s, device="cuda").to(dtype).requires_grad_()
+                  for s in ((tokens, width), (hidden, width), (hidden, width), (width, hidden))]
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        y = fused_hoad.gated_feed_forward(*leaves)
+        torch.autograd.grad(y, leaves, torch.ones_like(y))
+        end.record()
+        end.synchronize()
+        assert start.elapsed_time(end) < 500.0, (tokens, width, hidden)
+    assert fused_hoad.read_device_status(0) == 0
