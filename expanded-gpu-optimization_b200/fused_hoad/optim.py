@@ -66,9 +66,10 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits`` 32 keeps float32 moments (8 bytes a parameter), 8 keeps e4m3 codes with one
     scale for each 256 values (2.03 bytes a parameter). Parameters are float32 or bfloat16,
-    contiguous, and all on one CUDA device; those without a gradient are skipped. Each parameter
-    group has one step counter, on the device: every parameter of a group is meant to get its
-    first gradient in the same step.
+    contiguous, and all on one CUDA device; those without a gradient are skipped. Every parameter
+    counts its own steps, on the device; those of a group that have had their gradients in the
+    same steps share a counter and a launch. A step with new parameters, or with fewer than share
+    a counter, is taken once before one like it is captured in a CUDA graph.
     """
 
     def __init__(
@@ -92,22 +93,45 @@ class AdamW(torch.optim.Optimizer):
         if not weight_decay >= 0.0:
             raise ValueError("weight_decay must be >= 0")
         defaults = dict(lr=float(lr), betas=(float(betas[0]), float(betas[1])), eps=float(eps),
-                        weight_decay=float(weight_decay), state_bits=state_bits, step=None,
-                        capturable=True)
+                        weight_decay=float(weight_decay), state_bits=state_bits, capturable=True)
         super().__init__(params, defaults)
 
-    def _state_of(self, p: Tensor, state_bits: int) -> dict:
+    def _new_state(self, p: Tensor, state_bits: int, step: Tensor) -> None:
         state = self.state[p]
-        if not state:
-            if state_bits == 32:
-                state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
-                state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
-            else:
-                blocks = -(-p.numel() // ADAMW_BLOCK)
-                for name in ("exp_avg", "exp_avg_sq"):
-                    state[name] = torch.zeros_like(p, dtype=torch.float8_e4m3fn)
-                    state[name + "_scale"] = torch.zeros(blocks, device=p.device)
-        return state
+        state["step"] = step
+        if state_bits == 32:
+            state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+            state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+        else:
+            blocks = -(-p.numel() // ADAMW_BLOCK)
+            for name in ("exp_avg", "exp_avg_sq"):
+                state[name] = torch.zeros_like(p, dtype=torch.float8_e4m3fn)
+                state[name + "_scale"] = torch.zeros(blocks, device=p.device)
+
+    def _by_counter(self, group: dict) -> list[tuple[Tensor, list[Tensor]]]:
+        """The parameters with a gradient, by the step counter that they share. Those that share
+        one with a parameter that has none now get a counter of their own."""
+        params = [p for p in group["params"] if p.grad is not None]
+        new = [p for p in params if not self.state.get(p)]
+        idle = {id(self.state[p]["step"]) for p in group["params"] if p.grad is None and self.state.get(p)}
+        if new:
+            _refuse_capture(params[0])
+            counter = torch.zeros(1, dtype=torch.int64, device=params[0].device)
+            for p in new:
+                self._new_state(p, group["state_bits"], counter)
+        shared: dict[int, tuple[Tensor, list[Tensor]]] = {}
+        for p in params:
+            counter = self.state[p]["step"]
+            shared.setdefault(id(counter), (counter, []))[1].append(p)
+        result = []
+        for key, (counter, members) in shared.items():
+            if key in idle:
+                _refuse_capture(params[0])
+                counter = counter.clone()
+                for p in members:
+                    self.state[p]["step"] = counter
+            result.append((counter, members))
+        return result
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -116,35 +140,51 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
-            params = [p for p in group["params"] if p.grad is not None]
-            if not params:
-                continue
-            if group["step"] is None:
-                group["step"] = torch.zeros(1, dtype=torch.int64, device=params[0].device)
-            states = [self._state_of(p, group["state_bits"]) for p in params]
-            scales = {}
-            if group["state_bits"] == 8:
-                scales = {"exp_avg_scales": [s["exp_avg_scale"] for s in states],
-                          "exp_avg_sq_scales": [s["exp_avg_sq_scale"] for s in states]}
-            adamw_step(
-                params, [p.grad.contiguous() for p in params], [s["exp_avg"] for s in states],
-                [s["exp_avg_sq"] for s in states], group["step"], lr=group["lr"],
-                betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
-                **scales,
-            )
+            for counter, params in self._by_counter(group):
+                states = [self.state[p] for p in params]
+                scales = {}
+                if group["state_bits"] == 8:
+                    scales = {"exp_avg_scales": [s["exp_avg_scale"] for s in states],
+                              "exp_avg_sq_scales": [s["exp_avg_sq_scale"] for s in states]}
+                adamw_step(
+                    params, [p.grad.contiguous() for p in params], [s["exp_avg"] for s in states],
+                    [s["exp_avg_sq"] for s in states], counter, lr=group["lr"],
+                    betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                    **scales,
+                )
         return loss
 
     def load_state_dict(self, state_dict) -> None:
         """As ``torch.optim.Optimizer.load_state_dict``; the moments keep their own types (that
-        method would cast floating-point state to the parameter's type)."""
+        method would cast floating-point state to the parameter's type). Takes the states of
+        ``torch.optim.AdamW`` too (without ``amsgrad`` and ``maximize``), and those with one
+        counter for a group. Waits for the device to read the counters."""
+        for group in state_dict["param_groups"]:
+            if group.get("amsgrad") or group.get("maximize"):
+                raise ValueError("amsgrad and maximize are not supported")
         super().load_state_dict(state_dict)
         saved = state_dict["state"]
         for group, saved_group in zip(self.param_groups, state_dict["param_groups"]):
+            of_group = group.pop("step", None)
+            group.setdefault("state_bits", 32)
+            counters: dict[int, Tensor] = {}
             for p, index in zip(group["params"], saved_group["params"]):
-                if index in saved:
-                    self.state[p] = {
-                        name: value.to(p.device, copy=True) if isinstance(value, Tensor) else value
-                        for name, value in saved[index].items()
-                    }
-            if isinstance(group["step"], Tensor) and group["params"]:
-                group["step"] = group["step"].to(group["params"][0].device, copy=True)
+                if not saved.get(index):
+                    continue
+                state = {}
+                for name, value in saved[index].items():
+                    if isinstance(value, Tensor):
+                        moment = group["state_bits"] == 32 and name in ("exp_avg", "exp_avg_sq")
+                        value = value.to(p.device, torch.float32 if moment else None, copy=True)
+                    state[name] = value
+                count = int(state.get("step", of_group))
+                if count not in counters:
+                    counters[count] = torch.full((1,), count, dtype=torch.int64, device=p.device)
+                state["step"] = counters[count]
+                self.state[p] = state
+
+
+def _refuse_capture(p: Tensor) -> None:
+    """What is made while a graph is captured would be made anew by every replay."""
+    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the optimizer's states are made by a step before the captured one")
