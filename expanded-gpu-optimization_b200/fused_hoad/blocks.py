@@ -82,12 +82,25 @@ def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6) -> Tensor:
     return _norm(x, None, weight, None, None, 1.0, eps)[0]
 
 
+class _Float32Parameters(nn.ParameterList):
+    """Parameters that stay float32 when their module's type is changed."""
+
+    def _apply(self, fn, recurse=True):
+        def move(t: Tensor) -> Tensor:
+            moved = fn(t)
+            return moved if moved.dtype == t.dtype else t.to(moved.device)
+
+        return super()._apply(move, recurse)
+
+
 class GatedResidualTrunk(nn.Module):
     """A deep trunk for point-wise problems: ``Linear``, ``blocks`` gated feed-forward blocks
     with norms before and after, a gate per channel and a learned residual scale, a last norm
     and a ``Linear``. ``[..., input_dim] -> [..., output_dim]``, float32 or bfloat16.
 
-    The gates start at ``gate_init``, so that a deep trunk starts near its first layer.
+    The gates start at ``gate_init``, so that a deep trunk starts near its first layer. The residual
+    scales stay float32 whatever the trunk's type: they stay near 1, where bfloat16's steps are
+    larger than an optimizer's.
     """
 
     def __init__(
@@ -119,7 +132,7 @@ class GatedResidualTrunk(nn.Module):
         self.post = nn.ParameterList(torch.ones(width) for _ in range(blocks))
         self.channel_gate = nn.ParameterList(torch.full((width,), gate_init) for _ in range(blocks))
         self.pre = nn.ParameterList(torch.ones(width) for _ in range(blocks))
-        self.scale = nn.ParameterList(torch.ones(1) for _ in range(blocks))
+        self.scale = _Float32Parameters(torch.ones(1) for _ in range(blocks))
         self.decode = nn.Linear(width, output_dim)
 
     def forward(self, x: Tensor) -> Tensor:
@@ -130,9 +143,8 @@ class GatedResidualTrunk(nn.Module):
                 normed, self.gate[k].weight, self.up[k].weight, self.down[k].weight,
                 self.gate[k].bias, self.up[k].bias, self.down[k].bias, self.activation,
             )
-            # the scale is kept in float32 whatever the trunk's type
             stream, normed = residual_norm(
-                stream, branch, self.pre[k], self.post[k], self.channel_gate[k],
-                self.scale[k].float(), self.eps,
+                stream, branch, self.pre[k], self.post[k], self.channel_gate[k], self.scale[k],
+                self.eps,
             )
         return self.decode(normed)

@@ -353,3 +353,23 @@ def test_products_wait_for_their_last_copies_and_sums(dtype):
         end.synchronize()
         assert start.elapsed_time(end) < 500.0, (tokens, width, hidden)
     assert fused_hoad.read_device_status(0) == 0
+
+
+# ---- a trunk's residual scales ----
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_scales_of_a_bfloat16_trunk_move(bits):
+    """Steps of 1e-3 add up next to 1, where bfloat16's own are 2^-8 and 2^-7."""
+    torch.manual_seed(0)
+    trunk = fused_hoad.GatedResidualTrunk(2, 32, 64, 2).cuda().bfloat16()
+    optimizer = fused_hoad.AdamW(trunk.parameters(), lr=1e-3, weight_decay=0.0, state_bits=bits)
+    x = torch.rand(500, 2, device="cuda").bfloat16()
+    for k in range(3):
+        optimizer.zero_grad(set_to_none=True)
+        trunk(x).float().square().mean().backward()
+        before = [s.detach().clone() for s in trunk.scale]
+        assert all(s.grad.dtype == torch.float32 and bool(s.grad) for s in trunk.scale)
+        optimizer.step()
+        for s, b in zip(trunk.scale, before):
+            assert s.dtype == torch.float32 and 0 < float((s - b).abs()) <= 1.1e-3
