@@ -174,7 +174,8 @@ torch::Tensor ffn_forward(const Ffn& f, const torch::Tensor& x, torch::Tensor* s
   auto y = torch::empty(shape, x.options());
   if (saved != nullptr) *saved = bytes_for(fhb_ffn_saved_bytes(&f.problem), x);
   if (f.problem.tokens == 0) return y;
-  auto workspace = bytes_for(fhb_ffn_workspace_bytes(&f.problem, 0), x);
+  const int pass = saved != nullptr ? FHB_FFN_FORWARD_SAVING : FHB_FFN_FORWARD;
+  auto workspace = bytes_for(fhb_ffn_workspace_bytes(&f.problem, pass), x);
   check_status(fhb_ffn_forward(&f.problem, y.data_ptr(),
                                saved != nullptr ? saved->data_ptr() : nullptr, data_of(workspace),
                                static_cast<size_t>(workspace.numel()),
@@ -215,7 +216,7 @@ class FfnNode : public torch::autograd::Function<FfnNode> {
       if (t[i + 1].defined() && ctx->needs_input_grad(edge++)) out[i] = torch::empty(t[i + 1].sizes(), x.options());
     const auto place = [&](int i) { return out[i].defined() ? data_of(out[i]) : nullptr; };
     const fhb_ffn_grads grads{place(0), place(1), place(2), place(3), place(4), place(5), place(6)};
-    auto workspace = bytes_for(fhb_ffn_workspace_bytes(&p, 1), x);
+    auto workspace = bytes_for(fhb_ffn_workspace_bytes(&p, FHB_FFN_BACKWARD), x);
     check_status(fhb_ffn_backward(&p, data_of(dy), row_stride(dy), data_of(saved), &grads,
                                   data_of(workspace), static_cast<size_t>(workspace.numel()),
                                   at::cuda::getCurrentCUDAStream()),

@@ -62,7 +62,7 @@ __device__ __forceinline__ void block_activation(float g, float& a, float& slope
 
 // ---- gated_ffn.cu ----
 size_t ffn_saved_bytes(const fhb_ffn_problem& p);
-size_t ffn_workspace_bytes(const fhb_ffn_problem& p, bool backward, const DeviceInfo& dev);
+size_t ffn_workspace_bytes(const fhb_ffn_problem& p, int pass, const DeviceInfo& dev);  // FHB_FFN_*
 cudaError_t launch_ffn_forward(const fhb_ffn_problem& p, void* y, void* saved, void* workspace,
                                const DeviceInfo& dev, cudaStream_t stream);
 cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, int64_t grad_y_stride,

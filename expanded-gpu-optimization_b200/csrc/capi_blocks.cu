@@ -97,10 +97,12 @@ size_t fhb_ffn_saved_bytes(const fhb_ffn_problem* problem) {
   return check_ffn_sizes(problem) == FHB_OK ? fhb::ffn_saved_bytes(*problem) : 0;
 }
 
-size_t fhb_ffn_workspace_bytes(const fhb_ffn_problem* problem, int backward) {
+size_t fhb_ffn_workspace_bytes(const fhb_ffn_problem* problem, int pass) {
   const fhb::DeviceInfo* dev = nullptr;
-  if (check_ffn_sizes(problem) != FHB_OK || fhb::current_device_info(&dev) != FHB_OK) return 0;
-  return fhb::ffn_workspace_bytes(*problem, backward != 0, *dev);
+  if (check_ffn_sizes(problem) != FHB_OK || pass < FHB_FFN_FORWARD || pass > FHB_FFN_FORWARD_SAVING ||
+      fhb::current_device_info(&dev) != FHB_OK)
+    return 0;
+  return fhb::ffn_workspace_bytes(*problem, pass, *dev);
 }
 
 int fhb_ffn_forward(const fhb_ffn_problem* problem, void* y, void* saved, void* workspace,
@@ -114,7 +116,8 @@ int fhb_ffn_forward(const fhb_ffn_problem* problem, void* y, void* saved, void* 
   const fhb::DeviceInfo* dev = nullptr;
   code = fhb::current_device_info(&dev);
   if (code != FHB_OK) return code;
-  code = check_workspace(workspace, workspace_bytes, fhb::ffn_workspace_bytes(*problem, false, *dev));
+  const int pass = saved != nullptr ? FHB_FFN_FORWARD_SAVING : FHB_FFN_FORWARD;
+  code = check_workspace(workspace, workspace_bytes, fhb::ffn_workspace_bytes(*problem, pass, *dev));
   if (code != FHB_OK) return code;
   return fhb::record_cuda_error(
       fhb::launch_ffn_forward(*problem, y, saved, workspace, *dev, stream));
@@ -139,7 +142,7 @@ int fhb_ffn_backward(const fhb_ffn_problem* problem, const void* grad_y, int64_t
   const fhb::DeviceInfo* dev = nullptr;
   code = fhb::current_device_info(&dev);
   if (code != FHB_OK) return code;
-  code = check_workspace(workspace, workspace_bytes, fhb::ffn_workspace_bytes(*problem, true, *dev));
+  code = check_workspace(workspace, workspace_bytes, fhb::ffn_workspace_bytes(*problem, FHB_FFN_BACKWARD, *dev));
   if (code != FHB_OK) return code;
   return fhb::record_cuda_error(fhb::launch_ffn_backward(*problem, grad_y, grad_y_stride, saved,
                                                          *grads, workspace, *dev, stream));

@@ -28,15 +28,16 @@ struct Room {
   }
 };
 
-// What the forward keeps: h in operand form and the activation's factors.
+// What the forward makes: h in operand form, and for a backward the activation's factors.
 struct Saved {
   TcMatrix h;
   TcFactors factors;
 };
-Saved saved_in(const fhb_ffn_problem& p, Room& room) {
+Saved saved_in(const fhb_ffn_problem& p, Room& room, bool keep) {
   Saved s;
   s.h = tc_result(room.take(tc_result_bytes(p.tokens, p.hidden, p.dtype)), p.tokens, p.hidden, p.dtype);
-  s.factors = tc_factors(room.take(tc_factor_bytes(p.tokens, p.hidden, p.dtype)), p.tokens, p.hidden, p.dtype);
+  if (keep)
+    s.factors = tc_factors(room.take(tc_factor_bytes(p.tokens, p.hidden, p.dtype)), p.tokens, p.hidden, p.dtype);
   return s;
 }
 
@@ -171,7 +172,7 @@ Inputs inputs_in(const fhb_ffn_problem& p, const void* dy, int64_t dy_stride, Ro
   return x;
 }
 
-TcProduct gate_product(const fhb_ffn_problem& p, const Operands& o, const Saved& s, bool keep) {
+TcProduct gate_product(const fhb_ffn_problem& p, const Operands& o, const Saved& s) {
   TcProduct q;
   q.m = p.tokens, q.n = p.hidden, q.k = p.width;
   q.a[0] = o.x, q.b[0] = o.w_gate, q.b[1] = o.w_up;
@@ -179,7 +180,7 @@ TcProduct gate_product(const fhb_ffn_problem& p, const Operands& o, const Saved&
   q.dtype = p.dtype;
   q.bias[0] = p.b_gate, q.bias[1] = p.b_up;
   q.gated[0] = s.h;
-  if (keep) q.factors = s.factors;
+  q.factors = s.factors;
   q.activation = p.activation;
   return q;
 }
@@ -258,26 +259,28 @@ size_t column_bytes(const fhb_ffn_problem& p) {
 
 size_t ffn_saved_bytes(const fhb_ffn_problem& p) {
   Room room{nullptr};
-  saved_in(p, room);
+  saved_in(p, room, true);
   return room.used;
 }
 
-size_t ffn_workspace_bytes(const fhb_ffn_problem& p, bool backward, const DeviceInfo& dev) {
+size_t ffn_workspace_bytes(const fhb_ffn_problem& p, int pass, const DeviceInfo& dev) {
   Room room{nullptr};
   Operands o;
   if (p.tokens == 0) return 0;
-  if (!backward) {
+  if (pass != FHB_FFN_BACKWARD) {
+    const bool keep = pass == FHB_FFN_FORWARD_SAVING;
     inputs_in(p, nullptr, 0, room, o);
-    const Saved s = saved_in(p, room);
+    Room aside{nullptr};
+    const Saved s = saved_in(p, keep ? aside : room, keep);
     const TcProduct down = down_product(p, o, s, nullptr);
     room.take(gemm_tc_workspace_bytes(&down, 1, dev));
-    return std::max(room.used, ffn_small_bytes(p));
+    return keep ? room.used : std::max(room.used, ffn_small_bytes(p));
   }
   // the upstream gradient may need a copy: the size asked for does not depend on it
   inputs_in(p, nullptr, 0, room, o);
   room.take(tc_result_bytes(p.tokens, p.out_width, p.dtype));
   Room aside{nullptr};
-  const Saved s = saved_in(p, aside);
+  const Saved s = saved_in(p, aside, true);
   const Backward b = backward_of(p, o, s, all_grads(), room);
   room.take(column_bytes(p));
   room.take(gemm_tc_workspace_bytes(b.rest, kTcMaxProducts, dev));
@@ -294,8 +297,8 @@ cudaError_t launch_ffn_forward(const fhb_ffn_problem& p, void* y, void* saved, v
   bool packed = false;
   cudaError_t e = launch_pack(x.in, x.out, 5, p.dtype, &packed, stream);
   if (e != cudaSuccess) return e;
-  const Saved s = saved_in(p, saved != nullptr ? kept : room);
-  const TcProduct gate = gate_product(p, o, s, saved != nullptr);
+  const Saved s = saved_in(p, saved != nullptr ? kept : room, saved != nullptr);
+  const TcProduct gate = gate_product(p, o, s);
   e = launch_gemm_tc(&gate, 1, nullptr, packed, dev, stream);
   if (e != cudaSuccess) return e;
   const TcProduct down = down_product(p, o, s, y);
@@ -326,7 +329,7 @@ cudaError_t launch_ffn_backward(const fhb_ffn_problem& p, const void* grad_y, in
   bool packed = false;
   cudaError_t e = launch_pack(x.in, x.out, 5, p.dtype, &packed, stream);
   if (e != cudaSuccess) return e;
-  const Saved s = saved_in(p, kept);
+  const Saved s = saved_in(p, kept, true);
   const Backward b = backward_of(p, o, s, out, room);
   float* column_parts = static_cast<float*>(room.take(column_bytes(p)));
   void* sums = room.take(0);  // the rest

@@ -327,8 +327,12 @@ typedef struct fhb_ffn_grads {
 } fhb_ffn_grads;
 /* Bytes of the buffer in which the forward keeps what the backward needs (opaque). */
 size_t fhb_ffn_saved_bytes(const fhb_ffn_problem* problem);
-/* Workspace of the forward (backward == 0) or the backward call on the current device. */
-size_t fhb_ffn_workspace_bytes(const fhb_ffn_problem* problem, int backward);
+/* Workspace on the current device of a forward without `saved` (which holds h), of the backward, or
+ * of a forward that fills `saved`. */
+#define FHB_FFN_FORWARD 0
+#define FHB_FFN_BACKWARD 1
+#define FHB_FFN_FORWARD_SAVING 2
+size_t fhb_ffn_workspace_bytes(const fhb_ffn_problem* problem, int pass);
 /*
  * y [tokens][out_width], contiguous. `saved` (fhb_ffn_saved_bytes bytes, 128-byte aligned)
  * is filled for fhb_ffn_backward, or NULL where no gradient is wanted. Workspaces of these

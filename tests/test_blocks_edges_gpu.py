@@ -373,3 +373,48 @@ def test_scales_of_a_bfloat16_trunk_move(bits):
         optimizer.step()
         for s, b in zip(trunk.scale, before):
             assert s.dtype == torch.float32 and 0 < float((s - b).abs()) <= 1.1e-3
+
+
+# ---- memory ----
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_workspaces_hold_what_is_written(dtype):
+    """Without gradients a call needs h, and with them nothing that it keeps; the calls stay inside
+    what they ask for."""
+    tokens, width, hidden = 4096, 256, 1024
+    tensors = [torch.randn(s, device="cuda").mul_(0.05).to(dtype)
+               for s in ((tokens, width), (hidden, width), (hidden, width), (width, hidden))]
+    problem = _native.FfnProblem(
+        tokens=tokens, width=width, hidden=hidden, out_width=width, dtype=int(dtype == torch.bfloat16),
+        activation=1, x=tensors[0].data_ptr(), w_gate=tensors[1].data_ptr(), w_up=tensors[2].data_ptr(),
+        w_down=tensors[3].data_ptr(), x_stride=width, w_gate_stride=width, w_up_stride=width,
+        w_down_stride=hidden)
+    library, at = _native.library(), ctypes.byref(problem)
+    value = 6 if dtype == torch.float32 else 2  # bytes of an operand's value
+    packed = 6 * sum(t.numel() for t in tensors) if dtype == torch.float32 else 0
+    h = tokens * hidden * value
+    plain, saving = (library.fhb_ffn_workspace_bytes(at, k) for k in (0, 2))
+    parts = plain - packed - h  # FP32 sums of parts of K, if any
+    assert 0 <= parts <= 8 * tokens * width * 4 and saving == plain - h
+    assert library.fhb_ffn_workspace_bytes(at, 3) == library.fhb_ffn_workspace_bytes(at, -1) == 0
+    with torch.no_grad():
+        want = fused_hoad.gated_feed_forward(*tensors)
+    stream = torch.cuda.current_stream().cuda_stream
+    for size, keeps in ((plain, 0), (saving, library.fhb_ffn_saved_bytes(at))):
+        room, saved = (torch.full((n + 4096,), 77, device="cuda", dtype=torch.uint8) for n in (size, keeps))
+        y = torch.empty_like(want)
+        place = saved.data_ptr() if keeps else None
+        assert library.fhb_ffn_forward(at, y.data_ptr(), place, room.data_ptr(), max(size - 1, 0), stream) in (
+            (3,) if size else (0,))
+        assert library.fhb_ffn_forward(at, y.data_ptr(), place, room.data_ptr(), size, stream) == 0
+        assert torch.equal(y, want)
+        assert (room[size:] == 77).all() and (saved[keeps:] == 77).all()
+    # the same through the call with gradients: its peak is y, what it keeps and the workspace
+    leaf = tensors[0].clone().requires_grad_()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    y = fused_hoad.gated_feed_forward(leaf, *tensors[1:])
+    grown = torch.cuda.max_memory_allocated() - before
+    assert grown <= y.numel() * y.element_size() + library.fhb_ffn_saved_bytes(at) + saving + 2**21
