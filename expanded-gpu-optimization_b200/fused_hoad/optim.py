@@ -96,7 +96,7 @@ class AdamW(torch.optim.Optimizer):
                         weight_decay=float(weight_decay), state_bits=state_bits, capturable=True)
         super().__init__(params, defaults)
 
-    def _new_state(self, p: Tensor, state_bits: int, step: Tensor) -> None:
+    def _new_state(self, p: Tensor, state_bits: int, step: Tensor) -> dict:
         state = self.state[p]
         state["step"] = step
         if state_bits == 32:
@@ -107,31 +107,39 @@ class AdamW(torch.optim.Optimizer):
             for name in ("exp_avg", "exp_avg_sq"):
                 state[name] = torch.zeros_like(p, dtype=torch.float8_e4m3fn)
                 state[name + "_scale"] = torch.zeros(blocks, device=p.device)
+        return state
 
-    def _by_counter(self, group: dict) -> list[tuple[Tensor, list[Tensor]]]:
-        """The parameters with a gradient, by the step counter that they share. Those that share
-        one with a parameter that has none now get a counter of their own."""
-        params = [p for p in group["params"] if p.grad is not None]
-        new = [p for p in params if not self.state.get(p)]
-        idle = {id(self.state[p]["step"]) for p in group["params"] if p.grad is None and self.state.get(p)}
-        if new:
+    def _by_counter(self, group: dict) -> list[tuple[list[Tensor], list[Tensor], list[dict]]]:
+        """(parameters, gradients, states) for each step counter that parameters with a gradient
+        share. Those that share one with a parameter that has none now get one of their own."""
+        shared: dict[int, tuple[list[Tensor], list[Tensor], list[dict]]] = {}
+        idle = set()
+        fresh = None
+        for p in group["params"]:
+            state, grad = self.state.get(p), p.grad
+            if grad is None:
+                if state:
+                    idle.add(id(state["step"]))
+                continue
+            if not state:
+                if fresh is None:
+                    _refuse_capture(p)
+                    fresh = torch.zeros(1, dtype=torch.int64, device=p.device)
+                state = self._new_state(p, group["state_bits"], fresh)
+            key = id(state["step"])
+            if key not in shared:
+                shared[key] = ([], [], [])
+            params, grads, states = shared[key]
+            params.append(p)
+            grads.append(grad.contiguous())
+            states.append(state)
+        for key in idle & shared.keys():
+            params, _, states = shared[key]
             _refuse_capture(params[0])
-            counter = torch.zeros(1, dtype=torch.int64, device=params[0].device)
-            for p in new:
-                self._new_state(p, group["state_bits"], counter)
-        shared: dict[int, tuple[Tensor, list[Tensor]]] = {}
-        for p in params:
-            counter = self.state[p]["step"]
-            shared.setdefault(id(counter), (counter, []))[1].append(p)
-        result = []
-        for key, (counter, members) in shared.items():
-            if key in idle:
-                _refuse_capture(params[0])
-                counter = counter.clone()
-                for p in members:
-                    self.state[p]["step"] = counter
-            result.append((counter, members))
-        return result
+            own = states[0]["step"].clone()
+            for state in states:
+                state["step"] = own
+        return list(shared.values())
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -140,15 +148,14 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
-            for counter, params in self._by_counter(group):
-                states = [self.state[p] for p in params]
+            for params, grads, states in self._by_counter(group):
                 scales = {}
                 if group["state_bits"] == 8:
                     scales = {"exp_avg_scales": [s["exp_avg_scale"] for s in states],
                               "exp_avg_sq_scales": [s["exp_avg_sq_scale"] for s in states]}
                 adamw_step(
-                    params, [p.grad.contiguous() for p in params], [s["exp_avg"] for s in states],
-                    [s["exp_avg_sq"] for s in states], counter, lr=group["lr"],
+                    params, grads, [s["exp_avg"] for s in states],
+                    [s["exp_avg_sq"] for s in states], states[0]["step"], lr=group["lr"],
                     betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                     **scales,
                 )
