@@ -274,7 +274,7 @@ size_t ffn_workspace_bytes(const fhb_ffn_problem& p, int pass, const DeviceInfo&
     const Saved s = saved_in(p, keep ? aside : room, keep);
     const TcProduct down = down_product(p, o, s, nullptr);
     room.take(gemm_tc_workspace_bytes(&down, 1, dev));
-    return keep ? room.used : std::max(room.used, ffn_small_bytes(p));
+    return !keep && ffn_takes_small(p) ? ffn_small_bytes(p) : room.used;
   }
   // the upstream gradient may need a copy: the size asked for does not depend on it
   inputs_in(p, nullptr, 0, room, o);
@@ -289,7 +289,7 @@ size_t ffn_workspace_bytes(const fhb_ffn_problem& p, int pass, const DeviceInfo&
 
 cudaError_t launch_ffn_forward(const fhb_ffn_problem& p, void* y, void* saved, void* workspace,
                                const DeviceInfo& dev, cudaStream_t stream) {
-  if (saved == nullptr && p.tokens <= ffn_small_tokens(p.dtype))
+  if (saved == nullptr && ffn_takes_small(p))
     return launch_ffn_small(p, y, workspace, dev, stream);
   Room room{static_cast<char*>(workspace)}, kept{static_cast<char*>(saved)};
   Operands o;

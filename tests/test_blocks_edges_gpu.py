@@ -418,3 +418,18 @@ def test_workspaces_hold_what_is_written(dtype):
     y = fused_hoad.gated_feed_forward(leaf, *tensors[1:])
     grown = torch.cuda.max_memory_allocated() - before
     assert grown <= y.numel() * y.element_size() + library.fhb_ffn_saved_bytes(at) + saving + 2**21
+
+
+@pytest.mark.parametrize("tokens,width,hidden", [(1, 1024, 8000), (1, 4096, 6000), (1, 4096, 6200),
+                                                 (2, 4096, 3000), (2, 4096, 3200), (3, 1024, 512)])
+def test_few_tokens_on_both_sides_of_the_dot_products(tokens, width, hidden):
+    """bfloat16: the dot products' limit of tokens times weights lies between the sizes."""
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    x, wg, wu, wd = ((torch.randn(s, generator=g, device="cuda") * s[-1] ** -0.5).bfloat16()
+                     for s in ((tokens, width), (hidden, width), (hidden, width), (width, hidden)))
+    x = x * width**0.5
+    with torch.no_grad():
+        y = fused_hoad.gated_feed_forward(x, wg, wu, wd)
+    want = ffn(x.double(), wg.double(), wu.double(), wd.double())
+    rms = torch.full_like(want, float(want.square().mean().sqrt()))
+    assert_near(y, want, tolerance(torch.bfloat16, hidden), "y", rms)
