@@ -13,9 +13,12 @@
 // registers. A row is spread over 8, 16 or 32 lanes of a warp (32 to 8 rows a CTA), or over one
 // CTA, eight values a thread; a thread keeps its columns' weights, and in the backward the sums
 // of its columns, from row to row. The column sums end in a second kernel, in a fixed order.
-// 16,384 x 2048 with an fp32 residual, a bf16 branch and 16 gates: forward 75 us (402 MB, 5.4 TB/s),
-// backward 120 us (604 MB, 5.0 TB/s: ten registers a value leave an SM two rows at a time, and
-// the sums' barriers show) and 5 us for the column sums.
+// 16,384 x 2048 with an fp32 residual, a bf16 branch and 16 gates: forward 75.5 us (402 MB, 5.3 TB/s),
+// backward 121 us (604 MB, 5.0 TB/s: ten registers a value leave an SM two rows at a time, and the
+// sums' barriers show), 5 us of them for the column sums. Rows wider than 4,096 have 1,024 threads, whose
+// 64 registers do not hold the backward's values: it spills 0.3 KB a thread up to 8,192 and over 3 KB
+// above (4,096 x 8,192 bf16: forward 61.5 us, 4.4 TB/s, backward 200 us, 2.0 TB/s; 1,600 x 20,000: 160
+// and 1,160 us).
 #include <algorithm>
 #include <atomic>
 
